@@ -30,6 +30,10 @@ extern "C" {
 #define DG_EHIP (-4)      /* a HIP runtime call / launch failed */
 #define DG_ERCCL (-5)     /* RCCL could not be bound (librccl.so absent) or one of its calls failed */
 
+#define DG_F32 0  /* types of the RoI head's operators */
+#define DG_BF16 1
+#define DG_F16 2
+
 #define DG_POOL_AVG 0 /* rcnn/fast_rcnn.py:354 as written (AdaptiveAvgPool2d) */
 #define DG_POOL_MAX 1 /* north_star: max + argmax */
 
@@ -323,6 +327,36 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
                   int64_t n_det, const int32_t *tgt_img, const int32_t *tgt_cls, const float *tgt_box, int64_t n_tgt,
                   int64_t n_classes, int64_t n_images, float iou_thr, double *ap_out, int32_t *n_grt, void *ws,
                   size_t ws_bytes, dg_stream_t s);
+
+/* ---------------------------------------------------------------- the RoI head: attention over an image's boxes or cells
+ * NO COUNTERPART IN THE REFERENCE (its Fast R-CNN sketch classifies every RoI by itself, rcnn/fast_rcnn.py:379-384).
+ * q (batch, nq, q_heads, d), k and v (batch, nk, k_heads, d): strides of the first three axes in values, the last axis dense;
+ * pointers and strides multiples of 16 bytes.  Query head h reads key head h / (q_heads / k_heads).  Types: DG_F32, DG_BF16 (one
+ * for all of q, k, v, out and the gradients).  d: a multiple of 8 from 8 to 128.
+ *   s_ij = scale * q_i . k_j,  p_i = softmax over the keys that row i may see,  out_i = sum_j p_ij v_j,  lse_i = log sum_j exp s_ij
+ * A row i sees key j if i < q_counts[image], j < k_counts[image] (device int32, held to [0, n]; NULL = all) and mask[image][i][j] != 0
+ * (device bytes, batch and row stride in bytes -- a batch stride of 0 shares one mask; NULL = all).  What lies behind a count is
+ * never read.  A row that sees nothing gives out = 0, lse = -inf and has no gradient; so do the rows behind q_counts, and dk = dv = 0
+ * behind k_counts: every element of every output is written.  With a mask, a key that a row may not see does not reach it whatever
+ * its values are; a row that sees a key or value holding a NaN or an infinity (and with a mask, in the backward pass, a row
+ * holding one in q or grad_out) gives NaN.
+ * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
+ * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products.  Results are the
+ * same in every run (no atomics). */
+typedef struct dg_attn_shape {   /* host */
+    int64_t batch, nq, nk, q_heads, k_heads, d;
+    int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3];   /* batch, row, head; g: of grad_out (backward) */
+    int64_t mask_stride[2];                                       /* batch, row */
+    float scale;                                                  /* positive, finite */
+    int32_t dtype;
+} dg_attn_shape;
+size_t dg_roi_attn_workspace_bytes(const dg_attn_shape *shape, int backward);
+int dg_roi_attn_fwd(const dg_attn_shape *shape, const void *q, const void *k, const void *v, const int32_t *q_counts,
+                    const int32_t *k_counts, const uint8_t *mask, void *out, float *lse, void *ws, size_t ws_bytes, dg_stream_t s);
+/* out, lse: what the forward pass gave for the same inputs.  dq == NULL, or dk and dv both NULL: not computed */
+int dg_roi_attn_bwd(const dg_attn_shape *shape, const void *grad_out, const void *q, const void *k, const void *v, const void *out,
+                    const float *lse, const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv,
+                    void *ws, size_t ws_bytes, dg_stream_t s);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,808 @@
+// attention.hip — attention over padded sets of RoIs or map cells, forward and backward, on the matrix cores.
+//
+//   s_ij = scale * q_i . k_j over the keys j that row i may see,  l_i = log sum_j exp s_ij,  p_ij = exp(s_ij - l_i)
+//   o_i = sum_j p_ij v_j
+//   delta_i = do_i . o_i,  dp_ij = do_i . v_j,  ds_ij = p_ij (dp_ij - delta_i)
+//   dv_j = sum_i p_ij do_i,  dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//
+// The backward pass recomputes p from q, k and l; nothing of size rows x keys is ever stored.  dq and (dk, dv) come from two
+// kernels, each of which owns its outputs: two products of seven are computed twice, but there are no atomics and the result
+// has the same bits in every run.  Query heads that share a key head are laid out as one list of rows (row r = head r / n of
+// the group, query r % n), so a key tile is read once for all of them and their gradients add up in registers.
+//
+// Layout of the 32x32 matrix instruction's result: lane l holds column l & 31 and rows 8 (r / 4) + 4 (l / 32) + r % 4.  The
+// products are arranged so that the column is what the statistics belong to (S^T = K Q^T in the forward and dq kernels: one
+// query per lane) and so that a result feeds the next product as its second operand without moving between lanes: the
+// contraction index may be permuted as long as the first operand, read transposed from LDS, is permuted the same way.
+#include "common.hpp"
+#include <math.h>
+
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+
+#define AT_THREADS 256
+#define AT_WAVES 4
+#define AT_LOG2E 1.4426950408889634f
+#define AT_LN2 0.6931471805599453f
+
+template <typename T> struct at_vec;
+template <> struct at_vec<__bf16> { typedef bf16x8 frag; typedef bf16x4 quad; };
+template <> struct at_vec<float> { typedef f32x4 frag; typedef f32x4 quad; };
+
+// a block of contraction values: 16 bytes per lane of each operand, lanes 0..31 the first chunk, lanes 32..63 the second
+__device__ __forceinline__ f32x16 at_mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 at_mma(f32x4 a, f32x4 b, f32x16 c)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ float at_xor32(float v) { return __shfl_xor(v, 32, 64); }
+
+// A tile of rows in LDS, DP values wide, in 16-byte chunks whose place inside the row is swizzled by the row: eight lanes
+// reading the same chunk of eight successive rows, and sixteen lanes reading two chunks of four successive rows (the
+// transposing read), both cover 128 different bytes modulo 128.
+template <typename T, int DP> struct at_tile {
+    static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16;
+    static __device__ __forceinline__ int swz(int row) { return CPR >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : ((row & 2) | ((row >> 2) & 1)); }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
+    // rows of the tile as an operand: row l & 31, chunk 2 g + l / 32
+    static __device__ __forceinline__ typename at_vec<T>::frag row_frag(const char *t, int row, int chunk)
+    {
+        return *(const typename at_vec<T>::frag *)(t + at(row, chunk));
+    }
+};
+
+// acc[db] (32 values of d x 32 columns) += tile[rows base..base+31][d]^T * w, w in the result layout (rows = the tile's rows)
+template <int DP> __device__ __forceinline__ void at_acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane, const __bf16 *)
+{
+    typedef at_tile<__bf16, DP> tile;
+    const int h = lane >> 5, j = lane & 15, row0 = base + 4 * h + (j >> 2), part = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const f32x8 ws = s ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
+        const bf16x8 b = __builtin_convertvector(ws, bf16x8);       // one rounding to 8 bits; the sum stays in 32
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            typedef __attribute__((address_space(3))) s16x4 *lp;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + tile::at(row0 + 16 * s, db * 4 + part) + (j & 1) * 8));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + tile::at(row0 + 16 * s + 8, db * 4 + part) + (j & 1) * 8));
+            const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            acc[db] = at_mma(a, b, acc[db]);
+        }
+    }
+}
+template <int DP> __device__ __forceinline__ void at_acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane, const float *)
+{
+    typedef at_tile<float, DP> tile;
+    const int h = lane >> 5, d = lane & 31;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = base + 8 * (r >> 2) + 4 * h + (r & 3);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            const float a = *(const float *)(t + tile::at(row, db * 8 + (d >> 2)) + (d & 3) * 4);
+            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], acc[db], 0, 0, 0);
+        }
+    }
+}
+
+// what a call is made of, on the device's side
+template <typename T> struct at_args {
+    const T *q, *k, *v, *g;                       // g: gradient of the output (backward)
+    T *o, *dk;                                    // o: output / dq; dk, dv
+    T *dv;
+    float *lse;                                   // forward: output (b, hq, nq)
+    const float *lse2, *delta;                    // backward: statistics of the rows, base 2, (b, hq, nq)
+    float *part;                                  // partial results of a split call
+    const int32_t *qc, *kc;
+    const uint8_t *mask;
+    int64_t qs[3], ks[3], vs[3], gs[3];           // strides of batch, row, head, in values
+    int64_t ms[2];                                // mask: batch, row
+    int nq, nk, hq, hk, d, tiles, splits, per;    // per: rows or keys of a split, a multiple of the tile
+    float c, scale;                               // c = scale * log2(e)
+};
+
+__device__ __forceinline__ int at_count(const int32_t *c, int b, int n) { return c ? min(max(c[b], 0), n) : n; }
+
+// workgroups go round the eight XCDs; this gives each XCD a run of successive ids, so the tiles that read the same keys meet
+// in one L2
+__device__ __forceinline__ int at_xcd_id()
+{
+    const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
+    return x * q + min(x, r) + (int)(blockIdx.x >> 3);
+}
+
+template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p) { return *(const u32x4 *)p; }
+
+// with a pair mask, a row of K, V, Q or dO that some rows may not see must not reach them through 0 * NaN: non-finite values
+// are put to zero in the staged copy, and the caller marks the row so that those who do see it get NaN
+template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
+{
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (sizeof(T) == 2) {
+            const bool lo = (x[i] & 0x7f80u) == 0x7f80u, hi = (x[i] & 0x7f800000u) == 0x7f800000u;
+            if (lo) x[i] &= 0xffff0000u;
+            if (hi) x[i] &= 0x0000ffffu;
+            bad |= lo | hi;
+        } else {
+            const bool b = (x[i] & 0x7f800000u) == 0x7f800000u;
+            if (b) x[i] = 0;
+            bad |= b;
+        }
+    }
+    return bad;
+}
+#define AT_NAN4 ((u32x4){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu})   // NaN in bf16 and in fp32
+
+// ------------------------------------------------------------------ forward
+// A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of 64.  K and V tiles are double
+// buffered in LDS; the next tile's global loads are in flight while this one is computed.
+template <typename T, int DP> struct at_shape { static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32; };   // fp32 x 128: 64 KB of LDS
+
+template <typename T, int DP, bool MASK>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_fwd(const at_args<T> a)
+{
+    typedef at_tile<T, DP> tile;
+    typedef typename at_vec<T>::frag frag;
+    typedef typename at_vec<T>::quad quad;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U;
+    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+
+    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
+    const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+
+    if (sp == 0) {                                // rows behind the image's last one: nothing seen
+        const int pad = a.nq - nq;
+        for (int p = tix; p < G * pad; p += a.tiles) {
+            const int hq = hk * G + p / pad, n = nq + p % pad;
+            T *o = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
+            for (int d = threadIdx.x; d < a.d; d += AT_THREADS) o[d] = (T)0.f;
+            if (threadIdx.x == 0) a.lse[((int64_t)b * a.hq + hq) * a.nq + n] = -INFINITY;
+        }
+    }
+    if (tix * 32 * AT_WAVES >= R) return;
+
+    const int r = (tix * AT_WAVES + wave) * 32 + (lane & 31);
+    const bool live = r < R;
+    const int gh = live ? r / nq : 0, n = live ? r % nq : 0, hq = hk * G + gh;
+    const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2];
+    frag qf[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int d = (2 * g + h) * CH;
+        qf[g] = (live && d < a.d) ? *(const frag *)(qp + d) : (frag)(0.f);
+    }
+    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
+
+    const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
+    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
+    const bool cin = c16 * CH < a.d;
+    const T *kp = a.k + b * a.ks[0] + hk * a.ks[2] + c16 * CH, *vp = a.v + b * a.vs[0] + hk * a.vs[2] + c16 * CH;
+    u32x4 kr[NL], vr[NL];
+    auto load = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int key = kb + srow + i * STEP;
+            const bool in = cin && key < k1;
+            kr[i] = in ? at_load_chunk(kp + key * a.ks[1]) : (u32x4)(0u);
+            vr[i] = in ? at_load_chunk(vp + key * a.vs[1]) : (u32x4)(0u);
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int row = srow + i * STEP;
+            if (MASK && at_scrub<T>(vr[i])) kr[i] = AT_NAN4;    // scores of that key become NaN for the rows that see it
+            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = kr[i];
+            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = vr[i];
+        }
+    };
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
+    float m = -INFINITY, l = 0.f;                 // running maximum (of s / scale) and this lane's part of the sum
+
+    if (k0 < k1) {
+        load(k0);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
+        const bool more = kb + KT < k1;
+        if (more) load(kb + KT);
+        const char *K = lds[buf][0], *V = lds[buf][1];
+        f32x16 s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            s[u] = (f32x16)(0.f);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) s[u] = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s[u]);
+        }
+        if (MASK || !more) {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = kb + u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    const bool see = key < k1 && (!MASK || mp[key] != 0);
+                    s[u][e] = see ? s[u][e] : -INFINITY;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int e = 1; e < 16 * U; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
+        mx = fmaxf(mx, at_xor32(mx));
+        const float mn = fmaxf(m, mx);
+        if (__any(mn > m)) {
+            const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+            l *= al;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) o[i] *= al;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : m * a.c;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[u][e], a.c, -base));
+                s[u][e] = p;
+                l += p;
+            }
+            at_acc_t<DP>(o, V, u * 32, s[u], lane, (const T *)nullptr);
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    l += at_xor32(l);
+    if (!live) return;
+    const bool none = m == -INFINITY && !(l != l);
+    const float inv = none ? 0.f : 1.f / l;
+    const float lse2 = none ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l));
+    if (a.splits > 1) {
+        // partial result of the split: normalised values and their log-sum, joined by k_attn_join
+        const int64_t row = ((int64_t)bh * G + gh) * a.nq + n, rows = (int64_t)(gridDim.x / a.tiles / a.splits) * G * a.nq;
+        float *po = a.part + rows * a.splits + (row * a.splits + sp) * a.d;
+        if (h == 0) a.part[row * a.splits + sp] = lse2;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = i * 32 + 2 * e + 4 * h;
+                if (d < a.d) *(f32x4 *)(po + d) = (f32x4){o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv};
+            }
+        return;
+    }
+    T *op = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
+    if (h == 0) a.lse[((int64_t)b * a.hq + hq) * a.nq + n] = lse2 * AT_LN2;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = i * 32 + 2 * e + 4 * h;
+            if (d < a.d)
+                *(quad *)(op + d) = __builtin_convertvector(((f32x4){o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv}), quad);
+        }
+}
+
+// joins the splits of a row: one wave per row
+template <typename T>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, int64_t rows)
+{
+    const int64_t row = (int64_t)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (row >= rows) return;
+    const int n = (int)(row % a.nq), hq = (int)(row / a.nq % a.hq), b = (int)(row / a.nq / a.hq);
+    if (n >= at_count(a.qc, b, a.nq)) return;     // written by the first kernel
+    const float *ls = a.part + row * a.splits, *po = a.part + rows * a.splits + row * a.splits * a.d;
+    float m = -INFINITY;
+    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ls[s]);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    const float base = m == -INFINITY ? 0.f : m;
+    float tot = 0.f;
+    for (int s = lane; s < a.splits; s += 64) tot += __builtin_amdgcn_exp2f(ls[s] - base);
+#pragma unroll
+    for (int x = 32; x; x >>= 1) tot += __shfl_xor(tot, x, 64);
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
+    for (int d = lane; d < a.d; d += 64) {
+        float v = 0.f;
+        for (int s = 0; s < a.splits; ++s) v = fmaf(__builtin_amdgcn_exp2f(ls[s] - base), po[(int64_t)s * a.d + d], v);
+        a.o[(((int64_t)b * a.nq + n) * a.hq + hq) * a.d + d] = (T)(v * inv);
+    }
+    if (lane == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
+}
+
+// ------------------------------------------------------------------ backward
+// delta_i = do_i . o_i and the rows' log-sums in base 2; a row that sees nothing gets +inf there, so that its p is 0
+template <typename T, bool MASK>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, const T *__restrict__ out, const float *__restrict__ lse, float *__restrict__ lse2,
+                                                           float *__restrict__ delta, int64_t rows)
+{
+    constexpr int CH = 16 / (int)sizeof(T), LPR = 128 / CH, RPB = AT_THREADS / LPR;
+    const int sub = threadIdx.x % LPR;
+    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;     // (b, n, hq), heads innermost as in memory
+    if (row >= rows) return;
+    const int hq = (int)(row % a.hq), n = (int)(row / a.hq % a.nq), b = (int)(row / a.hq / a.nq);
+    const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
+    const bool live = n < at_count(a.qc, b, a.nq);
+    float sum = 0.f;
+    int bad = 0;
+    const int d = sub * CH;
+    if (live && d < a.d) {
+        const typename at_vec<T>::frag x = *(const typename at_vec<T>::frag *)(a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2] + d);
+        const typename at_vec<T>::frag y = *(const typename at_vec<T>::frag *)(out + row * a.d + d);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) sum = fmaf((float)x[i], (float)y[i], sum);
+        if (MASK) {
+            u32x4 xs = __builtin_bit_cast(u32x4, x), qs = at_load_chunk(a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2] + d);
+            bad = (int)at_scrub<T>(xs) | (int)at_scrub<T>(qs);
+        }
+    }
+#pragma unroll
+    for (int x = LPR / 2; x; x >>= 1) {
+        sum += __shfl_xor(sum, x, 64);
+        if (MASK) bad |= __shfl_xor(bad, x, 64);
+    }
+    if (sub) return;
+    const float l = live ? lse[at] : -INFINITY;
+    lse2[at] = bad ? __builtin_nanf("") : l == -INFINITY ? INFINITY : l * AT_LOG2E;
+    delta[at] = sum;
+}
+
+// dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp)
+template <typename T, int DP, bool MASK>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_dq(const at_args<T> a)
+{
+    typedef at_tile<T, DP> tile;
+    typedef typename at_vec<T>::frag frag;
+    typedef typename at_vec<T>::quad quad;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U;
+    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+
+    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
+    const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+
+    if (sp == 0) {
+        const int pad = a.nq - nq;
+        for (int p = tix; p < G * pad; p += a.tiles) {
+            T *o = a.o + (((int64_t)b * a.nq + nq + p % pad) * a.hq + hk * G + p / pad) * a.d;
+            for (int d = threadIdx.x; d < a.d; d += AT_THREADS) o[d] = (T)0.f;
+        }
+    }
+    if (tix * 32 * AT_WAVES >= R) return;
+
+    const int r = (tix * AT_WAVES + wave) * 32 + (lane & 31);
+    const bool live = r < R;
+    const int gh = live ? r / nq : 0, n = live ? r % nq : 0, hq = hk * G + gh;
+    const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2], *gp = a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2];
+    frag qf[NG], gf[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int d = (2 * g + h) * CH;
+        const bool in = live && d < a.d;
+        qf[g] = in ? *(const frag *)(qp + d) : (frag)(0.f);
+        gf[g] = in ? *(const frag *)(gp + d) : (frag)(0.f);
+    }
+    const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
+    const float lse2 = live ? a.lse2[at] : INFINITY, delta = live ? a.delta[at] : 0.f;
+    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
+
+    const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
+    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
+    const bool cin = c16 * CH < a.d;
+    const T *kp = a.k + b * a.ks[0] + hk * a.ks[2] + c16 * CH, *vp = a.v + b * a.vs[0] + hk * a.vs[2] + c16 * CH;
+    u32x4 kr[NL], vr[NL];
+    auto load = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int key = kb + srow + i * STEP;
+            const bool in = cin && key < k1;
+            kr[i] = in ? at_load_chunk(kp + key * a.ks[1]) : (u32x4)(0u);
+            vr[i] = in ? at_load_chunk(vp + key * a.vs[1]) : (u32x4)(0u);
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int row = srow + i * STEP;
+            if (MASK && at_scrub<T>(kr[i])) vr[i] = AT_NAN4;    // dp of that key becomes NaN
+            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = kr[i];
+            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = vr[i];
+        }
+    };
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
+    if (k0 < k1) {
+        load(k0);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
+        const bool more = kb + KT < k1;
+        if (more) load(kb + KT);
+        const char *K = lds[buf][0], *V = lds[buf][1];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            f32x16 s = (f32x16)(0.f), dp = (f32x16)(-delta);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                s = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
+                dp = at_mma(tile::row_frag(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse2)) * dp[e];
+                if (MASK || !more) {
+                    const int key = kb + u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+                    ds = key < k1 && (!MASK || mp[key] != 0) ? ds : 0.f;
+                }
+                s[e] = ds;
+            }
+            at_acc_t<DP>(o, K, u * 32, s, lane, (const T *)nullptr);
+        }
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    if (!live) return;
+    float *po = a.part + (((int64_t)bh * G + gh) * a.nq + n) * a.splits * a.d + (int64_t)sp * a.d;
+    T *op = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = i * 32 + 2 * e + 4 * h;
+            const f32x4 x = (f32x4){o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]} * a.scale;
+            if (d >= a.d) continue;
+            if (a.splits > 1) *(f32x4 *)(po + d) = x;
+            else *(quad *)(op + d) = __builtin_convertvector(x, quad);
+        }
+}
+
+// dk, dv: a workgroup owns 128 keys (a wave: 32, one per lane pair) and walks the rows; Q and dO tiles are read as rows (scores,
+// dp) and transposed (dk, dv)
+template <typename T, int DP, bool MASK>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_dkv(const at_args<T> a)
+{
+    typedef at_tile<T, DP> tile;
+    typedef typename at_vec<T>::frag frag;
+    typedef typename at_vec<T>::quad quad;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = 32;
+    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP > 0 ? KT / STEP : 1;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+    __shared__ __attribute__((aligned(16))) float st[2][2][KT];
+    __shared__ int mrow[2][KT];
+
+    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
+    const int R = tix * 32 * AT_WAVES < nk ? G * nq : 0;         // a tile of keys behind the image's last one: zeros
+    const int key = (tix * AT_WAVES + wave) * 32 + (lane & 31);
+    const bool live = key < nk;
+
+    const T *kp = a.k + b * a.ks[0] + (live ? key : 0) * a.ks[1] + hk * a.ks[2], *vp = a.v + b * a.vs[0] + (live ? key : 0) * a.vs[1] + hk * a.vs[2];
+    frag kf[NG], vf[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        const int d = (2 * g + h) * CH;
+        const bool in = live && d < a.d;
+        kf[g] = in ? *(const frag *)(kp + d) : (frag)(0.f);
+        vf[g] = in ? *(const frag *)(vp + d) : (frag)(0.f);
+    }
+    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + key : nullptr;
+
+    const int r0 = min(R, sp * a.per), r1 = min(R, r0 + a.per);
+    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
+    const bool cin = c16 * CH < a.d, sin = KT >= STEP || srow < KT;
+    const T *qp = a.q + b * a.qs[0] + c16 * CH, *gp = a.g + b * a.gs[0] + c16 * CH;
+    u32x4 qr[NL], gr[NL];
+    float str = 0.f;
+    int mr = 0;
+    auto load = [&](int rb) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int r = rb + srow + i * STEP;
+            const bool in = cin && sin && r < r1;
+            const int gh = G == 1 ? 0 : r / nq, n = r - gh * nq, hq = hk * G + gh;
+            qr[i] = in ? at_load_chunk(qp + n * a.qs[1] + hq * a.qs[2]) : (u32x4)(0u);
+            gr[i] = in ? at_load_chunk(gp + n * a.gs[1] + hq * a.gs[2]) : (u32x4)(0u);
+        }
+        if (threadIdx.x < 2 * KT) {               // the rows' statistics: first half log-sums, second half deltas
+            const int r = rb + (threadIdx.x & (KT - 1)), second = threadIdx.x >= KT;
+            const int gh = G == 1 ? 0 : r / nq, n = r - gh * nq;
+            const int64_t at = ((int64_t)b * a.hq + hk * G + gh) * a.nq + n;
+            str = r < r1 ? (second ? -a.delta[at] : a.lse2[at]) : (second ? 0.f : INFINITY);
+            mr = r < r1 ? n : 0;
+        }
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            if (!sin) break;
+            const int row = srow + i * STEP;
+            if (MASK) {                           // the row's log-sum already says NaN (k_attn_delta)
+                at_scrub<T>(qr[i]);
+                at_scrub<T>(gr[i]);
+            }
+            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = qr[i];
+            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = gr[i];
+        }
+        if (threadIdx.x < 2 * KT) st[buf][threadIdx.x / KT][threadIdx.x & (KT - 1)] = str;
+        if (MASK && threadIdx.x < KT) mrow[buf][threadIdx.x] = mr;
+    };
+
+    f32x16 ok[NB], ov[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) ok[i] = ov[i] = (f32x16)(0.f);
+    if (r0 < r1) {
+        load(r0);
+        store(0);
+    }
+    __syncthreads();
+    int buf = 0;
+    for (int rb = r0; rb < r1; rb += KT, buf ^= 1) {
+        const bool more = rb + KT < r1;
+        if (more) load(rb + KT);
+        const char *Q = lds[buf][0], *GO = lds[buf][1];
+        f32x16 s = (f32x16)(0.f), dp, ls;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const f32x4 x = *(const f32x4 *)&st[buf][0][2 * e + 4 * h], y = *(const f32x4 *)&st[buf][1][2 * e + 4 * h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { ls[e + i] = x[i]; dp[e + i] = y[i]; }
+        }
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            s = at_mma(tile::row_frag(Q, lane & 31, 2 * g + h), kf[g], s);
+            dp = at_mma(tile::row_frag(GO, lane & 31, 2 * g + h), vf[g], dp);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -ls[e]));
+            float ds = p * dp[e];
+            if (MASK) {
+                const int row = 8 * (e >> 2) + 4 * h + (e & 3);
+                const bool see = live && rb + row < r1 && mp[mrow[buf][row] * a.ms[1]] != 0;
+                p = see ? p : 0.f;
+                ds = see ? ds : 0.f;
+            }
+            s[e] = p;
+            dp[e] = ds;
+        }
+        at_acc_t<DP>(ov, GO, 0, s, lane, (const T *)nullptr);
+        at_acc_t<DP>(ok, Q, 0, dp, lane, (const T *)nullptr);
+        if (more) store(buf ^ 1);
+        __syncthreads();
+    }
+    if (key >= a.nk) return;
+    const int64_t rows = (int64_t)(gridDim.x / a.tiles / a.splits) * a.nk, prow = (int64_t)bh * a.nk + key;
+    float *pk = a.part + prow * a.splits * a.d + (int64_t)sp * a.d, *pv = pk + rows * a.splits * a.d;
+    const int64_t orow = (((int64_t)b * a.nk + key) * a.hk + hk) * a.d;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = i * 32 + 2 * e + 4 * h;
+            if (d >= a.d) continue;
+            f32x4 x = (f32x4){ok[i][e], ok[i][e + 1], ok[i][e + 2], ok[i][e + 3]} * a.scale, y = (f32x4){ov[i][e], ov[i][e + 1], ov[i][e + 2], ov[i][e + 3]};
+            if (!live) x = y = (f32x4)(0.f);
+            if (a.splits > 1) {
+                *(f32x4 *)(pk + d) = x;
+                *(f32x4 *)(pv + d) = y;
+            } else {
+                *(quad *)(a.dk + orow + d) = __builtin_convertvector(x, quad);
+                *(quad *)(a.dv + orow + d) = __builtin_convertvector(y, quad);
+            }
+        }
+}
+
+// sums a gradient's splits in their order: rows (b, h, n) of the partial sums -> (b, n, h); rows behind a count are left alone
+template <typename T>
+__global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict__ part, T *__restrict__ out, const int32_t *__restrict__ counts, int64_t rows, int heads,
+                                                         int nmax, int d, int splits)
+{
+    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x, row = i / d;
+    if (row >= rows) return;
+    const int x = (int)(i - row * d), n = (int)(row % nmax), hh = (int)(row / nmax % heads), b = (int)(row / nmax / heads);
+    if (n >= at_count(counts, b, nmax)) return;
+    const float *p = part + row * splits * d + x;
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += p[(int64_t)s * d];
+    out[(((int64_t)b * nmax + n) * heads + hh) * d + x] = (T)v;
+}
+
+// ------------------------------------------------------------------ host
+// A call that has too few tiles to fill the chip is split along the axis it walks: enough splits for two workgroups on each of
+// the 256 CUs, none shorter than 256 steps of that axis.
+static void at_split(int64_t blocks, int64_t walk, int64_t *splits, int64_t *per)
+{
+    int64_t s = 1;
+    if (blocks < 256) s = dg_cdiv(512, blocks > 0 ? blocks : 1);
+    const int64_t most = dg_cdiv(walk, 256);
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    *per = dg_round_up(dg_cdiv(walk > 0 ? walk : 1, s), 64);
+    *splits = dg_cdiv(walk > 0 ? walk : 1, *per);
+}
+
+struct at_plan { int64_t qtiles, ktiles, qsplits, qper, ksplits, kper, rows, stats, qpart, kpart; };
+
+static at_plan at_plan_of(const dg_attn_shape *s)
+{
+    at_plan p;
+    const int64_t g = s->q_heads / s->k_heads, bh = s->batch * s->k_heads;
+    p.qtiles = dg_cdiv(g * s->nq, 32 * AT_WAVES);
+    p.ktiles = dg_cdiv(s->nk, 32 * AT_WAVES);
+    at_split(bh * p.qtiles, s->nk, &p.qsplits, &p.qper);
+    at_split(bh * p.ktiles, g * s->nq, &p.ksplits, &p.kper);
+    p.rows = s->batch * s->q_heads * s->nq;
+    p.stats = dg_round_up(p.rows * 4, 256);
+    p.qpart = p.qsplits > 1 ? p.rows * p.qsplits * s->d * 4 : 0;
+    p.kpart = p.ksplits > 1 ? 2 * s->batch * s->k_heads * s->nk * p.ksplits * s->d * 4 : 0;
+    return p;
+}
+
+static int at_check(const dg_attn_shape *s, const char *who)
+{
+    DG_REQUIRE(s, "%s: null shape", who);
+    DG_REQUIRE(s->dtype == DG_F32 || s->dtype == DG_BF16, "%s: type must be DG_F32 or DG_BF16", who);
+    DG_REQUIRE(s->batch >= 0 && s->nq >= 0 && s->nk >= 0, "%s: negative size", who);
+    DG_REQUIRE(s->k_heads >= 1 && s->q_heads >= 1 && s->q_heads % s->k_heads == 0, "%s: q_heads must be a positive multiple of k_heads", who);
+    DG_REQUIRE(s->d >= 8 && s->d <= 128 && s->d % 8 == 0, "%s: head size %lld is not a multiple of 8 from 8 to 128", who, (long long)s->d);
+    DG_REQUIRE(s->scale > 0.f && s->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
+    const int64_t most = 1ll << 28;
+    DG_REQUIRE(s->batch <= most && s->nk <= most && s->q_heads <= most && s->nq <= most && s->nq * (s->q_heads / s->k_heads) <= most &&
+                   s->batch * s->q_heads <= most, "%s: more than 2^28 rows or keys", who);
+    const at_plan p = at_plan_of(s);
+    DG_REQUIRE(s->batch * s->k_heads * p.qtiles * p.qsplits < (1ll << 31) && s->batch * s->k_heads * p.ktiles * p.ksplits < (1ll << 31) &&
+                   dg_cdiv(p.rows, 4) < (1ll << 31), "%s: more than 2^31 tiles", who);
+    return DG_OK;
+}
+
+// 16-byte loads: the pointer and every stride that a call steps along
+static bool at_aligned(const void *p, const int64_t *st, const dg_attn_shape *s, int64_t n, int64_t heads)
+{
+    const int64_t e = s->dtype == DG_F32 ? 4 : 2, dims[3] = {s->batch, n, heads};
+    if (((uintptr_t)p) & 15) return false;
+    for (int i = 0; i < 3; ++i)
+        if (dims[i] > 1 && (st[i] < 0 || st[i] * e % 16)) return false;
+    return true;
+}
+
+extern "C" size_t dg_roi_attn_workspace_bytes(const dg_attn_shape *s, int backward)
+{
+    if (at_check(s, "roi_attn") != DG_OK) return 0;
+    const at_plan p = at_plan_of(s);
+    if (!backward) return (size_t)(p.qpart ? p.qpart + p.rows * p.qsplits * 4 : 0);
+    return (size_t)(2 * p.stats + (p.qpart > p.kpart ? p.qpart : p.kpart));
+}
+
+template <typename T>
+static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *qc, const int32_t *kc, const uint8_t *mask)
+{
+    at_args<T> a = {};
+    a.q = (const T *)q; a.k = (const T *)k; a.v = (const T *)v;
+    a.qc = qc; a.kc = kc; a.mask = mask;
+    for (int i = 0; i < 3; ++i) { a.qs[i] = s->q_stride[i]; a.ks[i] = s->k_stride[i]; a.vs[i] = s->v_stride[i]; a.gs[i] = s->g_stride[i]; }
+    a.ms[0] = s->mask_stride[0]; a.ms[1] = s->mask_stride[1];
+    a.nq = (int)s->nq; a.nk = (int)s->nk; a.hq = (int)s->q_heads; a.hk = (int)s->k_heads; a.d = (int)s->d;
+    a.scale = s->scale;
+    a.c = (float)((double)s->scale * 1.4426950408889634);
+    return a;
+}
+
+#define AT_LAUNCH(kernel, grid, a)                                                                                              \
+    do {                                                                                                                        \
+        const dim3 gr_((unsigned)(grid)), bl_(AT_THREADS);                                                                       \
+        if ((a).d <= 32) { if ((a).mask) hipLaunchKernelGGL((kernel<T, 32, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 32, false>), gr_, bl_, 0, st, a); } \
+        else if ((a).d <= 64) { if ((a).mask) hipLaunchKernelGGL((kernel<T, 64, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 64, false>), gr_, bl_, 0, st, a); } \
+        else { if ((a).mask) hipLaunchKernelGGL((kernel<T, 128, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 128, false>), gr_, bl_, 0, st, a); } \
+    } while (0)
+
+template <typename T>
+static int at_forward(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *qc, const int32_t *kc, const uint8_t *mask, void *out,
+                      float *lse, void *ws, hipStream_t st)
+{
+    const at_plan p = at_plan_of(s);
+    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc, mask);
+    a.o = (T *)out; a.lse = lse; a.part = (float *)ws;
+    a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
+    AT_LAUNCH(k_attn_fwd, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
+    if (p.qsplits > 1) hipLaunchKernelGGL((k_attn_join<T>), dim3((unsigned)dg_cdiv(p.rows, AT_WAVES)), dim3(AT_THREADS), 0, st, a, p.rows);
+    DG_CHECK_LAUNCH("k_attn_fwd");
+    return DG_OK;
+}
+
+extern "C" int dg_roi_attn_fwd(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *q_counts, const int32_t *k_counts,
+                               const uint8_t *mask, void *out, float *lse, void *ws, size_t ws_bytes, dg_stream_t stream)
+{
+    const int rc = at_check(s, "roi_attn_fwd");
+    if (rc != DG_OK) return rc;
+    if (s->batch == 0 || s->nq == 0) return DG_OK;
+    DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v)), "roi_attn_fwd: null pointer");
+    DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
+                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && (((uintptr_t)out) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes");
+    const size_t need = dg_roi_attn_workspace_bytes(s, 0);
+    if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_fwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
+    DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_fwd: workspace must be 16-byte aligned");
+    return s->dtype == DG_F32 ? at_forward<float>(s, q, k, v, q_counts, k_counts, mask, out, lse, ws, (hipStream_t)stream)
+                              : at_forward<__bf16>(s, q, k, v, q_counts, k_counts, mask, out, lse, ws, (hipStream_t)stream);
+}
+
+template <typename T>
+static int at_backward(const dg_attn_shape *s, const void *g, const void *q, const void *k, const void *v, const void *out, const float *lse, const int32_t *qc,
+                       const int32_t *kc, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, hipStream_t st)
+{
+    const at_plan p = at_plan_of(s);
+    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc, mask);
+    float *lse2 = (float *)ws, *delta = (float *)((char *)ws + p.stats);
+    a.g = (const T *)g; a.lse2 = lse2; a.delta = delta; a.part = (float *)((char *)ws + 2 * p.stats);
+    if (s->nq > 0) {
+        const int64_t rpb = AT_THREADS * (16 / (int64_t)sizeof(T)) / 128;
+        const dim3 grid((unsigned)dg_cdiv(p.rows, rpb));
+        if (mask) hipLaunchKernelGGL((k_attn_delta<T, true>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, lse2, delta, p.rows);
+        else hipLaunchKernelGGL((k_attn_delta<T, false>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, lse2, delta, p.rows);
+    }
+    if (s->nq > 0 && dq) {
+        a.o = (T *)dq;
+        a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
+        AT_LAUNCH(k_attn_dq, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
+        if (p.qsplits > 1)
+            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, qc, p.rows,
+                               (int)s->q_heads, (int)s->nq, (int)s->d, (int)p.qsplits);
+    }
+    if (s->nk > 0 && dk) {
+        a.dk = (T *)dk; a.dv = (T *)dv;
+        a.tiles = (int)p.ktiles; a.splits = (int)p.ksplits; a.per = (int)p.kper;
+        AT_LAUNCH(k_attn_dkv, s->batch * s->k_heads * p.ktiles * p.ksplits, a);
+        if (p.ksplits > 1) {
+            const int64_t rows = s->batch * s->k_heads * s->nk, half = rows * p.ksplits * s->d;
+            const dim3 grid((unsigned)dg_cdiv(rows * s->d, AT_THREADS));
+            hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dk, (const int32_t *)nullptr, rows, (int)s->k_heads,
+                               (int)s->nk, (int)s->d, (int)p.ksplits);
+            hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part + half, (T *)dv, (const int32_t *)nullptr, rows, (int)s->k_heads,
+                               (int)s->nk, (int)s->d, (int)p.ksplits);
+        }
+    }
+    DG_CHECK_LAUNCH("k_attn_dkv");
+    return DG_OK;
+}
+
+extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, const void *q, const void *k, const void *v, const void *out, const float *lse,
+                               const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, size_t ws_bytes,
+                               dg_stream_t stream)
+{
+    const int rc = at_check(s, "roi_attn_bwd");
+    if (rc != DG_OK) return rc;
+    if (s->batch == 0 || (s->nq == 0 && s->nk == 0)) return DG_OK;
+    DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv, "roi_attn_bwd: null pointer");
+    DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
+                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && at_aligned(grad_out, s->g_stride, s, s->nq, s->q_heads) &&
+                   ((((uintptr_t)out) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes");
+    const size_t need = dg_roi_attn_workspace_bytes(s, 1);
+    if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_bwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
+    DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_bwd: workspace must be 16-byte aligned");
+    return s->dtype == DG_F32
+               ? at_backward<float>(s, grad_out, q, k, v, out, lse, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream)
+               : at_backward<__bf16>(s, grad_out, q, k, v, out, lse, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream);
+}

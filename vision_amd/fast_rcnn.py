@@ -3,6 +3,11 @@
   slowroipool(output_size).foward(img, roi_ary, roi_idx)   rcnn/fast_rcnn.py:351-377
   nms(rects, scores) -> (rect, score)                      rcnn/fast_rcnn.py:590-610
 
+and, with no counterpart there (its sketch classifies every RoI by itself, :379-384), what a head that relates the RoIs of an
+image to each other trains on, with gradients:
+
+  roi_attention(q, k, v, ...)                              attention over an image's RoIs or map cells
+
 As written the reference pools with AdaptiveAvgPool2d stored in a field called `maxpool`
 (:354) and never defines backward (autograd).  `mode="avg"` (the default: an import swap must
 reproduce the class as written) is that; `mode="max"` is the RoI MAX-pooling north_star asks
@@ -84,3 +89,30 @@ def nms(rects, scores):
         ops.check(ops.load().dg_top_score_f64(ops.ptr(sc), sc.shape[0], ops.ptr(top), ops.stream_ptr(dev)))
     top = int(top.item())
     return rects_a[top], scores_a[top]
+
+
+# ------------------------------------------------------------------ RoI head
+class _RoIAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, q_counts, k_counts, mask, scale):
+        out, lse = ops.roi_attention(q, k, v, q_counts, k_counts, mask, scale)
+        ctx.save_for_backward(q, k, v, out, lse, q_counts, k_counts, mask)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, out, lse, q_counts, k_counts, mask = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv = ops.roi_attention_backward(grad_out, q, k, v, out, lse, q_counts, k_counts, mask, ctx.scale, need[0], need[1] or need[2])
+        return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
+
+
+def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
+    """ops.roi_attention's out, with a gradient for q, k and v.  Tensors on the CPU are copied in and the result back."""
+    dev = ops._abi.device_of(q, k, v)
+    was_cpu = not any(t.is_cuda for t in (q, k, v))
+    qc, kc, m = (c if c is None else torch.as_tensor(c).to(dev) for c in (q_counts, k_counts, mask))
+    out = _RoIAttentionFn.apply(q.to(dev), k.to(dev), v.to(dev), qc, kc, m, scale)
+    return out.cpu() if was_cpu else out

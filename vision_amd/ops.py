@@ -345,3 +345,99 @@ def kmeans_labels_i32(labels_u8):
     with torch.cuda.device(labels_u8.device):
         check(load().dg_kmeans_labels_i32(ptr(labels_u8), labels_u8.numel(), ptr(out), stream_ptr(labels_u8.device)))
     return out
+
+
+# ------------------------------------------------------------------ RoI head: attention
+def _scratch(nbytes, dev):
+    """Scratch of one call, from the caching allocator in the current stream's order: captured graphs and calls on other
+    streams never share it."""
+    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _vec16(t):
+    """t with a dense last axis and everything a kernel steps along a multiple of 16 bytes; copied if it is not."""
+    e = t.element_size()
+    if t.numel() == 0:
+        return t
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st * e % 16 == 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _counts(c, B, dev, what):
+    if c is None:
+        return None
+    c = _abi.to_dev(c, torch.int32, dev)
+    if c.shape != (B,):
+        raise ValueError(f"roi_attention: {what} must be ({B},), one count per image")
+    return c
+
+
+def _attn_call(q, k, v, q_counts, k_counts, mask, scale):
+    """checks and lays out what the forward and the backward pass have in common"""
+    dev = _abi.device_of(q, k, v)
+    q, k, v = (t.to(dev) for t in (q, k, v))
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+        raise ValueError("roi_attention: q (B,Nq,Hq,D), k and v (B,Nk,Hk,D)")
+    if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("roi_attention: q, k and v must all be float32 or all be bfloat16")
+    q, k, v = _vec16(q), _vec16(k), _vec16(v)
+    B, Nq, Hq, D = q.shape
+    Nk, Hk = k.shape[1], k.shape[2]
+    qc, kc = _counts(q_counts, B, dev, "q_counts"), _counts(k_counts, B, dev, "k_counts")
+    s = _abi.AttnShape(B, Nq, Nk, Hq, Hk, D)
+    s.q_stride[:], s.k_stride[:], s.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    s.scale = D ** -0.5 if scale is None else float(scale)
+    s.dtype = _abi.TYPES[q.dtype]
+    if mask is not None:
+        mask = mask.to(dev) if isinstance(mask, torch.Tensor) else torch.as_tensor(mask, device=dev)
+        if mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("roi_attention: mask must be bool (or uint8: not 0 = may be seen)")
+        if mask.dim() == 2:
+            mask = mask[None]
+        if mask.dim() != 3 or mask.shape[0] not in (1, B) or tuple(mask.shape[1:]) != (Nq, Nk):
+            raise ValueError("roi_attention: mask must be (Nq,Nk) or (B or 1,Nq,Nk)")
+        if Nk > 1 and mask.stride(2) != 1:
+            mask = mask.contiguous()
+        s.mask_stride[:] = (mask.stride(0) if mask.shape[0] > 1 else 0, mask.stride(1))
+    return dev, q, k, v, qc, kc, mask, s
+
+
+def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
+    """Attention over padded sets of RoIs or map cells: q (B,Nq,Hq,D), k and v (B,Nk,Hk,D), float32 or bfloat16, any strides,
+    Hq a multiple of Hk (query head h reads key head h // (Hq // Hk)), D a multiple of 8 up to 128 -> out (B,Nq,Hq,D),
+    lse (B,Hq,Nq) float32.  A row sees the keys before k_counts (B) of its image for which mask (B or 1,Nq,Nk) is not 0; scale
+    defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  No reference
+    counterpart.  For a gradient: fast_rcnn.roi_attention."""
+    dev, q, k, v, qc, kc, mask, s = _attn_call(q, k, v, q_counts, k_counts, mask, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
+    lib = load()
+    nbytes = lib.dg_roi_attn_workspace_bytes(s, 0)
+    ws = _scratch(nbytes, dev)
+    with torch.cuda.device(dev):
+        check(lib.dg_roi_attn_fwd(s, ptr(q), ptr(k), ptr(v), ptr(qc), ptr(kc), ptr(mask), ptr(out), ptr(lse), ptr(ws), nbytes, stream_ptr(dev)))
+    return out, lse
+
+
+def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=None, mask=None, scale=None, need_q=True, need_kv=True):
+    """Gradients of roi_attention from its inputs, out and lse, with the probabilities recomputed: dq (B,Nq,Hq,D), dk and dv
+    (B,Nk,Hk,D), rows behind a count 0.  need_q / need_kv False leaves those out (None)."""
+    dev, q, k, v, qc, kc, mask, s = _attn_call(q, k, v, q_counts, k_counts, mask, scale)
+    g, out, lse = grad_out.to(dev), out.to(dev).contiguous(), lse.to(dev).contiguous()
+    if g.shape != q.shape or out.shape != q.shape or g.dtype != q.dtype or out.dtype != q.dtype:
+        raise ValueError("roi_attention_backward: grad_out and out must have q's shape and type")
+    if lse.shape != (s.batch, s.q_heads, s.nq) or lse.dtype != torch.float32:
+        raise ValueError("roi_attention_backward: lse must be (B,Hq,Nq) float32")
+    g, out = _vec16(g), _vec16(out)
+    s.g_stride[:] = g.stride()[:3]
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
+    dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
+    dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
+    lib = load()
+    nbytes = lib.dg_roi_attn_workspace_bytes(s, 1)
+    ws = _scratch(nbytes, dev)
+    with torch.cuda.device(dev):
+        check(lib.dg_roi_attn_bwd(s, ptr(g), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(qc), ptr(kc), ptr(mask), ptr(dq), ptr(dk), ptr(dv),
+                                  ptr(ws), nbytes, stream_ptr(dev)))
+    return dq, dk, dv
