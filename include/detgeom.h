@@ -33,6 +33,7 @@ extern "C" {
 #define DG_F32 0  /* types of the RoI head's operators */
 #define DG_BF16 1
 #define DG_F16 2
+#define DG_F64 3
 
 #define DG_POOL_AVG 0 /* rcnn/fast_rcnn.py:354 as written (AdaptiveAvgPool2d) */
 #define DG_POOL_MAX 1 /* north_star: max + argmax */
@@ -357,6 +358,40 @@ int dg_roi_attn_fwd(const dg_attn_shape *shape, const void *q, const void *k, co
 int dg_roi_attn_bwd(const dg_attn_shape *shape, const void *grad_out, const void *q, const void *k, const void *v, const void *out,
                     const float *lse, const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv,
                     void *ws, size_t ws_bytes, dg_stream_t s);
+
+/* ---------------------------------------------------------------- the RoI head: rotary positions over several axes
+ * NO COUNTERPART IN THE REFERENCE.  q (batch, n, q_heads, d), k (batch, n, k_heads, d; either may have 0 heads and be NULL): strides
+ * of the first three axes in values, last axis dense; DG_F32, DG_BF16 or DG_F16.  pos (batch, n, axes) DG_F32 or DG_F64: strides of
+ * batch (0 = one set for all) and token, last axis dense.  Pair j < pairs of every head -- values j and j + pairs (DG_ROPE_HALVES)
+ * or 2 j and 2 j + 1 (DG_ROPE_NEIGHBOURS) -- is turned by pos[axis[j]] * turns[j] whole turns (axis is held to [0, axes)), by the
+ * negative of that if inverse != 0, which is the gradient; values behind 2 * pairs are copied.  The angle is reduced in 64 bits.
+ * out_q, out_k: dense, same type; not the inputs.  A position that is not finite gives NaN for its token's turned values. */
+#define DG_ROPE_HALVES 0
+#define DG_ROPE_NEIGHBOURS 1
+typedef struct dg_rope_shape {   /* host */
+    int64_t batch, n, q_heads, k_heads, d, pairs, axes;
+    int64_t q_stride[3], k_stride[3], pos_stride[2];
+    int32_t dtype, pos_dtype, pairing;
+} dg_rope_shape;
+int dg_rope_axes(const dg_rope_shape *shape, const void *q, const void *k, const void *pos, const double *turns, const int32_t *axis,
+                 int inverse, void *out_q, void *out_k, dg_stream_t s);
+
+/* ---------------------------------------------------------------- the RoI head: log probabilities of labels
+ * NO COUNTERPART IN THE REFERENCE (its classifiers end in torch's own loss).  logits (n, c): rows `stride` values apart, dense
+ * classes; DG_F32, DG_BF16 or DG_F16.  labels (n) int64: a negative one gives none (logp 0, no gradient), one at or above c gives
+ * NaN (logp, and the row's gradient) and sets bit 0 of *status (device int32, zeroed by the caller); labels may be NULL (then logp
+ * and status may be).  Outputs, fp32: logp (n) = z_y - lse, entropy (n; may be NULL) of the row's distribution in nats, norm
+ * (n, 2) = the row's maximum m and log sum e^(z-m), whose sum is lse = log sum e^z, and the `top` (0 to 32, at most c) classes of the
+ * largest logits, best first, equal logits by the lowest index, NaN last: top_logp (n, top), top_index (n, top) int64.  -inf is a
+ * masked class; a row of nothing else gives logp = -inf, norm = (-inf, 0), entropy 0, no gradient.  A NaN or +inf makes its row's
+ * numbers NaN.  Sums in 32 bits, one pass over the logits. */
+size_t dg_class_logprobs_workspace_bytes(int64_t n, int64_t c, int64_t top);
+int dg_class_logprobs(const void *logits, int dtype, const int64_t *labels, int64_t n, int64_t c, int64_t stride, int64_t top,
+                      float *logp, float *entropy, float *norm, float *top_logp, int64_t *top_index, int32_t *status, void *ws,
+                      size_t ws_bytes, dg_stream_t s);
+/* grad_logits (n, c) dense, of the logits' type, from grad_logp (n) and grad_entropy (n) (each may be NULL) and what the forward gave */
+int dg_class_logprobs_bwd(const void *logits, int dtype, const int64_t *labels, int64_t n, int64_t c, int64_t stride, const float *norm,
+                          const float *entropy, const float *grad_logp, const float *grad_entropy, void *grad_logits, dg_stream_t s);
 
 #ifdef __cplusplus
 }

@@ -17,7 +17,8 @@ OK, EINVAL, EEMPTYROI, ENOMEM, EHIP, ERCCL = 0, -1, -2, -3, -4, -5
 COMM_ID_BYTES = 128
 POOL_AVG, POOL_MAX = 0, 1
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, F64 = 0, 1, 2, 3
+ROPE_HALVES, ROPE_NEIGHBOURS = 0, 1
 TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 _vp, _i64, _i32, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_double, C.c_size_t
@@ -27,6 +28,12 @@ class AttnShape(C.Structure):
     _fields_ = [(n, _i64) for n in ("batch", "nq", "nk", "q_heads", "k_heads", "d")] + \
                [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "g_stride")] + \
                [("mask_stride", _i64 * 2), ("scale", _f32), ("dtype", _i32)]
+
+
+class RopeShape(C.Structure):
+    """dg_rope_shape of include/detgeom.h"""
+    _fields_ = [(n, _i64) for n in ("batch", "n", "q_heads", "k_heads", "d", "pairs", "axes")] + \
+               [("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("pos_stride", _i64 * 2)] + [(n, _i32) for n in ("dtype", "pos_dtype", "pairing")]
 
 
 # name -> (restype, argtypes); must list every symbol include/detgeom.h declares
@@ -92,6 +99,10 @@ SIGNATURES = {
     "dg_roi_attn_workspace_bytes": (_sz, [C.POINTER(AttnShape), C.c_int]),
     "dg_roi_attn_fwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 9 + [_sz, _vp]),
     "dg_roi_attn_bwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 13 + [_sz, _vp]),
+    "dg_rope_axes": (C.c_int, [C.POINTER(RopeShape)] + [_vp] * 5 + [C.c_int] + [_vp] * 3),
+    "dg_class_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "dg_class_logprobs": (C.c_int, [_vp, C.c_int, _vp, _i64, _i64, _i64, _i64] + [_vp] * 7 + [_sz, _vp]),
+    "dg_class_logprobs_bwd": (C.c_int, [_vp, C.c_int, _vp, _i64, _i64, _i64] + [_vp] * 6),
 }
 
 _lib = None

@@ -1,0 +1,419 @@
+// logprob.hip — log probabilities of given classes, with entropy and the best alternatives, and their gradient.
+//   l = log sum_j e^z_j,  logp = z_y - l,  H = log s - w / s  with  s = sum e^(z-m), w = sum e^(z-m) (z-m), m = max z
+//   dz_j = g (1[j = y] - p_j) - gH p_j (z_j - l + H),  p_j = e^(z_j - l)
+// The entropy is formed from differences to the maximum (not from l - sum p z), so that large scores of one row cost no digits.
+// For the same reason l is kept as the pair (m, log s), and log probabilities are (z - m) - log s.
+// The forward pass reads the scores once: maximum, sums and the list of the best run along together.  Bound by memory.
+#include "common.hpp"
+#include <hip/hip_bf16.h>
+#include <math.h>
+
+#define LP_LOG2E 1.4426950408889634f
+#define LP_NONE (~0ull)
+
+struct lp_args {
+    const void *z;
+    const int64_t *y;                             // may be NULL
+    int64_t n, c, stride;                         // stride of a row in values
+    float *logp, *entropy, *norm, *top_logp;      // logp and entropy may be NULL; norm: pairs
+    int64_t *top_index;
+    int32_t *status;
+    u64 *keys;                                    // partial results of split rows
+    float *part;
+    int64_t per;                                  // classes of a split
+    int top, splits;
+};
+
+// order of the best: larger scores first (-0 and 0 are one value), equal ones by index, NaN behind -inf
+__device__ __forceinline__ u32 lp_desc(float v) { return v != v ? 0xfffffffeu : dg_score_desc(v + 0.0f); }
+__device__ __forceinline__ u64 lp_key(float v, u32 j) { return ((u64)lp_desc(v) << 32) | j; }
+__device__ __forceinline__ float lp_value(u64 key)
+{
+    const u32 ord = ~(u32)(key >> 32);
+    return __uint_as_float((ord & 0x80000000u) ? ord & 0x7fffffffu : ~ord);
+}
+__device__ __forceinline__ u64 lp_lane(u64 v, int l)
+{
+    return ((u64)(u32)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) | (u32)__builtin_amdgcn_readlane((int)v, l);
+}
+
+// the best keys seen by a wave, ascending (best first): lane i holds the i-th
+struct lp_list {
+    u64 list = LP_NONE, thr = LP_NONE;
+    __device__ __forceinline__ void offer(u64 key, int keep, int lane)
+    {
+        u64 some = __ballot(key < thr);
+        while (some) {
+            const int l = __ffsll((unsigned long long)some) - 1;
+            const u64 c = lp_lane(key, l), up = __shfl_up(list, 1, 64);
+            list = list < c ? list : (lane == 0 || up < c) ? c : up;
+            thr = lp_lane(list, keep - 1);
+            if (lane == l) key = LP_NONE;
+            some = __ballot(key < thr);
+        }
+    }
+};
+
+// statistics of a set of scores: maximum, sum of e^(z-m), sum of e^(z-m) (z-m)
+struct lp_sum {
+    float m = -INFINITY, s = 0.f, w = 0.f;
+    __device__ __forceinline__ void raise(float mx)
+    {
+        if (mx > m) {
+            const float d = m - mx, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+            w = f == 0.f ? 0.f : f * fmaf(s, d, w);
+            s *= f;
+            m = mx;
+        }
+    }
+    __device__ __forceinline__ void add(float z)  // z <= m, or NaN
+    {
+        const float d = m == -INFINITY ? z : z - m, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        s += e;
+        w = fmaf(e, fmaxf(d, -3.0e38f), w);
+    }
+    __device__ __forceinline__ void join(float om, float os, float ow)
+    {
+        const float mx = fmaxf(m, om);
+        if (mx == -INFINITY) { s += os; return; } // nothing on either side, or only NaN
+        const float a = m - mx, b = om - mx;
+        const float fa = __builtin_amdgcn_exp2f(a * LP_LOG2E), fb = __builtin_amdgcn_exp2f(b * LP_LOG2E);
+        const float wa = fa == 0.f ? 0.f : fa * fmaf(s, a, w), wb = fb == 0.f ? 0.f : fb * fmaf(os, b, ow);
+        s = fa * s + fb * os;
+        w = wa + wb;
+        m = mx;
+    }
+    template <int L> __device__ __forceinline__ void join_lanes()
+    {
+#pragma unroll
+        for (int x = L / 2; x; x >>= 1) {
+            const float om = __shfl_xor(m, x, 64), os = __shfl_xor(s, x, 64), ow = __shfl_xor(w, x, 64);
+            join(om, os, ow);
+        }
+    }
+    __device__ __forceinline__ float entropy() const { return s == 0.f ? 0.f : fmaxf(logf(s) - w / s, 0.f) + (s - s); }
+};
+
+// what turns a score into a log probability; a row with nothing to choose from (all -inf): -inf throughout, entropy 0
+struct lp_norm {
+    float m, ls;
+    __device__ __forceinline__ explicit lp_norm(const lp_sum &t) : m(t.m), ls(t.s == 0.f ? 0.f : logf(t.s)) {}
+    __device__ __forceinline__ lp_norm(float m_, float ls_) : m(m_), ls(ls_) {}
+    __device__ __forceinline__ float of(float z) const { return m == -INFINITY && ls == 0.f ? -INFINITY : (z - m) - ls; }
+};
+
+// the numbers of a row beside its best: one lane writes them
+template <typename T>
+__device__ __forceinline__ void lp_write(const lp_args &a, int64_t row, const lp_sum &t, const lp_norm &nm)
+{
+    if (a.entropy) a.entropy[row] = t.entropy();
+    a.norm[2 * row] = nm.m;
+    a.norm[2 * row + 1] = nm.ls;
+    if (a.y) {
+        const int64_t y = a.y[row];
+        float v = 0.f;                            // a negative label: no class given
+        if (y >= a.c) { v = __builtin_nanf(""); atomicOr(a.status, 1); }
+        else if (y >= 0) v = nm.of((float)((const T *)a.z)[row * a.stride + y]);
+        a.logp[row] = v;
+    }
+}
+
+// ------------------------------------------------------------------ up to 512 classes: L lanes hold a row, 8 scores each
+template <typename T, int L>
+__global__ __launch_bounds__(256) void k_logprob_small(const lp_args a)
+{
+    const int sub = threadIdx.x & (L - 1);
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    if (row >= a.n) return;                       // whole groups: shuffles stay among the lanes of a row
+    const T *z = (const T *)a.z + row * a.stride;
+    float v[8];
+    lp_sum t;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int j = sub + i * L;
+        v[i] = j < a.c ? (float)z[j] : -INFINITY;
+        mx = fmaxf(mx, v[i]);
+    }
+#pragma unroll
+    for (int x = L / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
+    t.raise(mx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t.add(v[i]);
+#pragma unroll
+    for (int x = L / 2; x; x >>= 1) {             // one maximum for all lanes: the sums just add up
+        t.s += __shfl_xor(t.s, x, 64);
+        t.w += __shfl_xor(t.w, x, 64);
+    }
+    const lp_norm nm(t);
+    if (sub == 0) lp_write<T>(a, row, t, nm);
+    if (a.top == 0) return;
+    u32 key[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) key[i] = sub + i * L < a.c ? lp_desc(v[i]) : 0xffffffffu;
+    for (int r = 0; r < a.top; ++r) {
+        u32 best = 0xffffffffu, at = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (key[i] < best) { best = key[i]; at = i; }
+        u32 j = sub + at * L;
+#pragma unroll
+        for (int x = L / 2; x; x >>= 1) {
+            const u32 ob = __shfl_xor(best, x, 64), oj = __shfl_xor(j, x, 64);
+            if (ob < best || (ob == best && oj < j)) { best = ob; j = oj; }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (j == (u32)(sub + i * L)) key[i] = 0xffffffffu;
+        if (sub == 0) {
+            a.top_logp[row * a.top + r] = nm.of(lp_value((u64)best << 32));
+            a.top_index[row * a.top + r] = j;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ more classes: waves walk a row
+__device__ __forceinline__ void lp_best(const lp_args &a, int64_t row, const lp_list &b, const lp_norm &n, int lane)
+{
+    if (lane < a.top) {
+        a.top_logp[row * a.top + lane] = n.of(lp_value(b.list));
+        a.top_index[row * a.top + lane] = (u32)b.list;
+    }
+}
+
+// WPR waves walk one row's split (4: a workgroup, 1: each wave a row of its own).  Scores come 16 bytes at a time from the first
+// aligned one on; the few before and behind are single loads.
+template <typename T, int WPR>
+__global__ __launch_bounds__(256) void k_logprob_walk(const lp_args a)
+{
+    constexpr int V = 16 / (int)sizeof(T), UN = 4;
+    typedef T vec __attribute__((ext_vector_type(V)));
+    __shared__ float sums[4][3];
+    __shared__ u64 lists[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = WPR == 4 ? threadIdx.x : lane;
+    const int64_t part = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t row = part / a.splits, sp = part - row * a.splits;
+    if (row >= a.n) return;                       // WPR == 1: whole waves, and no barrier follows
+    const int keep = a.top;
+    const T *z = (const T *)a.z + row * a.stride;
+    const int64_t c0 = sp * a.per, c1 = min(a.c, c0 + a.per);
+    // first aligned class of the split, last whole piece
+    int64_t b0 = c0 + (int64_t)(((16 - ((uintptr_t)(z + c0) & 15)) & 15) / sizeof(T));
+    if (b0 > c1) b0 = c1;
+    const int64_t pieces = (c1 - b0) / V, b1 = b0 + pieces * V;
+
+    lp_sum t;
+    lp_list best;
+    auto single = [&](int64_t from, int64_t to) { // what lies before the first piece or behind the last: under V scores each
+        const int64_t j = from + lane;
+        const float v = j < to ? (float)z[j] : -INFINITY;
+        t.raise(v);
+        if (j < to) t.add(v);
+        if (keep) best.offer(j < to ? lp_key(v, (u32)j) : LP_NONE, keep, lane);
+    };
+    if (wave == 0 || WPR == 1) single(c0, b0);
+    const vec *zp = (const vec *)(z + b0);
+    for (int64_t p0 = 0; p0 < pieces; p0 += 64 * WPR * UN) {
+        float v[UN][V];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int64_t p = p0 + u * (64 * WPR) + tid;
+            if (p < pieces) {
+                const vec x = zp[p];
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[u][e] = (float)x[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[u][e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) mx = fmaxf(mx, v[u][e]);
+        }
+        t.raise(mx);
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+#pragma unroll
+            for (int e = 0; e < V; ++e) t.add(v[u][e]);
+        if (keep && __any(best.thr == LP_NONE || !(mx <= lp_value(best.thr)))) {
+#pragma unroll
+            for (int u = 0; u < UN; ++u) {
+                const int64_t p = p0 + u * (64 * WPR) + tid;
+#pragma unroll
+                for (int e = 0; e < V; ++e) best.offer(p < pieces ? lp_key(v[u][e], (u32)(b0 + p * V + e)) : LP_NONE, keep, lane);
+            }
+        }
+    }
+    if (wave == 0 || WPR == 1) single(b1, c1);    // in the order of the classes: an equal score that comes later never ranks before
+    t.join_lanes<64>();
+    if (WPR == 4) {
+        if (lane == 0) { sums[wave][0] = t.m; sums[wave][1] = t.s; sums[wave][2] = t.w; }
+        if (keep) lists[wave][lane] = best.list;
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            t.join(sums[i][0], sums[i][1], sums[i][2]);
+            if (keep) best.offer(lane < keep ? lists[i][lane] : LP_NONE, keep, lane);
+        }
+    }
+    if (a.splits > 1) {
+        if (lane == 0) {
+            float *o = a.part + part * 3;
+            o[0] = t.m; o[1] = t.s; o[2] = t.w;
+        }
+        if (lane < keep) a.keys[part * keep + lane] = best.list;
+        return;
+    }
+    const lp_norm nm(t);
+    if (lane == 0) lp_write<T>(a, row, t, nm);
+    if (a.top) lp_best(a, row, best, nm, lane);
+}
+
+// joins the splits of a row: one wave per row
+template <typename T>
+__global__ __launch_bounds__(64) void k_logprob_join(const lp_args a)
+{
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const int keep = a.top;
+    lp_sum t;
+    for (int s = lane; s < a.splits; s += 64) {
+        const float *p = a.part + (row * a.splits + s) * 3;
+        t.join(p[0], p[1], p[2]);
+    }
+    t.join_lanes<64>();
+    const lp_norm nm(t);
+    if (lane == 0) lp_write<T>(a, row, t, nm);
+    if (!keep) return;
+    lp_list best;
+    const u64 *k = a.keys + row * a.splits * keep;
+    for (int i0 = 0; i0 < a.splits * keep; i0 += 64) best.offer(i0 + lane < a.splits * keep ? k[i0 + lane] : LP_NONE, keep, lane);
+    lp_best(a, row, best, nm, lane);
+}
+
+// ------------------------------------------------------------------ backward: one read, one write
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void k_logprob_bwd(const T *__restrict__ z, const int64_t *__restrict__ y, int64_t n, int64_t c, int64_t stride,
+                                                     const float *__restrict__ norm, const float *__restrict__ entropy, const float *__restrict__ g,
+                                                     const float *__restrict__ gh, T *__restrict__ dz, int64_t blocks)
+{
+    typedef T vec __attribute__((ext_vector_type(VEC)));
+    const int64_t row = blockIdx.x / blocks, j0 = ((blockIdx.x - row * blocks) * 256 + threadIdx.x) * VEC;
+    if (j0 >= c) return;
+    const lp_norm nm(norm[2 * row], norm[2 * row + 1]);
+    const float h = gh ? entropy[row] : 0.f, gH = gh ? gh[row] : 0.f;
+    const int64_t lab = y ? y[row] : -1;
+    float gl = g && lab >= 0 ? g[row] : 0.f;
+    if (lab >= c) gl = __builtin_nanf("");
+    const vec x = *(const vec *)(z + row * stride + j0);
+    vec o;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+        const float lp = nm.of((float)x[e]), p = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
+        float v = p == 0.f ? 0.f : -p * fmaf(gH, lp + h, gl);
+        if (lab >= c) v = gl;
+        if (j0 + e == lab && nm.m != -INFINITY) v += gl;
+        o[e] = (T)v;
+    }
+    *(vec *)(dz + row * c + j0) = o;
+}
+
+// ------------------------------------------------------------------ host
+static int lp_check(int64_t n, int64_t c, int64_t stride, int dtype, int64_t top, const char *who)
+{
+    DG_REQUIRE(dtype == DG_F32 || dtype == DG_BF16 || dtype == DG_F16, "%s: type must be DG_F32, DG_BF16 or DG_F16", who);
+    DG_REQUIRE(n >= 0 && n < (1ll << 31), "%s: bad row count", who);
+    DG_REQUIRE(c >= 1 && c < (1ll << 31), "%s: 1 to 2^31 - 1 classes", who);
+    DG_REQUIRE(stride >= 0, "%s: negative stride", who);
+    DG_REQUIRE(top >= 0 && top <= 32 && top <= c, "%s: 0 to 32 alternatives, no more than classes", who);
+    return DG_OK;
+}
+
+// rows that are too few to fill the chip are split over their classes, 4096 of them at least, 256 workgroups' worth
+static void lp_split(int64_t n, int64_t c, int64_t *splits, int64_t *per)
+{
+    int64_t s = n > 0 && n < 256 ? dg_cdiv(512, n) : 1;
+    if (s > dg_cdiv(c, 4096)) s = dg_cdiv(c, 4096);
+    *per = dg_round_up(dg_cdiv(c, s), 64);
+    *splits = dg_cdiv(c, *per);
+}
+
+extern "C" size_t dg_class_logprobs_workspace_bytes(int64_t n, int64_t c, int64_t top)
+{
+    if (n <= 0 || c <= 512 || top < 0 || top > 32) return 0;
+    int64_t s, per;
+    lp_split(n, c, &s, &per);
+    return s > 1 ? (size_t)(n * s * (top * 8 + 12)) : 0;
+}
+
+template <typename T> static void lp_forward(lp_args &a, hipStream_t st)
+{
+    if (a.c <= 512) {
+#define LP_SMALL(L) hipLaunchKernelGGL((k_logprob_small<T, L>), dim3((unsigned)dg_cdiv(a.n, 256 / L)), dim3(256), 0, st, a)
+        if (a.c <= 32) LP_SMALL(4);
+        else if (a.c <= 64) LP_SMALL(8);
+        else if (a.c <= 128) LP_SMALL(16);
+        else if (a.c <= 256) LP_SMALL(32);
+        else LP_SMALL(64);
+        return;
+    }
+    if (a.splits == 1 && a.c <= 4096) hipLaunchKernelGGL((k_logprob_walk<T, 1>), dim3((unsigned)dg_cdiv(a.n, 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_logprob_walk<T, 4>), dim3((unsigned)(a.n * a.splits)), dim3(256), 0, st, a);
+    if (a.splits > 1) hipLaunchKernelGGL((k_logprob_join<T>), dim3((unsigned)a.n), dim3(64), 0, st, a);
+}
+
+extern "C" int dg_class_logprobs(const void *logits, int dtype, const int64_t *labels, int64_t n, int64_t c, int64_t stride, int64_t top, float *logp,
+                                 float *entropy, float *norm, float *top_logp, int64_t *top_index, int32_t *status, void *ws, size_t ws_bytes, dg_stream_t s)
+{
+    const int rc = lp_check(n, c, stride, dtype, top, "class_logprobs");
+    if (rc != DG_OK) return rc;
+    if (n == 0) return DG_OK;
+    DG_REQUIRE(logits && norm && (!labels || (logp && status)) && (!top || (top_logp && top_index)), "class_logprobs: null pointer");
+    DG_REQUIRE((((uintptr_t)logits) & (dtype == DG_F32 ? 3 : 1)) == 0, "class_logprobs: logits are not aligned to their type");
+    const size_t need = dg_class_logprobs_workspace_bytes(n, c, top);
+    if (ws_bytes < need || (need && !ws)) { dg_set_error("class_logprobs: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
+    DG_REQUIRE((((uintptr_t)ws) & 7) == 0, "class_logprobs: workspace must be 8-byte aligned");
+    lp_args a = {};
+    a.z = logits; a.y = labels; a.n = n; a.c = c; a.stride = stride;
+    a.logp = logp; a.entropy = entropy; a.norm = norm; a.top_logp = top_logp; a.top_index = top_index; a.status = status;
+    a.top = (int)top;
+    int64_t sp = 1, per = c;
+    if (c > 512) lp_split(n, c, &sp, &per);
+    a.splits = (int)sp; a.per = per;
+    a.keys = (u64 *)ws;
+    a.part = (float *)((char *)ws + (size_t)(n * sp * top * 8));
+    if (dtype == DG_F32) lp_forward<float>(a, (hipStream_t)s);
+    else if (dtype == DG_BF16) lp_forward<__bf16>(a, (hipStream_t)s);
+    else lp_forward<_Float16>(a, (hipStream_t)s);
+    DG_CHECK_LAUNCH("k_logprob");
+    return DG_OK;
+}
+
+template <typename T>
+static int lp_backward(const void *z, const int64_t *y, int64_t n, int64_t c, int64_t stride, const float *norm, const float *entropy, const float *g, const float *gh,
+                       void *dz, hipStream_t st)
+{
+    constexpr int V = 16 / (int)sizeof(T);
+    const bool wide = c % V == 0 && stride % V == 0 && ((((uintptr_t)z) | ((uintptr_t)dz)) & 15) == 0;
+    const int64_t blocks = dg_cdiv(c, 256 * (wide ? V : 1));
+    DG_REQUIRE(n * blocks < (1ll << 31), "class_logprobs_bwd: too large");
+    if (wide) hipLaunchKernelGGL((k_logprob_bwd<T, V>), dim3((unsigned)(n * blocks)), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz, blocks);
+    else hipLaunchKernelGGL((k_logprob_bwd<T, 1>), dim3((unsigned)(n * blocks)), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz, blocks);
+    DG_CHECK_LAUNCH("k_logprob_bwd");
+    return DG_OK;
+}
+
+extern "C" int dg_class_logprobs_bwd(const void *logits, int dtype, const int64_t *labels, int64_t n, int64_t c, int64_t stride, const float *norm, const float *entropy,
+                                     const float *grad_logp, const float *grad_entropy, void *grad_logits, dg_stream_t s)
+{
+    const int rc = lp_check(n, c, stride, dtype, 0, "class_logprobs_bwd");
+    if (rc != DG_OK) return rc;
+    if (n == 0) return DG_OK;
+    DG_REQUIRE(logits && norm && grad_logits && (!grad_logp || labels) && (!grad_entropy || entropy), "class_logprobs_bwd: null pointer");
+    DG_REQUIRE(((((uintptr_t)logits) | ((uintptr_t)grad_logits)) & (dtype == DG_F32 ? 3 : 1)) == 0, "class_logprobs_bwd: not aligned to the type");
+    hipStream_t st = (hipStream_t)s;
+    if (dtype == DG_F32) return lp_backward<float>(logits, labels, n, c, stride, norm, entropy, grad_logp, grad_entropy, grad_logits, st);
+    if (dtype == DG_BF16) return lp_backward<__bf16>(logits, labels, n, c, stride, norm, entropy, grad_logp, grad_entropy, grad_logits, st);
+    return lp_backward<_Float16>(logits, labels, n, c, stride, norm, entropy, grad_logp, grad_entropy, grad_logits, st);
+}

@@ -7,6 +7,8 @@ and, with no counterpart there (its sketch classifies every RoI by itself, :379-
 image to each other trains on, with gradients:
 
   roi_attention(q, k, v, ...)                              attention over an image's RoIs or map cells
+  rope_axes(q, k, pos, plan)                               rotary positions from box centres, frames, rows and columns
+  class_logprobs(logits, labels, top)                      log probabilities of the labels, entropy, best classes
 
 As written the reference pools with AdaptiveAvgPool2d stored in a field called `maxpool`
 (:354) and never defines backward (autograd).  `mode="avg"` (the default: an import swap must
@@ -14,6 +16,8 @@ reproduce the class as written) is that; `mode="max"` is the RoI MAX-pooling nor
 for -- the same module with AdaptiveMaxPool2d substituted -- and also yields the argmax used
 by the backward scatter.
 """
+from collections import namedtuple
+
 import numpy as np
 import torch
 
@@ -116,3 +120,67 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
     qc, kc, m = (c if c is None else torch.as_tensor(c).to(dev) for c in (q_counts, k_counts, mask))
     out = _RoIAttentionFn.apply(q.to(dev), k.to(dev), v.to(dev), qc, kc, m, scale)
     return out.cpu() if was_cpu else out
+
+
+class _RopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, plan, inverse):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(pos)
+        ctx.plan, ctx.inverse = plan, inverse
+        return ops.rope_axes(q, pos, plan, k=k, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        (pos,) = ctx.saved_tensors
+        if dq is not None and dk is not None:
+            dq, dk = _RopeFn.apply(dq, dk, pos, ctx.plan, not ctx.inverse)
+        elif dq is not None:
+            dq = _RopeFn.apply(dq, dq[:, :, :0], pos, ctx.plan, not ctx.inverse)[0]
+        elif dk is not None:
+            dk = _RopeFn.apply(dk[:, :, :0], dk, pos, ctx.plan, not ctx.inverse)[1]
+        return dq, dk, None, None, None
+
+
+def rope_axes(q, k, pos, plan):
+    """ops.rope_axes of queries and keys in one launch, with a gradient for both (none for the positions).  Tensors on the CPU
+    are copied in and the results back."""
+    dev = ops._abi.device_of(q, k)
+    was_cpu = not (q.is_cuda or k.is_cuda)
+    pos = torch.as_tensor(pos).to(dev)
+    if pos.requires_grad:
+        raise ValueError("rope_axes: positions have no gradient here; detach them")
+    q, k = _RopeFn.apply(q.to(dev), k.to(dev), pos, plan, False)
+    return (q.cpu(), k.cpu()) if was_cpu else (q, k)
+
+
+class _ClassLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, top):
+        logp, entropy, norm, best, index = ops.class_logprobs(logits, labels, top)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, labels, norm, entropy)
+        ctx.mark_non_differentiable(best, index)
+        return logp, entropy, best, index
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, gh, _best, _index):
+        logits, labels, norm, entropy = ctx.saved_tensors
+        if g is None and gh is None:
+            return None, None, None
+        return ops.class_logprobs_backward(g, gh, logits, labels, norm, entropy), None, None
+
+
+ClassLogprobs = namedtuple("ClassLogprobs", "logp entropy top_logp top_index")
+
+
+def class_logprobs(logits, labels=None, top=0):
+    """ops.class_logprobs' logp, entropy, top_logp and top_index, with a gradient of logp and entropy for the logits: the loss of
+    a classifier of RoIs is -logp.sum() / n over the labelled rows (label_proposals' labels; a negative label is left out).
+    Tensors on the CPU are copied in and the results back."""
+    dev = ops._abi.device_of(logits)
+    was_cpu = not logits.is_cuda
+    y = labels if labels is None else torch.as_tensor(labels).to(device=dev, dtype=torch.int64)
+    r = _ClassLogprobsFn.apply(logits.to(dev), y, int(top))
+    return ClassLogprobs(*(t.cpu() if was_cpu and t is not None else t for t in r))

@@ -1,6 +1,8 @@
 """Tensor-level front end of the HIP kernels: GPU tensors in, GPU tensors out, async on the
 current stream.  The reference-named drop-ins (yolo_v1.py, yolo_v2.py, rcnn_utils.py,
 fast_rcnn.py, cluster.py) are thin layers over these."""
+import math
+
 import torch
 
 from . import _abi
@@ -441,3 +443,135 @@ def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=
         check(lib.dg_roi_attn_bwd(s, ptr(g), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(qc), ptr(kc), ptr(mask), ptr(dq), ptr(dk), ptr(dv),
                                   ptr(ws), nbytes, stream_ptr(dev)))
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------ RoI head: rotary positions
+class RopePlan:
+    """Which axis turns each pair of a head and how fast: made once (rope_plan), kept by the program, used by every call."""
+
+    def __init__(self, turns, axis, axes, pairing):
+        self.turns, self.axis, self.axes, self.pairing = turns, axis, axes, pairing
+        self.pairs = turns.shape[0]
+
+    def to(self, device):
+        return self if self.turns.device == device else RopePlan(self.turns.to(device), self.axis.to(device), self.axes, self.pairing)
+
+
+def rope_plan(sections, theta=10000.0, ladder="axis", pairing="halves", device=None):
+    """sections: pairs of a head that each axis turns, e.g. (16, 24, 24) for frame, row and column of a head of 128.
+    ladder "axis": an axis's i-th of m pairs turns by theta ** (-i / m) radians per unit of its position; "shared": the j-th of
+    all pairs by theta ** (-j / sum(sections)).  pairing "halves": values j and j + sum(sections) form pair j; "neighbours":
+    values 2 j and 2 j + 1."""
+    sections = [int(m) for m in sections]
+    if not 1 <= len(sections) <= 16 or min(sections) < 0 or sum(sections) < 1:
+        raise ValueError("rope_plan: 1 to 16 axes, each with 0 or more pairs, one at least in all")
+    if ladder not in ("axis", "shared") or pairing not in ("halves", "neighbours"):
+        raise ValueError("rope_plan: ladder is 'axis' or 'shared', pairing 'halves' or 'neighbours'")
+    theta = float(theta)
+    if not 0.0 < theta < float("inf"):
+        raise ValueError("rope_plan: theta must be positive and finite")
+    n = sum(sections)
+    step = [i / m for m in sections for i in range(m)] if ladder == "axis" else [j / n for j in range(n)]
+    turns = torch.tensor([theta ** -e / (2.0 * math.pi) for e in step], dtype=torch.float64)
+    axis = torch.tensor([a for a, m in enumerate(sections) for _ in range(m)], dtype=torch.int32)
+    dev = torch.device(device) if device is not None else _abi.require_gpu()
+    return RopePlan(turns.to(dev), axis.to(dev), len(sections), pairing)
+
+
+def _dense_last(t):
+    return t if t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def rope_axes(q, pos, plan, k=None, inverse=False):
+    """Turns the pairs of q (B,N,H,D) (and of k (B,N,Hk,D) in the same launch) by the positions pos (B,N,A) or (N,A) of their
+    tokens as plan says; inverse: back, which is the gradient.  float32, bfloat16 or float16; values behind the plan's pairs are
+    copied; float32 or float64 positions are used as they are, whole numbers as float64.  -> the turned q, or (q, k).  No
+    reference counterpart.  For a gradient: fast_rcnn.rope_axes."""
+    dev = _abi.device_of(q, k, pos)
+    q = _dense_last(q.to(dev))
+    k = None if k is None else _dense_last(k.to(dev))
+    pos = pos.to(dev) if isinstance(pos, torch.Tensor) else torch.as_tensor(pos, device=dev)
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
+        raise ValueError("rope_axes: q (B,N,Hq,D), k (B,N,Hk,D) of one type")
+    if q.dtype not in _abi.TYPES:
+        raise ValueError("rope_axes: float32, bfloat16 or float16")
+    if pos.requires_grad:
+        raise ValueError("rope_axes: positions have no gradient here; detach them")
+    if not pos.is_floating_point():
+        pos = pos.to(torch.float64)
+    elif pos.dtype not in (torch.float32, torch.float64):
+        pos = pos.to(torch.float32)
+    B, N, Hq, D = q.shape
+    plan = plan.to(dev)
+    if pos.dim() not in (2, 3) or tuple(pos.shape[-2:]) != (N, plan.axes) or (pos.dim() == 3 and pos.shape[0] not in (1, B)):
+        raise ValueError(f"rope_axes: pos must be (B,N,{plan.axes}) or (N,{plan.axes})")
+    pos = _dense_last(pos)
+    s = _abi.RopeShape(B, N, Hq, 0 if k is None else k.shape[2], D, plan.pairs, plan.axes)
+    s.q_stride[:] = q.stride()[:3]
+    if k is not None:
+        s.k_stride[:] = k.stride()[:3]
+    s.pos_stride[:] = (pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2))
+    s.dtype, s.pos_dtype = _abi.TYPES[q.dtype], _abi.F64 if pos.dtype == torch.float64 else _abi.F32
+    s.pairing = _abi.ROPE_HALVES if plan.pairing == "halves" else _abi.ROPE_NEIGHBOURS
+    out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    out_k = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(load().dg_rope_axes(s, ptr(q), ptr(k), ptr(pos), ptr(plan.turns), ptr(plan.axis), int(bool(inverse)), ptr(out_q), ptr(out_k),
+                                  stream_ptr(dev)))
+    return out_q if k is None else (out_q, out_k)
+
+
+# ------------------------------------------------------------------ RoI head: log probabilities of labels
+def _logits(z, labels, what):
+    dev = _abi.device_of(z, labels)
+    z = z.to(dev) if isinstance(z, torch.Tensor) else torch.as_tensor(z, device=dev)
+    if z.dim() != 2 or z.shape[1] < 1 or z.dtype not in _abi.TYPES:
+        raise ValueError(f"{what}: logits must be (n,C), C >= 1, float32, bfloat16 or float16")
+    z = _dense_last(z)
+    if labels is not None:
+        labels = _abi.to_dev(labels, torch.int64, dev)
+        if labels.shape != z.shape[:1]:
+            raise ValueError(f"{what}: one label per row")
+    return dev, z, labels
+
+
+def class_logprobs(logits, labels=None, top=0):
+    """logits (n,C) float32, bfloat16 or float16, labels (n) or None -> logp (n) of the labels (None without them), entropy (n),
+    norm (n,2) (the row's maximum and the log of its sum of exponentials above it: what the gradient needs), top_logp (n,top),
+    top_index (n,top) int64: the most probable classes, best first, equal logits by the lowest index (top 0 to 32).  A negative label gives none (logp 0, no gradient); a label of C or more gives NaN.  -inf is a masked class.
+    No reference counterpart.  For a gradient: fast_rcnn.class_logprobs."""
+    dev, z, y = _logits(logits, labels, "class_logprobs")
+    n, c = z.shape
+    f32 = dict(dtype=torch.float32, device=dev)
+    top = int(top)
+    if not 0 <= top <= min(32, c):
+        raise ValueError("class_logprobs: top must be 0 to 32 and no more than the classes")
+    logp = torch.empty((n,), **f32) if y is not None else None
+    entropy, norm = torch.empty((n,), **f32), torch.empty((n, 2), **f32)
+    best, index = torch.empty((n, top), **f32), torch.empty((n, top), dtype=torch.int64, device=dev)
+    status = torch.empty((1,), dtype=torch.int32, device=dev) if y is not None else None    # the NaN itself says it here
+    lib = load()
+    nbytes = lib.dg_class_logprobs_workspace_bytes(n, c, top)
+    ws = _scratch(nbytes, dev)
+    with torch.cuda.device(dev):
+        check(lib.dg_class_logprobs(ptr(z), _abi.TYPES[z.dtype], ptr(y), n, c, z.stride(0), top, ptr(logp), ptr(entropy), ptr(norm), ptr(best), ptr(index),
+                                    ptr(status), ptr(ws), nbytes, stream_ptr(dev)))
+    return logp, entropy, norm, best, index
+
+
+def class_logprobs_backward(grad_logp, grad_entropy, logits, labels, norm, entropy):
+    """Gradient of the logits from those of logp and entropy (either may be None) and what class_logprobs gave."""
+    dev, z, y = _logits(logits, labels, "class_logprobs_backward")
+    n, c = z.shape
+    args = []
+    for t, shape in ((norm, (n, 2)), (entropy, (n,)), (grad_logp, (n,)), (grad_entropy, (n,))):
+        t = None if t is None else _abi.to_dev(t, torch.float32, dev)
+        if t is not None and t.shape != shape:
+            raise ValueError("class_logprobs_backward: norm (n,2), entropy and the gradients (n)")
+        args.append(t)
+    if y is None:
+        args[2] = None
+    dz = torch.empty((n, c), dtype=z.dtype, device=dev)
+    with torch.cuda.device(dev):
+        check(load().dg_class_logprobs_bwd(ptr(z), _abi.TYPES[z.dtype], ptr(y), n, c, z.stride(0), *(ptr(t) for t in args), ptr(dz), stream_ptr(dev)))
+    return dz
