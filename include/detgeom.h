@@ -332,7 +332,7 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
 /* ---------------------------------------------------------------- the RoI head: attention over an image's boxes or cells
  * NO COUNTERPART IN THE REFERENCE (its Fast R-CNN sketch classifies every RoI by itself, rcnn/fast_rcnn.py:379-384).
  * q (batch, nq, q_heads, d), k and v (batch, nk, k_heads, d): strides of the first three axes in values, the last axis dense;
- * pointers and strides multiples of 16 bytes.  Query head h reads key head h / (q_heads / k_heads).  Types: DG_F32, DG_BF16 (one
+ * pointers and strides multiples of 16 bytes, rows at most 2^22 values apart.  Query head h reads key head h / (q_heads / k_heads).  Types: DG_F32, DG_BF16 (one
  * for all of q, k, v, out and the gradients).  d: a multiple of 8 from 8 to 128.
  *   s_ij = scale * q_i . k_j,  p_i = softmax over the keys that row i may see,  out_i = sum_j p_ij v_j,  lse_i = log sum_j exp s_ij
  * A row i sees key j if i < q_counts[image], j < k_counts[image] (device int32, held to [0, n]; NULL = all) and mask[image][i][j] != 0

@@ -42,7 +42,14 @@ __device__ __forceinline__ f32x16 at_mma(f32x4 a, f32x4 b, f32x16 c)
     for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
     return c;
 }
-__device__ __forceinline__ float at_xor32(float v) { return __shfl_xor(v, 32, 64); }
+// the value of this lane and of the one 32 away, in either order
+__device__ __forceinline__ void at_both(float v, float &x, float &y)
+{
+    typedef u32 u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 r = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+    x = __uint_as_float(r[0]);
+    y = __uint_as_float(r[1]);
+}
 
 // A tile of rows in LDS, DP values wide, in 16-byte chunks whose place inside the row is swizzled by the row: eight lanes
 // reading the same chunk of eight successive rows, and sixteen lanes reading two chunks of four successive rows (the
@@ -120,6 +127,37 @@ __device__ __forceinline__ int at_xcd_id()
 
 template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p) { return *(const u32x4 *)p; }
 
+// A workgroup's loader of row tiles: thread t takes chunk t % CPR of rows t / CPR, + STEP, ...  Buffer loads: the tile's address is
+// uniform, a lane's offset inside it fixed, and a lane with nothing to load (a row behind the end, a chunk behind d) asks for an
+// offset out of range and gets zeros.  A tile spans less than 2^31 bytes (at_aligned).
+#define AT_OUT 0x7fffffff
+template <typename T, int DP, int ROWS> struct at_loader {
+    typedef at_tile<T, DP> tile;
+    static constexpr int STEP = AT_THREADS / tile::CPR, NL = ROWS / STEP > 0 ? ROWS / STEP : 1;
+    const T *base;
+    int64_t stride;
+    int row0, c16, off;                           // off: of the first row's chunk, in bytes
+    __device__ __forceinline__ at_loader(const T *p, int64_t st, int d) : base(p), stride(st), row0(threadIdx.x / tile::CPR), c16(threadIdx.x % tile::CPR)
+    {
+        off = c16 * 16 < d * (int)sizeof(T) ? row0 * (int)(st * (int)sizeof(T)) + c16 * 16 : AT_OUT;
+    }
+    __device__ __forceinline__ void load(u32x4 (&r)[NL], int64_t first, int rows) const
+    {
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(base + first * stride), 0, AT_OUT, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int o = row0 + i * STEP < rows ? off : AT_OUT;
+            r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o, i * STEP * (int)(stride * (int)sizeof(T)), 0));
+        }
+    }
+    __device__ __forceinline__ void store(char *lds, const u32x4 (&r)[NL]) const
+    {
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            if (ROWS >= STEP || row0 < ROWS) *(u32x4 *)(lds + tile::at(row0 + i * STEP, c16)) = r[i];
+    }
+};
+
 // with a pair mask, a row of K, V, Q or dO that some rows may not see must not reach them through 0 * NaN: non-finite values
 // are put to zero in the staged copy, and the caller marks the row so that those who do see it get NaN
 template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
@@ -145,16 +183,19 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // ------------------------------------------------------------------ forward
 // A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of 64.  K and V tiles are double
 // buffered in LDS; the next tile's global loads are in flight while this one is computed.
-template <typename T, int DP> struct at_shape { static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32; };   // fp32 x 128: 64 KB of LDS
+// KT keys of a tile (fp32 x 128: 32, for 64 KB of LDS); waves of a SIMD that the registers are cut for: two where two fit without
+// spilling, and the matrix results then stay in registers that the vector unit can read
+template <typename T, int DP> struct at_shape {
+    static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32, OCC = sizeof(T) * DP > 256 ? 1 : 2, OCC_KV = sizeof(T) * DP > 128 ? 1 : 2;
+};
 
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_fwd(const at_args<T> a)
+__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd(const at_args<T> a)
 {
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U;
-    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
@@ -186,27 +227,20 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_fwd(const at_args<T> a)
     const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
 
     const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
-    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
-    const bool cin = c16 * CH < a.d;
-    const T *kp = a.k + b * a.ks[0] + hk * a.ks[2] + c16 * CH, *vp = a.v + b * a.vs[0] + hk * a.vs[2] + c16 * CH;
-    u32x4 kr[NL], vr[NL];
+    const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
+    u32x4 kr[kl.NL], vr[kl.NL];
     auto load = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int key = kb + srow + i * STEP;
-            const bool in = cin && key < k1;
-            kr[i] = in ? at_load_chunk(kp + key * a.ks[1]) : (u32x4)(0u);
-            vr[i] = in ? at_load_chunk(vp + key * a.vs[1]) : (u32x4)(0u);
-        }
+        kl.load(kr, kb, k1 - kb);
+        vl.load(vr, kb, k1 - kb);
     };
     auto store = [&](int buf) {
+        if (MASK) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int row = srow + i * STEP;
-            if (MASK && at_scrub<T>(vr[i])) kr[i] = AT_NAN4;    // scores of that key become NaN for the rows that see it
-            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = kr[i];
-            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = vr[i];
+            for (int i = 0; i < kl.NL; ++i)
+                if (at_scrub<T>(vr[i])) kr[i] = AT_NAN4;    // scores of that key become NaN for the rows that see it
         }
+        kl.store(lds[buf][0], kr);
+        vl.store(lds[buf][1], vr);
     };
 
     f32x16 o[NB];
@@ -244,8 +278,9 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_fwd(const at_args<T> a)
         float mx = s[0][0];
 #pragma unroll
         for (int e = 1; e < 16 * U; ++e) mx = fmaxf(mx, s[e >> 4][e & 15]);
-        mx = fmaxf(mx, at_xor32(mx));
-        const float mn = fmaxf(m, mx);
+        float mx2;
+        at_both(mx, mx, mx2);
+        const float mn = fmaxf(m, fmaxf(mx, mx2));
         if (__any(mn > m)) {
             const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
             l *= al;
@@ -267,7 +302,9 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_fwd(const at_args<T> a)
         if (more) store(buf ^ 1);
         __syncthreads();
     }
-    l += at_xor32(l);
+    float l2;
+    at_both(l, l, l2);
+    l += l2;
     if (!live) return;
     const bool none = m == -INFINITY && !(l != l);
     const float inv = none ? 0.f : 1.f / l;
@@ -365,13 +402,12 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
 
 // dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp)
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_dq(const at_args<T> a)
+__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(const at_args<T> a)
 {
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U;
-    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
@@ -405,27 +441,20 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_dq(const at_args<T> a)
     const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
 
     const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
-    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
-    const bool cin = c16 * CH < a.d;
-    const T *kp = a.k + b * a.ks[0] + hk * a.ks[2] + c16 * CH, *vp = a.v + b * a.vs[0] + hk * a.vs[2] + c16 * CH;
-    u32x4 kr[NL], vr[NL];
+    const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
+    u32x4 kr[kl.NL], vr[kl.NL];
     auto load = [&](int kb) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int key = kb + srow + i * STEP;
-            const bool in = cin && key < k1;
-            kr[i] = in ? at_load_chunk(kp + key * a.ks[1]) : (u32x4)(0u);
-            vr[i] = in ? at_load_chunk(vp + key * a.vs[1]) : (u32x4)(0u);
-        }
+        kl.load(kr, kb, k1 - kb);
+        vl.load(vr, kb, k1 - kb);
     };
     auto store = [&](int buf) {
+        if (MASK) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int row = srow + i * STEP;
-            if (MASK && at_scrub<T>(kr[i])) vr[i] = AT_NAN4;    // dp of that key becomes NaN
-            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = kr[i];
-            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = vr[i];
+            for (int i = 0; i < kl.NL; ++i)
+                if (at_scrub<T>(kr[i])) vr[i] = AT_NAN4;    // dp of that key becomes NaN
         }
+        kl.store(lds[buf][0], kr);
+        vl.store(lds[buf][1], vr);
     };
 
     f32x16 o[NB];
@@ -478,25 +507,25 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_dq(const at_args<T> a)
         }
 }
 
+#define AT_RT 32
 // dk, dv: a workgroup owns 128 keys (a wave: 32, one per lane pair) and walks the rows; Q and dO tiles are read as rows (scores,
 // dp) and transposed (dk, dv)
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_dkv(const at_args<T> a)
+__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = 32;
-    constexpr int TB = KT * tile::RB, STEP = AT_THREADS / tile::CPR, NL = KT / STEP > 0 ? KT / STEP : 1;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = AT_RT, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];
-    __shared__ int mrow[2][KT];
 
     const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
-    const int R = tix * 32 * AT_WAVES < nk ? G * nq : 0;         // a tile of keys behind the image's last one: zeros
+    // the walk: row tiles of each query head of the group in turn; none where all keys lie behind the image's last one (zeros)
+    const int ht = (nq + KT - 1) / KT, W = tix * 32 * AT_WAVES < nk ? G * ht : 0;
     const int key = (tix * AT_WAVES + wave) * 32 + (lane & 31);
     const bool live = key < nk;
 
@@ -511,58 +540,52 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_dkv(const at_args<T> a)
     }
     const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + key : nullptr;
 
-    const int r0 = min(R, sp * a.per), r1 = min(R, r0 + a.per);
-    const int c16 = threadIdx.x % tile::CPR, srow = threadIdx.x / tile::CPR;
-    const bool cin = c16 * CH < a.d, sin = KT >= STEP || srow < KT;
-    const T *qp = a.q + b * a.qs[0] + c16 * CH, *gp = a.g + b * a.gs[0] + c16 * CH;
-    u32x4 qr[NL], gr[NL];
+    const int w0 = min(W, sp * a.per), w1 = min(W, w0 + a.per);
+    int wg = ht ? w0 / ht : 0, wn = ht ? w0 - wg * ht : 0;       // the next tile to load
+    u32x4 qr[at_loader<T, DP, KT>::NL], gr[at_loader<T, DP, KT>::NL];
+    const at_loader<T, DP, KT> ql(a.q + b * a.qs[0] + hk * G * a.qs[2], a.qs[1], a.d), gl(a.g + b * a.gs[0] + hk * G * a.gs[2], a.gs[1], a.d);
     float str = 0.f;
-    int mr = 0;
-    auto load = [&](int rb) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            const int r = rb + srow + i * STEP;
-            const bool in = cin && sin && r < r1;
-            const int gh = G == 1 ? 0 : r / nq, n = r - gh * nq, hq = hk * G + gh;
-            qr[i] = in ? at_load_chunk(qp + n * a.qs[1] + hq * a.qs[2]) : (u32x4)(0u);
-            gr[i] = in ? at_load_chunk(gp + n * a.gs[1] + hq * a.gs[2]) : (u32x4)(0u);
-        }
+    auto load = [&]() {
+        const int n0 = wn * KT, rows = nq - n0;
+        at_loader<T, DP, KT> q1 = ql, g1 = gl;
+        q1.base += wg * a.qs[2];
+        g1.base += wg * a.gs[2];
+        q1.load(qr, n0, rows);
+        g1.load(gr, n0, rows);
         if (threadIdx.x < 2 * KT) {               // the rows' statistics: first half log-sums, second half deltas
-            const int r = rb + (threadIdx.x & (KT - 1)), second = threadIdx.x >= KT;
-            const int gh = G == 1 ? 0 : r / nq, n = r - gh * nq;
-            const int64_t at = ((int64_t)b * a.hq + hk * G + gh) * a.nq + n;
-            str = r < r1 ? (second ? -a.delta[at] : a.lse2[at]) : (second ? 0.f : INFINITY);
-            mr = r < r1 ? n : 0;
+            const int n = threadIdx.x & (KT - 1), second = threadIdx.x >= KT;
+            const int64_t at = ((int64_t)b * a.hq + hk * G + wg) * a.nq + n0 + n;
+            str = n < rows ? (second ? -a.delta[at] : a.lse2[at]) : (second ? 0.f : INFINITY);
         }
+        if (++wn == ht) { wn = 0; ++wg; }
     };
     auto store = [&](int buf) {
+        if (MASK) {                               // the row's log-sum already says NaN (k_attn_delta)
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            if (!sin) break;
-            const int row = srow + i * STEP;
-            if (MASK) {                           // the row's log-sum already says NaN (k_attn_delta)
+            for (int i = 0; i < ql.NL; ++i) {
                 at_scrub<T>(qr[i]);
                 at_scrub<T>(gr[i]);
             }
-            *(u32x4 *)(lds[buf][0] + tile::at(row, c16)) = qr[i];
-            *(u32x4 *)(lds[buf][1] + tile::at(row, c16)) = gr[i];
         }
+        ql.store(lds[buf][0], qr);
+        gl.store(lds[buf][1], gr);
         if (threadIdx.x < 2 * KT) st[buf][threadIdx.x / KT][threadIdx.x & (KT - 1)] = str;
-        if (MASK && threadIdx.x < KT) mrow[buf][threadIdx.x] = mr;
     };
 
     f32x16 ok[NB], ov[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) ok[i] = ov[i] = (f32x16)(0.f);
-    if (r0 < r1) {
-        load(r0);
+    int mn = wn * KT;                             // first row of the tile being computed
+    if (w0 < w1) {
+        load();
         store(0);
     }
     __syncthreads();
     int buf = 0;
-    for (int rb = r0; rb < r1; rb += KT, buf ^= 1) {
-        const bool more = rb + KT < r1;
-        if (more) load(rb + KT);
+    for (int w = w0; w < w1; ++w, buf ^= 1) {
+        const bool more = w + 1 < w1;
+        const int next = wn * KT;
+        if (more) load();
         const char *Q = lds[buf][0], *GO = lds[buf][1];
         f32x16 s = (f32x16)(0.f), dp, ls;
 #pragma unroll
@@ -582,7 +605,7 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_dkv(const at_args<T> a)
             float ds = p * dp[e];
             if (MASK) {
                 const int row = 8 * (e >> 2) + 4 * h + (e & 3);
-                const bool see = live && rb + row < r1 && mp[mrow[buf][row] * a.ms[1]] != 0;
+                const bool see = live && mn + row < nq && mp[(mn + row) * a.ms[1]] != 0;
                 p = see ? p : 0.f;
                 ds = see ? ds : 0.f;
             }
@@ -591,6 +614,7 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_dkv(const at_args<T> a)
         }
         at_acc_t<DP>(ov, GO, 0, s, lane, (const T *)nullptr);
         at_acc_t<DP>(ok, Q, 0, dp, lane, (const T *)nullptr);
+        mn = next;
         if (more) store(buf ^ 1);
         __syncthreads();
     }
@@ -654,7 +678,8 @@ static at_plan at_plan_of(const dg_attn_shape *s)
     p.qtiles = dg_cdiv(g * s->nq, 32 * AT_WAVES);
     p.ktiles = dg_cdiv(s->nk, 32 * AT_WAVES);
     at_split(bh * p.qtiles, s->nk, &p.qsplits, &p.qper);
-    at_split(bh * p.ktiles, g * s->nq, &p.ksplits, &p.kper);
+    at_split(bh * p.ktiles, g * dg_cdiv(s->nq, AT_RT) * AT_RT, &p.ksplits, &p.kper);
+    p.kper /= AT_RT;                              // in row tiles
     p.rows = s->batch * s->q_heads * s->nq;
     p.stats = dg_round_up(p.rows * 4, 256);
     p.qpart = p.qsplits > 1 ? p.rows * p.qsplits * s->d * 4 : 0;
@@ -679,13 +704,14 @@ static int at_check(const dg_attn_shape *s, const char *who)
     return DG_OK;
 }
 
-// 16-byte loads: the pointer and every stride that a call steps along
+// 16-byte loads: the pointer and every stride that a call steps along; 64 rows of a tile span less than 2^31 bytes
+#define AT_ROW_MOST (1ll << 22)
 static bool at_aligned(const void *p, const int64_t *st, const dg_attn_shape *s, int64_t n, int64_t heads)
 {
     const int64_t e = s->dtype == DG_F32 ? 4 : 2, dims[3] = {s->batch, n, heads};
     if (((uintptr_t)p) & 15) return false;
     for (int i = 0; i < 3; ++i)
-        if (dims[i] > 1 && (st[i] < 0 || st[i] * e % 16)) return false;
+        if (dims[i] > 1 && (st[i] < 0 || st[i] * e % 16 || (i == 1 && st[i] > AT_ROW_MOST))) return false;
     return true;
 }
 
@@ -741,7 +767,7 @@ extern "C" int dg_roi_attn_fwd(const dg_attn_shape *s, const void *q, const void
     if (s->batch == 0 || s->nq == 0) return DG_OK;
     DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v)), "roi_attn_fwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
-                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && (((uintptr_t)out) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes");
+                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && (((uintptr_t)out) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 0);
     if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_fwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
     DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_fwd: workspace must be 16-byte aligned");
@@ -798,7 +824,7 @@ extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, con
     DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv, "roi_attn_bwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && at_aligned(grad_out, s->g_stride, s, s->nq, s->q_heads) &&
-                   ((((uintptr_t)out) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes");
+                   ((((uintptr_t)out) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 1);
     if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_bwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
     DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_bwd: workspace must be 16-byte aligned");

@@ -357,11 +357,13 @@ def _scratch(nbytes, dev):
 
 
 def _vec16(t):
-    """t with a dense last axis and everything a kernel steps along a multiple of 16 bytes; copied if it is not."""
+    """(B,N,H,D) with a dense last axis and everything a kernel steps along a multiple of 16 bytes (rows at most 2^22 values
+    apart); copied if it is not."""
     e = t.element_size()
     if t.numel() == 0:
         return t
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st * e % 16 == 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])):
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st * e % 16 == 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])) \
+            and (t.shape[1] == 1 or t.stride(1) <= 1 << 22):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
