@@ -51,12 +51,16 @@ __device__ __forceinline__ void at_both(float v, float &x, float &y)
     y = __uint_as_float(r[1]);
 }
 
-// A tile of rows in LDS, DP values wide, in 16-byte chunks whose place inside the row is swizzled by the row: eight lanes
-// reading the same chunk of eight successive rows, and sixteen lanes reading two chunks of four successive rows (the
-// transposing read), both cover 128 different bytes modulo 128.
+// A tile of rows in LDS, DP values wide, in 16-byte chunks whose place inside the row is swizzled by the row.  LDS gives 256 bytes
+// a clock to reads; sixteen lanes that read the same chunk of sixteen successive rows, and thirty-two that read four chunks of four
+// successive rows (the transposing read), both cover all 256 bytes modulo 256.  Measured on 16001 rows x 128: a swizzle for 128
+// bytes a clock spent 40% of the LDS's active cycles on conflicts.
 template <typename T, int DP> struct at_tile {
     static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16;
-    static __device__ __forceinline__ int swz(int row) { return CPR >= 8 ? (((row & 3) << 1) | ((row >> 2) & 1)) : ((row & 2) | ((row >> 2) & 1)); }
+    static __device__ __forceinline__ int swz(int row)
+    {
+        return CPR >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CPR == 8 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
+    }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
     // rows of the tile as an operand: row l & 31, chunk 2 g + l / 32
     static __device__ __forceinline__ typename at_vec<T>::frag row_frag(const char *t, int row, int chunk)
@@ -117,12 +121,15 @@ template <typename T> struct at_args {
 
 __device__ __forceinline__ int at_count(const int32_t *c, int b, int n) { return c ? min(max(c[b], 0), n) : n; }
 
-// workgroups go round the eight XCDs; this gives each XCD a run of successive ids, so the tiles that read the same keys meet
-// in one L2
-__device__ __forceinline__ int at_xcd_id()
+// Workgroups go round the eight XCDs.  The tiles of one (image, key head) stay on one XCD, so that they find its keys in one L2, and
+// (image, key head) pairs go round the XCDs one by one, so that images of different counts even out; what is left over of a
+// multiple of eight pairs is cut into eight runs of tiles.
+__device__ __forceinline__ int at_xcd_id(int per)  // per: tiles x splits of a pair -> pair * per + tile
 {
-    const int n = gridDim.x, x = blockIdx.x & 7, q = n >> 3, r = n & 7;
-    return x * q + min(x, r) + (int)(blockIdx.x >> 3);
+    const int x = blockIdx.x & 7, j = blockIdx.x >> 3, pairs = (int)(gridDim.x / per), whole = pairs & ~7;
+    if (j < (whole >> 3) * per) return (x + 8 * (j / per)) * per + j % per;
+    const int n = (pairs - whole) * per, q = n >> 3, r = n & 7;
+    return whole * per + x * q + min(x, r) + j - (whole >> 3) * per;
 }
 
 template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p) { return *(const u32x4 *)p; }
@@ -186,7 +193,7 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // KT keys of a tile (fp32 x 128: 32, for 64 KB of LDS); waves of a SIMD that the registers are cut for: two where two fit without
 // spilling, and the matrix results then stay in registers that the vector unit can read
 template <typename T, int DP> struct at_shape {
-    static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32, OCC = sizeof(T) * DP > 256 ? 1 : 2, OCC_KV = sizeof(T) * DP > 128 ? 1 : 2;
+    static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32, OCC = sizeof(T) * DP > 256 ? 1 : 2, OCC_KV = sizeof(T) * DP > 256 || (sizeof(T) == 4 && DP == 64) ? 1 : 2;
 };
 
 template <typename T, int DP, bool MASK>
@@ -198,7 +205,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
-    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -410,7 +417,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
     constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
-    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -519,8 +526,10 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
     constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = AT_RT, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];
+    constexpr bool VL = sizeof(T) == 2 && DP == 128;          // V stays in LDS: its registers are what would keep a second wave off the SIMD
+    __shared__ __attribute__((aligned(16))) char vt[VL ? 32 * AT_WAVES * tile::RB : 16];
 
-    const int id = at_xcd_id(), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
+    const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
@@ -530,13 +539,15 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
     const bool live = key < nk;
 
     const T *kp = a.k + b * a.ks[0] + (live ? key : 0) * a.ks[1] + hk * a.ks[2], *vp = a.v + b * a.vs[0] + (live ? key : 0) * a.vs[1] + hk * a.vs[2];
-    frag kf[NG], vf[NG];
+    frag kf[NG], vf[VL ? 1 : NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
         const int d = (2 * g + h) * CH;
         const bool in = live && d < a.d;
         kf[g] = in ? *(const frag *)(kp + d) : (frag)(0.f);
-        vf[g] = in ? *(const frag *)(vp + d) : (frag)(0.f);
+        const frag x = in ? *(const frag *)(vp + d) : (frag)(0.f);
+        if (VL) *(frag *)(vt + tile::at(wave * 32 + (lane & 31), 2 * g + h)) = x;
+        else vf[VL ? 0 : g] = x;
     }
     const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + key : nullptr;
 
@@ -587,33 +598,43 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
         const int next = wn * KT;
         if (more) load();
         const char *Q = lds[buf][0], *GO = lds[buf][1];
-        f32x16 s = (f32x16)(0.f), dp, ls;
+        // the LDS addresses of a tile are formed anew in every turn: kept across the loop they would cost a wave of the SIMD
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int lr = ln & 31, lh = ln >> 5;
+        f32x16 s = (f32x16)(0.f), dp;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) s = at_mma(tile::row_frag(Q, lr, 2 * g + lh), kf[g], s);
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
-            const f32x4 x = *(const f32x4 *)&st[buf][0][2 * e + 4 * h], y = *(const f32x4 *)&st[buf][1][2 * e + 4 * h];
+            const f32x4 y = *(const f32x4 *)&st[buf][1][2 * e + 4 * lh];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { ls[e + i] = x[i]; dp[e + i] = y[i]; }
+            for (int i = 0; i < 4; ++i) dp[e + i] = y[i];
         }
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            s = at_mma(tile::row_frag(Q, lane & 31, 2 * g + h), kf[g], s);
-            dp = at_mma(tile::row_frag(GO, lane & 31, 2 * g + h), vf[g], dp);
+        for (int g = 0; g < NG; ++g)
+            dp = at_mma(tile::row_frag(GO, lr, 2 * g + lh), VL ? tile::row_frag(vt, wave * 32 + lr, 2 * g + lh) : vf[VL ? 0 : g], dp);
+        
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const f32x4 ls = *(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh];
+            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -ls[e & 3]));
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -ls[e]));
-            float ds = p * dp[e];
+            float ds = s[e] * dp[e];
             if (MASK) {
                 const int row = 8 * (e >> 2) + 4 * h + (e & 3);
                 const bool see = live && mn + row < nq && mp[(mn + row) * a.ms[1]] != 0;
-                p = see ? p : 0.f;
+                s[e] = see ? s[e] : 0.f;
                 ds = see ? ds : 0.f;
             }
-            s[e] = p;
             dp[e] = ds;
         }
-        at_acc_t<DP>(ov, GO, 0, s, lane, (const T *)nullptr);
-        at_acc_t<DP>(ok, Q, 0, dp, lane, (const T *)nullptr);
+        
+        at_acc_t<DP>(ov, GO, 0, s, ln, (const T *)nullptr);
+        
+        at_acc_t<DP>(ok, Q, 0, dp, ln, (const T *)nullptr);
         mn = next;
         if (more) store(buf ^ 1);
         __syncthreads();
