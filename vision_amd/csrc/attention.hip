@@ -116,7 +116,7 @@ template <typename T> struct at_args {
     int64_t qs[3], ks[3], vs[3], gs[3];           // strides of batch, row, head, in values
     int64_t ms[2];                                // mask: batch, row
     int nq, nk, hq, hk, d, tiles, splits, per;    // per: rows or keys of a split, a multiple of the tile
-    float c, scale;                               // c = scale * log2(e)
+    float c, scale, slack;                        // c = scale * log2(e); slack = 8 / c
 };
 
 __device__ __forceinline__ int at_count(const int32_t *c, int b, int n) { return c ? min(max(c[b], 0), n) : n; }
@@ -138,6 +138,7 @@ template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p)
 // uniform, a lane's offset inside it fixed, and a lane with nothing to load (a row behind the end, a chunk behind d) asks for an
 // offset out of range and gets zeros.  A tile spans less than 2^31 bytes (at_aligned).
 #define AT_OUT 0x7fffffff
+#define AT_VM0 0x0f70                             // s_waitcnt vmcnt(0), the other counters free
 template <typename T, int DP, int ROWS> struct at_loader {
     typedef at_tile<T, DP> tile;
     static constexpr int STEP = AT_THREADS / tile::CPR, NL = ROWS / STEP > 0 ? ROWS / STEP : 1;
@@ -253,12 +254,13 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     f32x16 o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
-    float m = -INFINITY, l = 0.f;                 // running maximum (of s / scale) and this lane's part of the sum
+    float m = -INFINITY, l = 0.f;                 // maximum in use (of s / scale, at most slack below the true one), this lane's part of the sum
 
     if (k0 < k1) {
         load(k0);
         store(0);
     }
+    __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
     __syncthreads();
     int buf = 0;
     for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         float mx2;
         at_both(mx, mx, mx2);
         const float mn = fmaxf(m, fmaxf(mx, mx2));
-        if (__any(mn > m)) {
+        if (__any(mn > m + a.slack)) {            // otherwise the old maximum still does: no p exceeds 2^8
             const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
             l *= al;
 #pragma unroll
@@ -471,6 +473,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
         load(k0);
         store(0);
     }
+    __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
     __syncthreads();
     int buf = 0;
     for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
@@ -591,6 +594,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
         load();
         store(0);
     }
+    __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
     __syncthreads();
     int buf = 0;
     for (int w = w0; w < w1; ++w, buf ^= 1) {
@@ -755,6 +759,7 @@ static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, 
     a.nq = (int)s->nq; a.nk = (int)s->nk; a.hq = (int)s->q_heads; a.hk = (int)s->k_heads; a.d = (int)s->d;
     a.scale = s->scale;
     a.c = (float)((double)s->scale * 1.4426950408889634);
+    a.slack = fminf(8.f / a.c, 1e30f);
     return a;
 }
 
