@@ -336,7 +336,7 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * for all of q, k, v, out and the gradients).  d: a multiple of 8 from 8 to 128.
  *   s_ij = scale * q_i . k_j,  p_i = softmax over the keys that row i may see,  out_i = sum_j p_ij v_j,  lse_i = log sum_j exp s_ij
  * A row i sees key j if i < q_counts[image], j < k_counts[image] (device int32, held to [0, n]; NULL = all) and mask[image][i][j] != 0
- * (device bytes, batch and row stride in bytes -- a batch stride of 0 shares one mask; NULL = all).  What lies behind a count is
+ * (device bytes, a row's keys dense, strides of image and row in bytes; shape->masks of them, NULL with 0 = all).  What lies behind a count is
  * never read.  A row that sees nothing gives out = 0, lse = -inf and has no gradient; so do the rows behind q_counts, and dk = dv = 0
  * behind k_counts: every element of every output is written.  With a mask, a key that a row may not see does not reach it whatever
  * its values are; a row that sees a key or value holding a NaN or an infinity (and with a mask, in the backward pass, a row
@@ -347,7 +347,7 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
 typedef struct dg_attn_shape {   /* host */
     int64_t batch, nq, nk, q_heads, k_heads, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3];   /* batch, row, head; g: of grad_out (backward) */
-    int64_t mask_stride[2];                                       /* batch, row */
+    int64_t masks, mask_stride[2];                                /* 0: no mask, 1: one for all images, batch: one each; batch, row */
     float scale;                                                  /* positive, finite */
     int32_t dtype;
 } dg_attn_shape;

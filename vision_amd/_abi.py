@@ -27,7 +27,7 @@ class AttnShape(C.Structure):
     """dg_attn_shape of include/detgeom.h"""
     _fields_ = [(n, _i64) for n in ("batch", "nq", "nk", "q_heads", "k_heads", "d")] + \
                [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "g_stride")] + \
-               [("mask_stride", _i64 * 2), ("scale", _f32), ("dtype", _i32)]
+               [("masks", _i64), ("mask_stride", _i64 * 2), ("scale", _f32), ("dtype", _i32)]
 
 
 class RopeShape(C.Structure):

@@ -20,6 +20,7 @@
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -109,13 +110,13 @@ template <typename T> struct at_args {
     T *o, *dk;                                    // o: output / dq; dk, dv
     T *dv;
     float *lse;                                   // forward: output (b, hq, nq)
-    const float *lse2, *delta;                    // backward: statistics of the rows, base 2, (b, hq, nq)
+    const f32x2 *stat;                            // backward: (b, hq, nq) pairs of a row's log-sum in base 2 and -delta
     float *part;                                  // partial results of a split call
     const int32_t *qc, *kc;
-    const uint8_t *mask;
+    const u32 *bits;                              // pair mask, 32 keys a word: (masks, nq, words)
     int64_t qs[3], ks[3], vs[3], gs[3];           // strides of batch, row, head, in values
-    int64_t ms[2];                                // mask: batch, row
-    int nq, nk, hq, hk, d, tiles, splits, per;    // per: rows or keys of a split, a multiple of the tile
+    int64_t bs;                                   // words of an image's mask (0: one mask for all)
+    int words, batch, nq, nk, hq, hk, d, tiles, splits, per;    // per: rows or keys of a split, a multiple of the tile
     float c, scale, slack;                        // c = scale * log2(e); slack = 8 / c
 };
 
@@ -132,6 +133,29 @@ __device__ __forceinline__ int at_xcd_id(int per)  // per: tiles x splits of a p
     return whole * per + x * q + min(x, r) + j - (whole >> 3) * per;
 }
 
+// Images of different counts: the workgroups that come first take the images with the most pairs of rows and keys, so that what
+// runs last is short.  i-th image in that order (equal ones by index); every wave finds it for itself from the counts.
+__device__ __forceinline__ int at_image(int i, int batch, const int32_t *qc, const int32_t *kc, int nq, int nk)
+{
+    if ((!qc && !kc) || batch < 2 || batch > 64) return i;
+    const int lane = threadIdx.x & 63;
+    const float w = lane < batch ? (float)at_count(qc, lane, nq) * (float)at_count(kc, lane, nk) : -1.f;
+    int rank = 0;
+    for (int j = 0; j < batch; ++j) {
+        const float o = __uint_as_float((u32)__builtin_amdgcn_readlane((int)__float_as_uint(w), j));
+        rank += o > w || (o == w && j < lane);
+    }
+    return __ffsll((unsigned long long)__ballot(lane < batch && rank == i)) - 1;
+}
+
+// the word of a row's mask that holds keys kb .. kb + 31 (kb a multiple of 32), without those from k1 on
+__device__ __forceinline__ u32 at_word(const u32 *row, int kb, int k1)
+{
+    if (kb >= k1) return 0;
+    const u32 w = row[kb >> 5];
+    return k1 - kb < 32 ? w & ((1u << (k1 - kb)) - 1) : w;
+}
+
 template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p) { return *(const u32x4 *)p; }
 
 // A workgroup's loader of row tiles: thread t takes chunk t % CPR of rows t / CPR, + STEP, ...  Buffer loads: the tile's address is
@@ -139,19 +163,36 @@ template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p)
 // offset out of range and gets zeros.  A tile spans less than 2^31 bytes (at_aligned).
 #define AT_OUT 0x7fffffff
 #define AT_VM0 0x0f70                             // s_waitcnt vmcnt(0), the other counters free
-template <typename T, int DP, int ROWS> struct at_loader {
+template <typename T, int DP, int ROWS, bool LEAN = false> struct at_loader {
     typedef at_tile<T, DP> tile;
     static constexpr int STEP = AT_THREADS / tile::CPR, NL = ROWS / STEP > 0 ? ROWS / STEP : 1;
     const T *base;
     int64_t stride;
-    int row0, c16, off;                           // off: of the first row's chunk, in bytes
-    __device__ __forceinline__ at_loader(const T *p, int64_t st, int d) : base(p), stride(st), row0(threadIdx.x / tile::CPR), c16(threadIdx.x % tile::CPR)
+    int bytes, row0_, c16_, off_;                 // bytes: of a row; off: of the first row's chunk
+    __device__ __forceinline__ at_loader(const T *p, int64_t st, int d) : base(p), stride(st), bytes(d * (int)sizeof(T))
     {
-        off = c16 * 16 < d * (int)sizeof(T) ? row0 * (int)(st * (int)sizeof(T)) + c16 * 16 : AT_OUT;
+        place(threadIdx.x, row0_, c16_, off_);
+    }
+    __device__ __forceinline__ void place(int t, int &row0, int &c16, int &off) const
+    {
+        row0 = t / tile::CPR;
+        c16 = t % tile::CPR;
+        off = c16 * 16 < bytes ? row0 * (int)(stride * (int)sizeof(T)) + c16 * 16 : AT_OUT;
+    }
+    // LEAN: a thread's place is formed anew in every turn, where keeping it would cost registers that are not there
+    __device__ __forceinline__ void place(int &row0, int &c16, int &off) const
+    {
+        if (LEAN) {
+            int t = threadIdx.x;
+            asm volatile("" : "+v"(t));
+            place(t, row0, c16, off);
+        } else { row0 = row0_; c16 = c16_; off = off_; }
     }
     __device__ __forceinline__ void load(u32x4 (&r)[NL], int64_t first, int rows) const
     {
         const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(base + first * stride), 0, AT_OUT, 0x00027000);
+        int row0, c16, off;
+        place(row0, c16, off);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             const int o = row0 + i * STEP < rows ? off : AT_OUT;
@@ -160,6 +201,8 @@ template <typename T, int DP, int ROWS> struct at_loader {
     }
     __device__ __forceinline__ void store(char *lds, const u32x4 (&r)[NL]) const
     {
+        int row0, c16, off;
+        place(row0, c16, off);
 #pragma unroll
         for (int i = 0; i < NL; ++i)
             if (ROWS >= STEP || row0 < ROWS) *(u32x4 *)(lds + tile::at(row0 + i * STEP, c16)) = r[i];
@@ -191,10 +234,18 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // ------------------------------------------------------------------ forward
 // A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of 64.  K and V tiles are double
 // buffered in LDS; the next tile's global loads are in flight while this one is computed.
-// KT keys of a tile (fp32 x 128: 32, for 64 KB of LDS); waves of a SIMD that the registers are cut for: two where two fit without
-// spilling, and the matrix results then stay in registers that the vector unit can read
+// Never taken (d is 8 at least): it parts a turn of the loop between the products and the exponentials.  In one piece the scheduler
+// keeps so many operands of later products in registers that others are spilled (16001 x 128: dk, dv 2545 -> 2220 us, dq 1650 -> 1530).
+#define AT_PART(when) if ((when) && a.d <= 0) break
+
+// Keys of a tile (KT forward, KT_Q dq) and waves of a SIMD that the registers are cut for.  Up to 64 values a head in bf16, four
+// waves with tiles of 32 keys hide more than three with 64 (16 x 2000 rows: 174 to 180 us); at 128 two fit, and tiles of 64 halve
+// the barriers (forward); dq and (dk, dv) keep more in registers.  The limits also keep matrix results in registers that the
+// vector unit can read.
 template <typename T, int DP> struct at_shape {
-    static constexpr int KT = sizeof(T) * DP > 256 ? 32 : 64, U = KT / 32, OCC = sizeof(T) * DP > 256 ? 1 : 2, OCC_KV = sizeof(T) * DP > 256 || (sizeof(T) == 4 && DP == 64) ? 1 : 2;
+    static constexpr int BYTES = sizeof(T) * DP, H = sizeof(T) == 2;
+    static constexpr int KT = H && DP == 128 ? 64 : 32, KT_Q = 32;
+    static constexpr int OCC = BYTES > 256 ? 1 : H && DP <= 64 ? 4 : 2, OCC_Q = BYTES > 256 ? 1 : H && DP <= 64 ? 3 : 2, OCC_KV = H ? DP <= 64 ? 3 : 2 : BYTES > 128 ? 1 : 2;
 };
 
 template <typename T, int DP, bool MASK>
@@ -203,11 +254,11 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = KT / 32, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
 
@@ -232,7 +283,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         const int d = (2 * g + h) * CH;
         qf[g] = (live && d < a.d) ? *(const frag *)(qp + d) : (frag)(0.f);
     }
-    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
+    const u32 *mp = MASK ? a.bits + b * a.bs + (int64_t)n * a.words : nullptr;
 
     const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
     const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
@@ -256,9 +307,12 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
     float m = -INFINITY, l = 0.f;                 // maximum in use (of s / scale, at most slack below the true one), this lane's part of the sum
 
+    u32 mw[U], mnext[U];                            // MASK: this tile's words and the next one's
     if (k0 < k1) {
         load(k0);
         store(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mw[u] = MASK ? at_word(mp, k0 + 32 * u, k1) : 0;
     }
     __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
     __syncthreads();
@@ -266,6 +320,8 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
         const bool more = kb + KT < k1;
         if (more) load(kb + KT);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mnext[u] = MASK ? at_word(mp, kb + KT + 32 * u, k1) : 0;
         const char *K = lds[buf][0], *V = lds[buf][1];
         f32x16 s[U];
 #pragma unroll
@@ -276,13 +332,12 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         }
         if (MASK || !more) {
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const int left = k1 - kb - u * 32;
+                const u32 w = (MASK ? mw[u] : left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u) >> (4 * h);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = kb + u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    const bool see = key < k1 && (!MASK || mp[key] != 0);
-                    s[u][e] = see ? s[u][e] : -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e) s[u][e] = w & (1u << (8 * (e >> 2) + (e & 3))) ? s[u][e] : -INFINITY;
+            }
         }
         float mx = s[0][0];
 #pragma unroll
@@ -297,6 +352,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
             for (int i = 0; i < NB; ++i) o[i] *= al;
             m = mn;
         }
+        AT_PART(DP == 128);
         const float base = m == -INFINITY ? 0.f : m * a.c;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -309,6 +365,8 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
             at_acc_t<DP>(o, V, u * 32, s[u], lane, (const T *)nullptr);
         }
         if (more) store(buf ^ 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mw[u] = mnext[u];
         __syncthreads();
     }
     float l2;
@@ -320,7 +378,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     const float lse2 = none ? -INFINITY : fmaf(m, a.c, __builtin_amdgcn_logf(l));
     if (a.splits > 1) {
         // partial result of the split: normalised values and their log-sum, joined by k_attn_join
-        const int64_t row = ((int64_t)bh * G + gh) * a.nq + n, rows = (int64_t)(gridDim.x / a.tiles / a.splits) * G * a.nq;
+        const int64_t row = ((int64_t)b * a.hq + hq) * a.nq + n, rows = (int64_t)(gridDim.x / a.tiles / a.splits) * G * a.nq;
         float *po = a.part + rows * a.splits + (row * a.splits + sp) * a.d;
         if (h == 0) a.part[row * a.splits + sp] = lse2;
 #pragma unroll
@@ -344,39 +402,62 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         }
 }
 
-// joins the splits of a row: one wave per row
-template <typename T>
+// Joins the splits of a row by their log-sums.  A row has 32 lanes of four values; up to 16 splits eight rows share a workgroup, more
+// of them are dealt to the workgroup's eight lane groups, which then add up through LDS.
+#define AT_JOIN_FEW 16
+template <typename T, bool MANY>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, int64_t rows)
 {
-    const int64_t row = (int64_t)blockIdx.x * AT_WAVES + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    if (row >= rows) return;
+    typedef typename at_vec<T>::quad quad;
+    __shared__ __attribute__((aligned(16))) f32x4 red[MANY ? 8 : 1][32];
+    __shared__ float tot8[8], max8[8];
+    const int grp = threadIdx.x >> 5, sub = threadIdx.x & 31;
+    const int64_t row = MANY ? blockIdx.x : (int64_t)blockIdx.x * 8 + grp;
+    if (row >= rows) return;                      // MANY: the whole workgroup
     const int n = (int)(row % a.nq), hq = (int)(row / a.nq % a.hq), b = (int)(row / a.nq / a.hq);
     if (n >= at_count(a.qc, b, a.nq)) return;     // written by the first kernel
     const float *ls = a.part + row * a.splits, *po = a.part + rows * a.splits + row * a.splits * a.d;
+    const int s0 = MANY ? grp : 0, step = MANY ? 8 : 1;
     float m = -INFINITY;
-    for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ls[s]);
+    for (int s = MANY ? (int)threadIdx.x : sub; s < a.splits; s += MANY ? AT_THREADS : 32) m = fmaxf(m, ls[s]);
 #pragma unroll
-    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
-    const float base = m == -INFINITY ? 0.f : m;
-    float tot = 0.f;
-    for (int s = lane; s < a.splits; s += 64) tot += __builtin_amdgcn_exp2f(ls[s] - base);
+    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    if (MANY) {
+        if (sub == 0) max8[grp] = m;
+        __syncthreads();
 #pragma unroll
-    for (int x = 32; x; x >>= 1) tot += __shfl_xor(tot, x, 64);
-    const float inv = tot == 0.f ? 0.f : 1.f / tot;
-    for (int d = lane; d < a.d; d += 64) {
-        float v = 0.f;
-        for (int s = 0; s < a.splits; ++s) v = fmaf(__builtin_amdgcn_exp2f(ls[s] - base), po[(int64_t)s * a.d + d], v);
-        a.o[(((int64_t)b * a.nq + n) * a.hq + hq) * a.d + d] = (T)(v * inv);
+        for (int g = 0; g < 8; ++g) m = fmaxf(m, max8[g]);
     }
-    if (lane == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
+    const float base = m == -INFINITY ? 0.f : m;
+    const bool in = sub * 4 < a.d;
+    float tot = 0.f;
+    f32x4 v = (f32x4)(0.f);
+#pragma unroll 4
+    for (int s = s0; s < a.splits; s += step) {
+        const float w = __builtin_amdgcn_exp2f(ls[s] - base);
+        tot += w;
+        if (in) v += *(const f32x4 *)(po + (int64_t)s * a.d + sub * 4) * w;
+    }
+    if (MANY) {
+        red[grp][sub] = v;
+        if (sub == 0) tot8[grp] = tot;
+        __syncthreads();
+        if (grp) return;
+        for (int g = 1; g < 8; ++g) {
+            v += red[g][sub];
+            tot += tot8[g];
+        }
+    }
+    const float inv = tot == 0.f ? 0.f : 1.f / tot;
+    if (in) *(quad *)(a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d + sub * 4) = __builtin_convertvector(v * inv, quad);
+    if (sub == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
 }
 
 // ------------------------------------------------------------------ backward
 // delta_i = do_i . o_i and the rows' log-sums in base 2; a row that sees nothing gets +inf there, so that its p is 0
 template <typename T, bool MASK>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, const T *__restrict__ out, const float *__restrict__ lse, float *__restrict__ lse2,
-                                                           float *__restrict__ delta, int64_t rows)
+__global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, const T *__restrict__ out, const float *__restrict__ lse, f32x2 *__restrict__ stat,
+                                                           int64_t rows)
 {
     constexpr int CH = 16 / (int)sizeof(T), LPR = 128 / CH, RPB = AT_THREADS / LPR;
     const int sub = threadIdx.x % LPR;
@@ -405,22 +486,21 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
     }
     if (sub) return;
     const float l = live ? lse[at] : -INFINITY;
-    lse2[at] = bad ? __builtin_nanf("") : l == -INFINITY ? INFINITY : l * AT_LOG2E;
-    delta[at] = sum;
+    stat[at] = (f32x2){bad ? __builtin_nanf("") : l == -INFINITY ? INFINITY : l * AT_LOG2E, -sum};
 }
 
 // dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp)
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(const at_args<T> a)
+__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_dq(const at_args<T> a)
 {
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = at_shape<T, DP>::U, TB = KT * tile::RB;
+    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT_Q, U = KT / 32, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
 
@@ -446,8 +526,9 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
         gf[g] = in ? *(const frag *)(gp + d) : (frag)(0.f);
     }
     const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
-    const float lse2 = live ? a.lse2[at] : INFINITY, delta = live ? a.delta[at] : 0.f;
-    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + n * a.ms[1] : nullptr;
+    const f32x2 stat = live ? a.stat[at] : (f32x2){INFINITY, 0.f};
+    const float lse2 = stat[0];
+    const u32 *mp = MASK ? a.bits + b * a.bs + (int64_t)n * a.words : nullptr;
 
     const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
     const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
@@ -469,9 +550,12 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
     f32x16 o[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
+    u32 mw[U], mnext[U];                            // MASK: this tile's words and the next one's
     if (k0 < k1) {
         load(k0);
         store(0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mw[u] = MASK ? at_word(mp, k0 + 32 * u, k1) : 0;
     }
     __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
     __syncthreads();
@@ -479,31 +563,35 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
     for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
         const bool more = kb + KT < k1;
         if (more) load(kb + KT);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mnext[u] = MASK ? at_word(mp, kb + KT + 32 * u, k1) : 0;
         const char *K = lds[buf][0], *V = lds[buf][1];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            f32x16 s = (f32x16)(0.f), dp = (f32x16)(-delta);
+            f32x16 s = (f32x16)(0.f), dp = (f32x16)(stat[1]);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 s = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
                 dp = at_mma(tile::row_frag(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
             }
+            const int left = k1 - kb - u * 32;
+            const u32 w = (MASK ? mw[u] : left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u) >> (4 * h);
+            AT_PART(DP == 128);
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse2)) * dp[e];
-                if (MASK || !more) {
-                    const int key = kb + u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-                    ds = key < k1 && (!MASK || mp[key] != 0) ? ds : 0.f;
-                }
+                if (MASK || !more) ds = w & (1u << (8 * (e >> 2) + (e & 3))) ? ds : 0.f;
                 s[e] = ds;
             }
             at_acc_t<DP>(o, K, u * 32, s, lane, (const T *)nullptr);
         }
         if (more) store(buf ^ 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) mw[u] = mnext[u];
         __syncthreads();
     }
     if (!live) return;
-    float *po = a.part + (((int64_t)bh * G + gh) * a.nq + n) * a.splits * a.d + (int64_t)sp * a.d;
+    float *po = a.part + (((int64_t)b * a.hq + hq) * a.nq + n) * a.splits * a.d + (int64_t)sp * a.d;
     T *op = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
 #pragma unroll
     for (int i = 0; i < NB; ++i)
@@ -521,7 +609,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_dq(
 // dk, dv: a workgroup owns 128 keys (a wave: 32, one per lane pair) and walks the rows; Q and dO tiles are read as rows (scores,
 // dp) and transposed (dk, dv)
 template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
+__global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
     typedef at_tile<T, DP> tile;
     typedef typename at_vec<T>::frag frag;
@@ -529,11 +617,12 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
     constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = AT_RT, TB = KT * tile::RB;
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];
+    constexpr bool LEAN = sizeof(T) == 2 && DP >= 64;
     constexpr bool VL = sizeof(T) == 2 && DP == 128;          // V stays in LDS: its registers are what would keep a second wave off the SIMD
     __shared__ __attribute__((aligned(16))) char vt[VL ? 32 * AT_WAVES * tile::RB : 16];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = bh / a.hk, hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     // the walk: row tiles of each query head of the group in turn; none where all keys lie behind the image's last one (zeros)
@@ -549,27 +638,31 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
         const bool in = live && d < a.d;
         kf[g] = in ? *(const frag *)(kp + d) : (frag)(0.f);
         const frag x = in ? *(const frag *)(vp + d) : (frag)(0.f);
-        if (VL) *(frag *)(vt + tile::at(wave * 32 + (lane & 31), 2 * g + h)) = x;
+        if (VL) *(frag *)(vt + (wave * NG + g) * 1024 + lane * 16) = x;
         else vf[VL ? 0 : g] = x;
     }
-    const uint8_t *mp = MASK ? a.mask + b * a.ms[0] + key : nullptr;
 
     const int w0 = min(W, sp * a.per), w1 = min(W, w0 + a.per);
     int wg = ht ? w0 / ht : 0, wn = ht ? w0 - wg * ht : 0;       // the next tile to load
-    u32x4 qr[at_loader<T, DP, KT>::NL], gr[at_loader<T, DP, KT>::NL];
-    const at_loader<T, DP, KT> ql(a.q + b * a.qs[0] + hk * G * a.qs[2], a.qs[1], a.d), gl(a.g + b * a.gs[0] + hk * G * a.gs[2], a.gs[1], a.d);
-    float str = 0.f;
+    u32x4 qr[at_loader<T, DP, KT, LEAN>::NL], gr[at_loader<T, DP, KT, LEAN>::NL];
+    const at_loader<T, DP, KT, LEAN> ql(a.q + b * a.qs[0] + hk * G * a.qs[2], a.qs[1], a.d), gl(a.g + b * a.gs[0] + hk * G * a.gs[2], a.gs[1], a.d);
+    __shared__ __attribute__((aligned(16))) u32 mws[2][AT_WAVES][MASK ? KT : 4];
+    const u32 *mp = MASK ? a.bits + b * a.bs : nullptr;
+    u64 sr = 0;
+    u32 mr = 0;
     auto load = [&]() {
         const int n0 = wn * KT, rows = nq - n0;
-        at_loader<T, DP, KT> q1 = ql, g1 = gl;
+        at_loader<T, DP, KT, LEAN> q1 = ql, g1 = gl;
         q1.base += wg * a.qs[2];
         g1.base += wg * a.gs[2];
         q1.load(qr, n0, rows);
         g1.load(gr, n0, rows);
-        if (threadIdx.x < 2 * KT) {               // the rows' statistics: first half log-sums, second half deltas
-            const int n = threadIdx.x & (KT - 1), second = threadIdx.x >= KT;
-            const int64_t at = ((int64_t)b * a.hq + hk * G + wg) * a.nq + n0 + n;
-            str = n < rows ? (second ? -a.delta[at] : a.lse2[at]) : (second ? 0.f : INFINITY);
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(a.stat + ((int64_t)b * a.hq + hk * G + wg) * a.nq + n0), 0, AT_OUT, 0x00027000);
+        // the rows' statistics; zeros behind the end, where q and grad_out are zeros too
+        sr = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(rs, (int)threadIdx.x < min(KT, rows) ? (int)threadIdx.x * 8 : AT_OUT, 0, 0));
+        if (MASK && threadIdx.x < KT * AT_WAVES) {   // the words of the tile's rows for each wave's keys
+            const int n = threadIdx.x / AT_WAVES, kw = tix * AT_WAVES + threadIdx.x % AT_WAVES;
+            mr = n < rows && kw < a.words ? mp[(int64_t)(n0 + n) * a.words + kw] : 0;
         }
         if (++wn == ht) { wn = 0; ++wg; }
     };
@@ -583,13 +676,16 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
         }
         ql.store(lds[buf][0], qr);
         gl.store(lds[buf][1], gr);
-        if (threadIdx.x < 2 * KT) st[buf][threadIdx.x / KT][threadIdx.x & (KT - 1)] = str;
+        if (MASK && threadIdx.x < KT * AT_WAVES) mws[buf][threadIdx.x % AT_WAVES][threadIdx.x / AT_WAVES] = mr;
+        if (threadIdx.x < KT) {
+            st[buf][0][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[0];
+            st[buf][1][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[1];
+        }
     };
 
     f32x16 ok[NB], ov[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) ok[i] = ov[i] = (f32x16)(0.f);
-    int mn = wn * KT;                             // first row of the tile being computed
     if (w0 < w1) {
         load();
         store(0);
@@ -599,7 +695,6 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
     int buf = 0;
     for (int w = w0; w < w1; ++w, buf ^= 1) {
         const bool more = w + 1 < w1;
-        const int next = wn * KT;
         if (more) load();
         const char *Q = lds[buf][0], *GO = lds[buf][1];
         // the LDS addresses of a tile are formed anew in every turn: kept across the loop they would cost a wave of the SIMD
@@ -610,26 +705,18 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
 #pragma unroll
         for (int g = 0; g < NG; ++g) s = at_mma(tile::row_frag(Q, lr, 2 * g + lh), kf[g], s);
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const f32x4 y = *(const f32x4 *)&st[buf][1][2 * e + 4 * lh];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dp[e + i] = y[i];
-        }
+        for (int e = 0; e < 16; ++e) dp[e] = (*(const f32x4 *)&st[buf][1][2 * (e & ~3) + 4 * lh])[e & 3];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            dp = at_mma(tile::row_frag(GO, lr, 2 * g + lh), VL ? tile::row_frag(vt, wave * 32 + lr, 2 * g + lh) : vf[VL ? 0 : g], dp);
-        
+            dp = at_mma(tile::row_frag(GO, lr, 2 * g + lh), VL ? *(const frag *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
+        AT_PART(DP >= 64);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const f32x4 ls = *(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh];
-            s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -ls[e & 3]));
-        }
+        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -(*(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh])[e & 3]));
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             float ds = s[e] * dp[e];
             if (MASK) {
-                const int row = 8 * (e >> 2) + 4 * h + (e & 3);
-                const bool see = live && mn + row < nq && mp[(mn + row) * a.ms[1]] != 0;
+                const bool see = live && ((*(const u32x4 *)&mws[buf][wave][2 * (e & ~3) + 4 * lh])[e & 3] >> lr) & 1;
                 s[e] = see ? s[e] : 0.f;
                 ds = see ? ds : 0.f;
             }
@@ -639,12 +726,11 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_KV)) void k_attn_
         at_acc_t<DP>(ov, GO, 0, s, ln, (const T *)nullptr);
         
         at_acc_t<DP>(ok, Q, 0, dp, ln, (const T *)nullptr);
-        mn = next;
         if (more) store(buf ^ 1);
         __syncthreads();
     }
     if (key >= a.nk) return;
-    const int64_t rows = (int64_t)(gridDim.x / a.tiles / a.splits) * a.nk, prow = (int64_t)bh * a.nk + key;
+    const int64_t rows = (int64_t)(gridDim.x / a.tiles / a.splits) * a.nk, prow = ((int64_t)b * a.hk + hk) * a.nk + key;
     float *pk = a.part + prow * a.splits * a.d + (int64_t)sp * a.d, *pv = pk + rows * a.splits * a.d;
     const int64_t orow = (((int64_t)b * a.nk + key) * a.hk + hk) * a.d;
 #pragma unroll
@@ -670,31 +756,52 @@ template <typename T>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict__ part, T *__restrict__ out, const int32_t *__restrict__ counts, int64_t rows, int heads,
                                                          int nmax, int d, int splits)
 {
-    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x, row = i / d;
+    typedef typename at_vec<T>::quad quad;
+    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x, row = i / (d / 4);
     if (row >= rows) return;
-    const int x = (int)(i - row * d), n = (int)(row % nmax), hh = (int)(row / nmax % heads), b = (int)(row / nmax / heads);
+    const int x = (int)(i - row * (d / 4)) * 4, n = (int)(row % nmax), hh = (int)(row / nmax % heads), b = (int)(row / nmax / heads);
     if (n >= at_count(counts, b, nmax)) return;
     const float *p = part + row * splits * d + x;
-    float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += p[(int64_t)s * d];
-    out[(((int64_t)b * nmax + n) * heads + hh) * d + x] = (T)v;
+    f32x4 v = (f32x4)(0.f);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(p + (int64_t)s * d);
+    *(quad *)(out + (((int64_t)b * nmax + n) * heads + hh) * d + x) = __builtin_convertvector(v, quad);
+}
+
+// pair mask -> bits: a word of 32 keys per thread
+__global__ __launch_bounds__(AT_THREADS) void k_attn_bits(const uint8_t *__restrict__ mask, int64_t sb, int64_t sr, u32 *__restrict__ bits, int64_t n, int nq, int nk, int words)
+{
+    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x;
+    if (i >= n) return;
+    const int w = (int)(i % words), k0 = w * 32;
+    const int64_t r = i / words;
+    const uint8_t *m = mask + r / nq * sb + r % nq * sr + k0;
+    u32 x = 0;
+    if (nk - k0 >= 32) {
+        uint8_t v[32];
+        __builtin_memcpy(v, m, 32);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x |= v[j] ? 1u << j : 0u;
+    } else
+        for (int j = 0; j < nk - k0; ++j) x |= m[j] ? 1u << j : 0u;
+    bits[i] = x;
 }
 
 // ------------------------------------------------------------------ host
 // A call that has too few tiles to fill the chip is split along the axis it walks: enough splits for two workgroups on each of
-// the 256 CUs, none shorter than 256 steps of that axis.
+// the 256 CUs, none shorter than 128 steps of that axis.
 static void at_split(int64_t blocks, int64_t walk, int64_t *splits, int64_t *per)
 {
     int64_t s = 1;
     if (blocks < 256) s = dg_cdiv(512, blocks > 0 ? blocks : 1);
-    const int64_t most = dg_cdiv(walk, 256);
+    const int64_t most = dg_cdiv(walk, 128);
     if (s > most) s = most;
     if (s < 1) s = 1;
     *per = dg_round_up(dg_cdiv(walk > 0 ? walk : 1, s), 64);
     *splits = dg_cdiv(walk > 0 ? walk : 1, *per);
 }
 
-struct at_plan { int64_t qtiles, ktiles, qsplits, qper, ksplits, kper, rows, stats, qpart, kpart; };
+struct at_plan { int64_t words, bits, qtiles, ktiles, qsplits, qper, ksplits, kper, rows, stats, qpart, kpart; };
 
 static at_plan at_plan_of(const dg_attn_shape *s)
 {
@@ -706,7 +813,9 @@ static at_plan at_plan_of(const dg_attn_shape *s)
     at_split(bh * p.ktiles, g * dg_cdiv(s->nq, AT_RT) * AT_RT, &p.ksplits, &p.kper);
     p.kper /= AT_RT;                              // in row tiles
     p.rows = s->batch * s->q_heads * s->nq;
-    p.stats = dg_round_up(p.rows * 4, 256);
+    p.words = dg_cdiv(s->nk, 32);
+    p.bits = dg_round_up(s->masks * s->nq * p.words * 4, 256);
+    p.stats = dg_round_up(p.rows * 8, 256);
     p.qpart = p.qsplits > 1 ? p.rows * p.qsplits * s->d * 4 : 0;
     p.kpart = p.ksplits > 1 ? 2 * s->batch * s->k_heads * s->nk * p.ksplits * s->d * 4 : 0;
     return p;
@@ -720,12 +829,13 @@ static int at_check(const dg_attn_shape *s, const char *who)
     DG_REQUIRE(s->k_heads >= 1 && s->q_heads >= 1 && s->q_heads % s->k_heads == 0, "%s: q_heads must be a positive multiple of k_heads", who);
     DG_REQUIRE(s->d >= 8 && s->d <= 128 && s->d % 8 == 0, "%s: head size %lld is not a multiple of 8 from 8 to 128", who, (long long)s->d);
     DG_REQUIRE(s->scale > 0.f && s->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
+    DG_REQUIRE(s->masks == 0 || s->masks == 1 || s->masks == s->batch, "%s: masks is 0, 1 (for all images) or the batch", who);
     const int64_t most = 1ll << 28;
     DG_REQUIRE(s->batch <= most && s->nk <= most && s->q_heads <= most && s->nq <= most && s->nq * (s->q_heads / s->k_heads) <= most &&
                    s->batch * s->q_heads <= most, "%s: more than 2^28 rows or keys", who);
     const at_plan p = at_plan_of(s);
     DG_REQUIRE(s->batch * s->k_heads * p.qtiles * p.qsplits < (1ll << 31) && s->batch * s->k_heads * p.ktiles * p.ksplits < (1ll << 31) &&
-                   dg_cdiv(p.rows, 4) < (1ll << 31), "%s: more than 2^31 tiles", who);
+                   dg_cdiv(p.rows, 4) < (1ll << 31) && dg_cdiv(s->masks * s->nq * p.words, AT_THREADS) < (1ll << 31), "%s: more than 2^31 tiles", who);
     return DG_OK;
 }
 
@@ -744,31 +854,43 @@ extern "C" size_t dg_roi_attn_workspace_bytes(const dg_attn_shape *s, int backwa
 {
     if (at_check(s, "roi_attn") != DG_OK) return 0;
     const at_plan p = at_plan_of(s);
-    if (!backward) return (size_t)(p.qpart ? p.qpart + p.rows * p.qsplits * 4 : 0);
-    return (size_t)(2 * p.stats + (p.qpart > p.kpart ? p.qpart : p.kpart));
+    if (!backward) return (size_t)(p.bits + (p.qpart ? p.qpart + p.rows * p.qsplits * 4 : 0));
+    return (size_t)(p.bits + p.stats + (p.qpart > p.kpart ? p.qpart : p.kpart));
 }
 
 template <typename T>
-static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *qc, const int32_t *kc, const uint8_t *mask)
+static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *qc, const int32_t *kc)
 {
     at_args<T> a = {};
     a.q = (const T *)q; a.k = (const T *)k; a.v = (const T *)v;
-    a.qc = qc; a.kc = kc; a.mask = mask;
+    a.qc = qc; a.kc = kc;
     for (int i = 0; i < 3; ++i) { a.qs[i] = s->q_stride[i]; a.ks[i] = s->k_stride[i]; a.vs[i] = s->v_stride[i]; a.gs[i] = s->g_stride[i]; }
-    a.ms[0] = s->mask_stride[0]; a.ms[1] = s->mask_stride[1];
-    a.nq = (int)s->nq; a.nk = (int)s->nk; a.hq = (int)s->q_heads; a.hk = (int)s->k_heads; a.d = (int)s->d;
+    a.batch = (int)s->batch; a.nq = (int)s->nq; a.nk = (int)s->nk; a.hq = (int)s->q_heads; a.hk = (int)s->k_heads; a.d = (int)s->d;
     a.scale = s->scale;
     a.c = (float)((double)s->scale * 1.4426950408889634);
     a.slack = fminf(8.f / a.c, 1e30f);
     return a;
 }
 
+// the mask's bits at the front of the workspace; what follows them is returned
+template <typename T> static void *at_bits(const dg_attn_shape *s, const at_plan &p, const uint8_t *mask, at_args<T> &a, void *ws, hipStream_t st)
+{
+    if (!p.bits) return ws;
+    const int64_t n = s->masks * s->nq * p.words;
+    hipLaunchKernelGGL(k_attn_bits, dim3((unsigned)dg_cdiv(n, AT_THREADS)), dim3(AT_THREADS), 0, st, mask, s->mask_stride[0], s->mask_stride[1], (u32 *)ws, n, (int)s->nq,
+                       (int)s->nk, (int)p.words);
+    a.bits = (const u32 *)ws;
+    a.words = (int)p.words;
+    a.bs = s->masks > 1 ? s->nq * p.words : 0;
+    return (char *)ws + p.bits;
+}
+
 #define AT_LAUNCH(kernel, grid, a)                                                                                              \
     do {                                                                                                                        \
         const dim3 gr_((unsigned)(grid)), bl_(AT_THREADS);                                                                       \
-        if ((a).d <= 32) { if ((a).mask) hipLaunchKernelGGL((kernel<T, 32, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 32, false>), gr_, bl_, 0, st, a); } \
-        else if ((a).d <= 64) { if ((a).mask) hipLaunchKernelGGL((kernel<T, 64, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 64, false>), gr_, bl_, 0, st, a); } \
-        else { if ((a).mask) hipLaunchKernelGGL((kernel<T, 128, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 128, false>), gr_, bl_, 0, st, a); } \
+        if ((a).d <= 32) { if ((a).bits) hipLaunchKernelGGL((kernel<T, 32, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 32, false>), gr_, bl_, 0, st, a); } \
+        else if ((a).d <= 64) { if ((a).bits) hipLaunchKernelGGL((kernel<T, 64, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 64, false>), gr_, bl_, 0, st, a); } \
+        else { if ((a).bits) hipLaunchKernelGGL((kernel<T, 128, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 128, false>), gr_, bl_, 0, st, a); } \
     } while (0)
 
 template <typename T>
@@ -776,11 +898,13 @@ static int at_forward(const dg_attn_shape *s, const void *q, const void *k, cons
                       float *lse, void *ws, hipStream_t st)
 {
     const at_plan p = at_plan_of(s);
-    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc, mask);
+    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc);
+    ws = at_bits(s, p, mask, a, ws, st);
     a.o = (T *)out; a.lse = lse; a.part = (float *)ws;
     a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
     AT_LAUNCH(k_attn_fwd, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
-    if (p.qsplits > 1) hipLaunchKernelGGL((k_attn_join<T>), dim3((unsigned)dg_cdiv(p.rows, AT_WAVES)), dim3(AT_THREADS), 0, st, a, p.rows);
+    if (p.qsplits > AT_JOIN_FEW) hipLaunchKernelGGL((k_attn_join<T, true>), dim3((unsigned)p.rows), dim3(AT_THREADS), 0, st, a, p.rows);
+    else if (p.qsplits > 1) hipLaunchKernelGGL((k_attn_join<T, false>), dim3((unsigned)dg_cdiv(p.rows, 8)), dim3(AT_THREADS), 0, st, a, p.rows);
     DG_CHECK_LAUNCH("k_attn_fwd");
     return DG_OK;
 }
@@ -791,7 +915,7 @@ extern "C" int dg_roi_attn_fwd(const dg_attn_shape *s, const void *q, const void
     const int rc = at_check(s, "roi_attn_fwd");
     if (rc != DG_OK) return rc;
     if (s->batch == 0 || s->nq == 0) return DG_OK;
-    DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v)), "roi_attn_fwd: null pointer");
+    DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v && !mask == !s->masks)), "roi_attn_fwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && (((uintptr_t)out) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 0);
@@ -806,21 +930,22 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
                        const int32_t *kc, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, hipStream_t st)
 {
     const at_plan p = at_plan_of(s);
-    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc, mask);
-    float *lse2 = (float *)ws, *delta = (float *)((char *)ws + p.stats);
-    a.g = (const T *)g; a.lse2 = lse2; a.delta = delta; a.part = (float *)((char *)ws + 2 * p.stats);
+    at_args<T> a = at_fill<T>(s, q, k, v, qc, kc);
+    ws = at_bits(s, p, mask, a, ws, st);
+    f32x2 *stat = (f32x2 *)ws;
+    a.g = (const T *)g; a.stat = stat; a.part = (float *)((char *)ws + p.stats);
     if (s->nq > 0) {
         const int64_t rpb = AT_THREADS * (16 / (int64_t)sizeof(T)) / 128;
         const dim3 grid((unsigned)dg_cdiv(p.rows, rpb));
-        if (mask) hipLaunchKernelGGL((k_attn_delta<T, true>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, lse2, delta, p.rows);
-        else hipLaunchKernelGGL((k_attn_delta<T, false>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, lse2, delta, p.rows);
+        if (a.bits) hipLaunchKernelGGL((k_attn_delta<T, true>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, p.rows);
+        else hipLaunchKernelGGL((k_attn_delta<T, false>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, p.rows);
     }
     if (s->nq > 0 && dq) {
         a.o = (T *)dq;
         a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
         AT_LAUNCH(k_attn_dq, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
         if (p.qsplits > 1)
-            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, qc, p.rows,
+            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d / 4, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, qc, p.rows,
                                (int)s->q_heads, (int)s->nq, (int)s->d, (int)p.qsplits);
     }
     if (s->nk > 0 && dk) {
@@ -829,7 +954,7 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
         AT_LAUNCH(k_attn_dkv, s->batch * s->k_heads * p.ktiles * p.ksplits, a);
         if (p.ksplits > 1) {
             const int64_t rows = s->batch * s->k_heads * s->nk, half = rows * p.ksplits * s->d;
-            const dim3 grid((unsigned)dg_cdiv(rows * s->d, AT_THREADS));
+            const dim3 grid((unsigned)dg_cdiv(rows * s->d / 4, AT_THREADS));
             hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dk, (const int32_t *)nullptr, rows, (int)s->k_heads,
                                (int)s->nk, (int)s->d, (int)p.ksplits);
             hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part + half, (T *)dv, (const int32_t *)nullptr, rows, (int)s->k_heads,
@@ -847,7 +972,7 @@ extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, con
     const int rc = at_check(s, "roi_attn_bwd");
     if (rc != DG_OK) return rc;
     if (s->batch == 0 || (s->nq == 0 && s->nk == 0)) return DG_OK;
-    DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv, "roi_attn_bwd: null pointer");
+    DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv && (s->nk == 0 || s->nq == 0 || !mask == !s->masks), "roi_attn_bwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && at_aligned(grad_out, s->g_stride, s, s->nq, s->q_heads) &&
                    ((((uintptr_t)out) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");

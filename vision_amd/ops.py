@@ -403,7 +403,8 @@ def _attn_call(q, k, v, q_counts, k_counts, mask, scale):
             raise ValueError("roi_attention: mask must be (Nq,Nk) or (B or 1,Nq,Nk)")
         if Nk > 1 and mask.stride(2) != 1:
             mask = mask.contiguous()
-        s.mask_stride[:] = (mask.stride(0) if mask.shape[0] > 1 else 0, mask.stride(1))
+        s.masks = mask.shape[0]
+        s.mask_stride[:] = mask.stride()[:2]
     return dev, q, k, v, qc, kc, mask, s
 
 
