@@ -24,16 +24,17 @@ TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _vp, _i64, _i32, _f32, _f64, _sz = C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_double, C.c_size_t
 
 class AttnShape(C.Structure):
-    """dg_attn_shape of include/detgeom.h"""
+    """dg_attn_shape of include/detgeom.h, its arrays field by field"""
     _fields_ = [(n, _i64) for n in ("batch", "nq", "nk", "q_heads", "k_heads", "d")] + \
-               [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "g_stride")] + \
-               [("masks", _i64), ("mask_stride", _i64 * 2), ("scale", _f32), ("dtype", _i32)]
+               [(t + "_stride_" + a, _i64) for t in "qkvg" for a in ("batch", "row", "head")] + \
+               [("masks", _i64), ("mask_stride_batch", _i64), ("mask_stride_row", _i64), ("scale", _f32), ("dtype", _i32)]
 
 
 class RopeShape(C.Structure):
-    """dg_rope_shape of include/detgeom.h"""
+    """dg_rope_shape of include/detgeom.h, its arrays field by field"""
     _fields_ = [(n, _i64) for n in ("batch", "n", "q_heads", "k_heads", "d", "pairs", "axes")] + \
-               [("q_stride", _i64 * 3), ("k_stride", _i64 * 3), ("pos_stride", _i64 * 2)] + [(n, _i32) for n in ("dtype", "pos_dtype", "pairing")]
+               [(t + "_stride_" + a, _i64) for t in "qk" for a in ("batch", "row", "head")] + \
+               [("pos_stride_batch", _i64), ("pos_stride_row", _i64)] + [(n, _i32) for n in ("dtype", "pos_dtype", "pairing")]
 
 
 # name -> (restype, argtypes); must list every symbol include/detgeom.h declares
@@ -169,6 +170,21 @@ def stream_ptr(device=None):
 
 def ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
+
+
+class on_device:
+    """torch.cuda.device(device) that costs nothing where it already is the current one"""
+
+    def __init__(self, device):
+        self.other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.other is not None:
+            self.other.__enter__()
+
+    def __exit__(self, *exc):
+        if self.other is not None:
+            self.other.__exit__(*exc)
 
 
 # scratch, grown on demand (the C ABI allocates nothing).  One buffer per (device, stream): calls in flight on different

@@ -37,6 +37,22 @@ __device__ __forceinline__ u64 lp_lane(u64 v, int l)
     return ((u64)(u32)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32) | (u32)__builtin_amdgcn_readlane((int)v, l);
 }
 
+// maximum over the wave, by lane moves of the vector unit: 1, 2, 4, 8 lanes on inside sixteen, then across; the last lane has it
+template <int MOVE> __device__ __forceinline__ float lp_max_move(float v)
+{
+    return fmaxf(v, __uint_as_float((u32)__builtin_amdgcn_update_dpp((int)0xff800000, (int)__float_as_uint(v), MOVE, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float lp_wave_max(float v)
+{
+    v = lp_max_move<0x111>(v);                    // row_shr:1, 2, 4, 8
+    v = lp_max_move<0x112>(v);
+    v = lp_max_move<0x114>(v);
+    v = lp_max_move<0x118>(v);
+    v = lp_max_move<0x142>(v);                    // row_bcast:15, 31
+    v = lp_max_move<0x143>(v);
+    return __uint_as_float((u32)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
+}
+
 // the best keys seen by a wave, ascending (best first): lane i holds the i-th
 struct lp_list {
     u64 list = LP_NONE, thr = LP_NONE;
@@ -66,9 +82,10 @@ struct lp_sum {
             m = mx;
         }
     }
-    __device__ __forceinline__ void add(float z)  // z <= m, or NaN
+    __device__ __forceinline__ float from() const { return m == -INFINITY ? 0.f : m; }
+    __device__ __forceinline__ void add(float z, float from)  // z <= m, or NaN
     {
-        const float d = m == -INFINITY ? z : z - m, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
+        const float d = z - from, e = __builtin_amdgcn_exp2f(d * LP_LOG2E);
         s += e;
         w = fmaf(e, fmaxf(d, -3.0e38f), w);
     }
@@ -139,7 +156,7 @@ __global__ __launch_bounds__(256) void k_logprob_small(const lp_args a)
     for (int x = L / 2; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x, 64));
     t.raise(mx);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t.add(v[i]);
+    for (int i = 0; i < 8; ++i) t.add(v[i], t.from());
 #pragma unroll
     for (int x = L / 2; x; x >>= 1) {             // one maximum for all lanes: the sums just add up
         t.s += __shfl_xor(t.s, x, 64);
@@ -181,12 +198,14 @@ __device__ __forceinline__ void lp_best(const lp_args &a, int64_t row, const lp_
     }
 }
 
+// 8192 x 20011 bf16: 85 us, 3.9 TB/s (maximum, three sums and the comparisons, about ten operations a score, bound it); 4096 x 32000
+// fp32: 98 us, 5.3 TB/s, the rate of a copy.  Sixteen scores a lane and turn: with 32 of them fewer waves fit (100 us).
 // WPR waves walk one row's split (4: a workgroup, 1: each wave a row of its own).  Scores come 16 bytes at a time from the first
 // aligned one on; the few before and behind are single loads.
 template <typename T, int WPR>
-__global__ __launch_bounds__(256) void k_logprob_walk(const lp_args a)
+__global__ __launch_bounds__(256, (sizeof(T) == 2 ? 8 : 6)) void k_logprob_walk(const lp_args a)
 {
-    constexpr int V = 16 / (int)sizeof(T), UN = 4;
+    constexpr int V = 16 / (int)sizeof(T), UN = 16 / V;
     typedef T vec __attribute__((ext_vector_type(V)));
     __shared__ float sums[4][3];
     __shared__ u64 lists[4][64];
@@ -208,11 +227,20 @@ __global__ __launch_bounds__(256) void k_logprob_walk(const lp_args a)
         const int64_t j = from + lane;
         const float v = j < to ? (float)z[j] : -INFINITY;
         t.raise(v);
-        if (j < to) t.add(v);
+        if (j < to) t.add(v, t.from());
         if (keep) best.offer(j < to ? lp_key(v, (u32)j) : LP_NONE, keep, lane);
     };
     if (wave == 0 || WPR == 1) single(c0, b0);
     const vec *zp = (const vec *)(z + b0);
+    vec next[UN];                                 // the following turn's pieces are on their way while this one's are summed
+    auto fetch = [&](int64_t p0) {
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int64_t p = p0 + u * (64 * WPR) + tid;
+            if (p < pieces) next[u] = zp[p];
+        }
+    };
+    fetch(0);
     for (int64_t p0 = 0; p0 < pieces; p0 += 64 * WPR * UN) {
         float v[UN][V];
         float mx = -INFINITY;
@@ -220,9 +248,8 @@ __global__ __launch_bounds__(256) void k_logprob_walk(const lp_args a)
         for (int u = 0; u < UN; ++u) {
             const int64_t p = p0 + u * (64 * WPR) + tid;
             if (p < pieces) {
-                const vec x = zp[p];
 #pragma unroll
-                for (int e = 0; e < V; ++e) v[u][e] = (float)x[e];
+                for (int e = 0; e < V; ++e) v[u][e] = (float)next[u][e];
             } else {
 #pragma unroll
                 for (int e = 0; e < V; ++e) v[u][e] = -INFINITY;
@@ -230,18 +257,30 @@ __global__ __launch_bounds__(256) void k_logprob_walk(const lp_args a)
 #pragma unroll
             for (int e = 0; e < V; ++e) mx = fmaxf(mx, v[u][e]);
         }
+        fetch(p0 + 64 * WPR * UN);
         t.raise(mx);
+        const float from = t.from();
 #pragma unroll
         for (int u = 0; u < UN; ++u)
 #pragma unroll
-            for (int e = 0; e < V; ++e) t.add(v[u][e]);
-        if (keep && __any(best.thr == LP_NONE || !(mx <= lp_value(best.thr)))) {
-#pragma unroll
-            for (int u = 0; u < UN; ++u) {
-                const int64_t p = p0 + u * (64 * WPR) + tid;
-#pragma unroll
-                for (int e = 0; e < V; ++e) best.offer(p < pieces ? lp_key(v[u][e], (u32)(b0 + p * V + e)) : LP_NONE, keep, lane);
+            for (int e = 0; e < V; ++e) t.add(v[u][e], from);
+        if (!keep) continue;
+        // A score enters the list only from `least` on: the keep-th best so far, or, before there is a list, the keep-th largest of
+        // the lanes' maxima -- which leaves little more than the best themselves to be sorted in, not the first ones met.
+        float least = lp_value(best.thr);
+        if (best.thr == LP_NONE) {
+            float x = mx;
+            for (int i = 0; i < keep; ++i) {
+                least = lp_wave_max(x);
+                if (lane == __ffsll((unsigned long long)__ballot(x == least)) - 1) x = -INFINITY;
             }
+        } else if (!__any(mx > least)) continue;  // later classes rank behind equal ones
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int64_t p = p0 + u * (64 * WPR) + tid;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                if (__any(!(v[u][e] < least))) best.offer(p < pieces ? lp_key(v[u][e], (u32)(b0 + p * V + e)) : LP_NONE, keep, lane);
         }
     }
     if (wave == 0 || WPR == 1) single(b1, c1);    // in the order of the classes: an equal score that comes later never ranks before
@@ -293,30 +332,59 @@ __global__ __launch_bounds__(64) void k_logprob_join(const lp_args a)
 }
 
 // ------------------------------------------------------------------ backward: one read, one write
-template <typename T, int VEC>
+// VEC values of the dense gradient, in one list over all rows so that odd numbers of classes stay aligned; a thread that crosses
+// the end of a row takes up the next one's numbers.  UN pieces of a thread, 256 apart: four where there is enough for all CUs (8192 x
+// 20011 bf16: 143 us, 4.6 TB/s, the rate of a copy; 164 with one), one for small calls (32000 x 81 fp32: 9 us; 12 with four).
+template <typename T, int VEC, bool DENSE, int UN>
 __global__ __launch_bounds__(256) void k_logprob_bwd(const T *__restrict__ z, const int64_t *__restrict__ y, int64_t n, int64_t c, int64_t stride,
                                                      const float *__restrict__ norm, const float *__restrict__ entropy, const float *__restrict__ g,
-                                                     const float *__restrict__ gh, T *__restrict__ dz, int64_t blocks)
+                                                     const float *__restrict__ gh, T *__restrict__ dz)
 {
     typedef T vec __attribute__((ext_vector_type(VEC)));
-    const int64_t row = blockIdx.x / blocks, j0 = ((blockIdx.x - row * blocks) * 256 + threadIdx.x) * VEC;
-    if (j0 >= c) return;
-    const lp_norm nm(norm[2 * row], norm[2 * row + 1]);
-    const float h = gh ? entropy[row] : 0.f, gH = gh ? gh[row] : 0.f;
-    const int64_t lab = y ? y[row] : -1;
-    float gl = g && lab >= 0 ? g[row] : 0.f;
-    if (lab >= c) gl = __builtin_nanf("");
-    const vec x = *(const vec *)(z + row * stride + j0);
-    vec o;
+    const int64_t end = n * c, first = ((int64_t)blockIdx.x * (256 * UN) + threadIdx.x) * VEC;
+    vec x[UN];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        const float lp = nm.of((float)x[e]), p = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
-        float v = p == 0.f ? 0.f : -p * fmaf(gH, lp + h, gl);
-        if (lab >= c) v = gl;
-        if (j0 + e == lab && nm.m != -INFINITY) v += gl;
-        o[e] = (T)v;
+    for (int u = 0; u < UN; ++u) {
+        const int64_t i0 = first + u * (256 * VEC);
+        if (DENSE && i0 + VEC <= end) x[u] = *(const vec *)(z + i0);
     }
-    *(vec *)(dz + row * c + j0) = o;
+    int64_t row = -1, lab = -1;
+    lp_norm nm(0.f, 0.f);
+    float h = 0.f, gH = 0.f, gl = 0.f;
+    auto take = [&](int64_t r) {
+        row = r;
+        nm = lp_norm(norm[2 * row], norm[2 * row + 1]);
+        h = gh ? entropy[row] : 0.f;
+        gH = gh ? gh[row] : 0.f;
+        lab = y ? y[row] : -1;
+        gl = g && lab >= 0 ? g[row] : 0.f;
+        if (lab >= c) gl = __builtin_nanf("");
+    };
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+        const int64_t i0 = first + u * (256 * VEC);
+        if (i0 >= end) return;
+        const int64_t r = end < (1ll << 32) ? (int64_t)((u32)i0 / (u32)c) : i0 / c;
+        if (r != row) take(r);
+        int64_t j = i0 - row * c;
+        const bool whole = i0 + VEC <= end;
+        vec o;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            if (i0 + e >= end) break;
+            const float lp = nm.of(DENSE && whole ? (float)x[u][e] : (float)z[row * stride + j]), p = __builtin_amdgcn_exp2f(lp * LP_LOG2E);
+            float v = p == 0.f ? 0.f : -p * fmaf(gH, lp + h, gl);
+            if (lab >= c) v = gl;
+            if (j == lab && nm.m != -INFINITY) v += gl;
+            o[e] = (T)v;
+            if (!whole) dz[i0 + e] = o[e];
+            if (++j == c && e + 1 < VEC && row + 1 < n) {
+                j = 0;
+                take(row + 1);
+            }
+        }
+        if (whole) *(vec *)(dz + i0) = o;
+    }
 }
 
 // ------------------------------------------------------------------ host
@@ -358,7 +426,8 @@ template <typename T> static void lp_forward(lp_args &a, hipStream_t st)
         else LP_SMALL(64);
         return;
     }
-    if (a.splits == 1 && a.c <= 4096) hipLaunchKernelGGL((k_logprob_walk<T, 1>), dim3((unsigned)dg_cdiv(a.n, 4)), dim3(256), 0, st, a);
+    // a wave a row where rows alone give every SIMD four waves, or where a row is short; four waves a row elsewhere
+    if (a.splits == 1 && (a.c <= 4096 || a.n >= 4096)) hipLaunchKernelGGL((k_logprob_walk<T, 1>), dim3((unsigned)dg_cdiv(a.n, 4)), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_logprob_walk<T, 4>), dim3((unsigned)(a.n * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((k_logprob_join<T>), dim3((unsigned)a.n), dim3(64), 0, st, a);
 }
@@ -395,11 +464,16 @@ static int lp_backward(const void *z, const int64_t *y, int64_t n, int64_t c, in
                        void *dz, hipStream_t st)
 {
     constexpr int V = 16 / (int)sizeof(T);
-    const bool wide = c % V == 0 && stride % V == 0 && ((((uintptr_t)z) | ((uintptr_t)dz)) & 15) == 0;
-    const int64_t blocks = dg_cdiv(c, 256 * (wide ? V : 1));
-    DG_REQUIRE(n * blocks < (1ll << 31), "class_logprobs_bwd: too large");
-    if (wide) hipLaunchKernelGGL((k_logprob_bwd<T, V>), dim3((unsigned)(n * blocks)), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz, blocks);
-    else hipLaunchKernelGGL((k_logprob_bwd<T, 1>), dim3((unsigned)(n * blocks)), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz, blocks);
+    const bool wide = (((uintptr_t)dz) & 15) == 0, dense = stride == c && (((uintptr_t)z) & 15) == 0;
+    const bool many = wide && n * c >= (1ll << 24);
+    const int64_t blocks = dg_cdiv(n * c, 256 * (many ? 4 * V : wide ? V : 1));
+    DG_REQUIRE(blocks < (1ll << 31), "class_logprobs_bwd: too large");
+#define LP_BWD(VEC, DENSE, UN) hipLaunchKernelGGL((k_logprob_bwd<T, VEC, DENSE, UN>), dim3((unsigned)blocks), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz)
+    if (many && dense) LP_BWD(V, true, 4);
+    else if (many) LP_BWD(V, false, 4);
+    else if (wide && dense) LP_BWD(V, true, 1);
+    else if (wide) LP_BWD(V, false, 1);
+    else LP_BWD(1, false, 1);
     DG_CHECK_LAUNCH("k_logprob_bwd");
     return DG_OK;
 }

@@ -1,6 +1,7 @@
 """Tensor-level front end of the HIP kernels: GPU tensors in, GPU tensors out, async on the
 current stream.  The reference-named drop-ins (yolo_v1.py, yolo_v2.py, rcnn_utils.py,
 fast_rcnn.py, cluster.py) are thin layers over these."""
+import functools
 import math
 
 import torch
@@ -353,17 +354,27 @@ def kmeans_labels_i32(labels_u8):
 def _scratch(nbytes, dev):
     """Scratch of one call, from the caching allocator in the current stream's order: captured graphs and calls on other
     streams never share it."""
-    return torch.empty(int(nbytes), dtype=torch.uint8, device=dev) if nbytes else None
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(dev):
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+@functools.lru_cache(maxsize=1024)
+def _strides_fit(shape, strides, e):
+    """whether a kernel that loads 16 bytes at a time can step along a (B,N,H,D) tensor: a dense last axis, everything else a
+    multiple of 16 bytes, rows at most 2^22 values apart"""
+    return strides[3] == 1 and all(n == 1 or st * e % 16 == 0 for n, st in zip(shape[:3], strides)) and (shape[1] == 1 or strides[1] <= 1 << 22)
 
 
 def _vec16(t):
-    """(B,N,H,D) with a dense last axis and everything a kernel steps along a multiple of 16 bytes (rows at most 2^22 values
-    apart); copied if it is not."""
-    e = t.element_size()
-    if t.numel() == 0:
-        return t
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or st * e % 16 == 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])) \
-            and (t.shape[1] == 1 or t.stride(1) <= 1 << 22):
+    """t, or a copy of it, such that _strides_fit and its first value lies on a multiple of 16 bytes"""
+    if t.numel() == 0 or (t.data_ptr() % 16 == 0 and _strides_fit(t.shape, t.stride(), t.element_size())):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -377,35 +388,38 @@ def _counts(c, B, dev, what):
     return c
 
 
-def _attn_call(q, k, v, q_counts, k_counts, mask, scale):
+@functools.lru_cache(maxsize=1024)
+def _attn_plan(q_shape, k_shape, q_stride, k_stride, v_stride, g_stride, masks, mask_stride, scale, dtype, backward):
+    """the call's description for the library and its workspace's size: by shapes alone"""
+    B, Nq, Hq, D = q_shape
+    s = _abi.AttnShape(B, Nq, k_shape[1], Hq, k_shape[2], D, *q_stride[:3], *k_stride[:3], *v_stride[:3], *g_stride[:3], masks, *mask_stride[:2],
+                       D ** -0.5 if scale is None else scale, _abi.TYPES[dtype])
+    return s, load().dg_roi_attn_workspace_bytes(s, backward)
+
+
+def _attn_args(q, k, v, q_counts, k_counts, mask):
     """checks and lays out what the forward and the backward pass have in common"""
     dev = _abi.device_of(q, k, v)
-    q, k, v = (t.to(dev) for t in (q, k, v))
+    if not (q.device == dev and k.device == dev and v.device == dev):
+        q, k, v = q.to(dev), k.to(dev), v.to(dev)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError("roi_attention: q (B,Nq,Hq,D), k and v (B,Nk,Hk,D)")
     if q.dtype not in (torch.float32, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("roi_attention: q, k and v must all be float32 or all be bfloat16")
-    q, k, v = _vec16(q), _vec16(k), _vec16(v)
-    B, Nq, Hq, D = q.shape
-    Nk, Hk = k.shape[1], k.shape[2]
+    B, Nq, Nk = q.shape[0], q.shape[1], k.shape[1]
     qc, kc = _counts(q_counts, B, dev, "q_counts"), _counts(k_counts, B, dev, "k_counts")
-    s = _abi.AttnShape(B, Nq, Nk, Hq, Hk, D)
-    s.q_stride[:], s.k_stride[:], s.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    s.scale = D ** -0.5 if scale is None else float(scale)
-    s.dtype = _abi.TYPES[q.dtype]
-    if mask is not None:
-        mask = mask.to(dev) if isinstance(mask, torch.Tensor) else torch.as_tensor(mask, device=dev)
-        if mask.dtype not in (torch.bool, torch.uint8):
-            raise ValueError("roi_attention: mask must be bool (or uint8: not 0 = may be seen)")
-        if mask.dim() == 2:
-            mask = mask[None]
-        if mask.dim() != 3 or mask.shape[0] not in (1, B) or tuple(mask.shape[1:]) != (Nq, Nk):
-            raise ValueError("roi_attention: mask must be (Nq,Nk) or (B or 1,Nq,Nk)")
-        if Nk > 1 and mask.stride(2) != 1:
-            mask = mask.contiguous()
-        s.masks = mask.shape[0]
-        s.mask_stride[:] = mask.stride()[:2]
-    return dev, q, k, v, qc, kc, mask, s
+    if mask is None:
+        return dev, _vec16(q), _vec16(k), _vec16(v), qc, kc, None, 0, (0, 0)
+    mask = mask.to(dev) if isinstance(mask, torch.Tensor) else torch.as_tensor(mask, device=dev)
+    if mask.dtype not in (torch.bool, torch.uint8):
+        raise ValueError("roi_attention: mask must be bool (or uint8: not 0 = may be seen)")
+    if mask.dim() == 2:
+        mask = mask[None]
+    if mask.dim() != 3 or mask.shape[0] not in (1, B) or tuple(mask.shape[1:]) != (Nq, Nk):
+        raise ValueError("roi_attention: mask must be (Nq,Nk) or (B or 1,Nq,Nk)")
+    if Nk > 1 and mask.stride(2) != 1:
+        mask = mask.contiguous()
+    return dev, _vec16(q), _vec16(k), _vec16(v), qc, kc, mask, mask.shape[0], mask.stride()
 
 
 def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
@@ -414,37 +428,35 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
     lse (B,Hq,Nq) float32.  A row sees the keys before k_counts (B) of its image for which mask (B or 1,Nq,Nk) is not 0; scale
     defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  No reference
     counterpart.  For a gradient: fast_rcnn.roi_attention."""
-    dev, q, k, v, qc, kc, mask, s = _attn_call(q, k, v, q_counts, k_counts, mask, scale)
+    dev, q, k, v, qc, kc, mask, masks, ms = _attn_args(q, k, v, q_counts, k_counts, mask)
+    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, scale, q.dtype, 0)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
-    lib = load()
-    nbytes = lib.dg_roi_attn_workspace_bytes(s, 0)
     ws = _scratch(nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib.dg_roi_attn_fwd(s, ptr(q), ptr(k), ptr(v), ptr(qc), ptr(kc), ptr(mask), ptr(out), ptr(lse), ptr(ws), nbytes, stream_ptr(dev)))
+    with _abi.on_device(dev):
+        check(load().dg_roi_attn_fwd(s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(qc), _at(kc), _at(mask), out.data_ptr(), lse.data_ptr(), _at(ws), nbytes,
+                                     _stream(dev)))
     return out, lse
 
 
 def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=None, mask=None, scale=None, need_q=True, need_kv=True):
     """Gradients of roi_attention from its inputs, out and lse, with the probabilities recomputed: dq (B,Nq,Hq,D), dk and dv
     (B,Nk,Hk,D), rows behind a count 0.  need_q / need_kv False leaves those out (None)."""
-    dev, q, k, v, qc, kc, mask, s = _attn_call(q, k, v, q_counts, k_counts, mask, scale)
+    dev, q, k, v, qc, kc, mask, masks, ms = _attn_args(q, k, v, q_counts, k_counts, mask)
     g, out, lse = grad_out.to(dev), out.to(dev).contiguous(), lse.to(dev).contiguous()
     if g.shape != q.shape or out.shape != q.shape or g.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError("roi_attention_backward: grad_out and out must have q's shape and type")
-    if lse.shape != (s.batch, s.q_heads, s.nq) or lse.dtype != torch.float32:
+    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         raise ValueError("roi_attention_backward: lse must be (B,Hq,Nq) float32")
     g, out = _vec16(g), _vec16(out)
-    s.g_stride[:] = g.stride()[:3]
+    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, scale, q.dtype, 1)
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
     dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
     dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
-    lib = load()
-    nbytes = lib.dg_roi_attn_workspace_bytes(s, 1)
     ws = _scratch(nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib.dg_roi_attn_bwd(s, ptr(g), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), ptr(qc), ptr(kc), ptr(mask), ptr(dq), ptr(dk), ptr(dv),
-                                  ptr(ws), nbytes, stream_ptr(dev)))
+    with _abi.on_device(dev):
+        check(load().dg_roi_attn_bwd(s, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _at(qc), _at(kc), _at(mask),
+                                     _at(dq), _at(dk), _at(dv), _at(ws), nbytes, _stream(dev)))
     return dq, dk, dv
 
 
@@ -485,14 +497,21 @@ def _dense_last(t):
     return t if t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
+def _rope_shape(q_shape, k_heads, pairs, axes, q_stride, k_stride, pos_batch, pos_row, dtype, pos64, pairing):
+    B, N, Hq, D = q_shape
+    return _abi.RopeShape(B, N, Hq, k_heads, D, pairs, axes, *q_stride[:3], *k_stride[:3], pos_batch, pos_row, _abi.TYPES[dtype],
+                          _abi.F64 if pos64 else _abi.F32, _abi.ROPE_HALVES if pairing == "halves" else _abi.ROPE_NEIGHBOURS)
+
+
 def rope_axes(q, pos, plan, k=None, inverse=False):
     """Turns the pairs of q (B,N,H,D) (and of k (B,N,Hk,D) in the same launch) by the positions pos (B,N,A) or (N,A) of their
     tokens as plan says; inverse: back, which is the gradient.  float32, bfloat16 or float16; values behind the plan's pairs are
     copied; float32 or float64 positions are used as they are, whole numbers as float64.  -> the turned q, or (q, k).  No
     reference counterpart.  For a gradient: fast_rcnn.rope_axes."""
     dev = _abi.device_of(q, k, pos)
-    q = _dense_last(q.to(dev))
-    k = None if k is None else _dense_last(k.to(dev))
+    q = _dense_last(q if q.device == dev else q.to(dev))
+    k = None if k is None else _dense_last(k if k.device == dev else k.to(dev))
     pos = pos.to(dev) if isinstance(pos, torch.Tensor) else torch.as_tensor(pos, device=dev)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
         raise ValueError("rope_axes: q (B,N,Hq,D), k (B,N,Hk,D) of one type")
@@ -509,18 +528,13 @@ def rope_axes(q, pos, plan, k=None, inverse=False):
     if pos.dim() not in (2, 3) or tuple(pos.shape[-2:]) != (N, plan.axes) or (pos.dim() == 3 and pos.shape[0] not in (1, B)):
         raise ValueError(f"rope_axes: pos must be (B,N,{plan.axes}) or (N,{plan.axes})")
     pos = _dense_last(pos)
-    s = _abi.RopeShape(B, N, Hq, 0 if k is None else k.shape[2], D, plan.pairs, plan.axes)
-    s.q_stride[:] = q.stride()[:3]
-    if k is not None:
-        s.k_stride[:] = k.stride()[:3]
-    s.pos_stride[:] = (pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2))
-    s.dtype, s.pos_dtype = _abi.TYPES[q.dtype], _abi.F64 if pos.dtype == torch.float64 else _abi.F32
-    s.pairing = _abi.ROPE_HALVES if plan.pairing == "halves" else _abi.ROPE_NEIGHBOURS
+    s = _rope_shape(q.shape, 0 if k is None else k.shape[2], plan.pairs, plan.axes, q.stride(), (0, 0, 0) if k is None else k.stride(),
+                    pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2), q.dtype, pos.dtype == torch.float64, plan.pairing)
     out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
     out_k = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
-    with torch.cuda.device(dev):
-        check(load().dg_rope_axes(s, ptr(q), ptr(k), ptr(pos), ptr(plan.turns), ptr(plan.axis), int(bool(inverse)), ptr(out_q), ptr(out_k),
-                                  stream_ptr(dev)))
+    with _abi.on_device(dev):
+        check(load().dg_rope_axes(s, q.data_ptr(), _at(k), pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), 1 if inverse else 0, out_q.data_ptr(),
+                                  _at(out_k), _stream(dev)))
     return out_q if k is None else (out_q, out_k)
 
 
@@ -556,9 +570,9 @@ def class_logprobs(logits, labels=None, top=0):
     lib = load()
     nbytes = lib.dg_class_logprobs_workspace_bytes(n, c, top)
     ws = _scratch(nbytes, dev)
-    with torch.cuda.device(dev):
-        check(lib.dg_class_logprobs(ptr(z), _abi.TYPES[z.dtype], ptr(y), n, c, z.stride(0), top, ptr(logp), ptr(entropy), ptr(norm), ptr(best), ptr(index),
-                                    ptr(status), ptr(ws), nbytes, stream_ptr(dev)))
+    with _abi.on_device(dev):
+        check(lib.dg_class_logprobs(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), top, _at(logp), entropy.data_ptr(), norm.data_ptr(),
+                                    best.data_ptr(), index.data_ptr(), _at(status), _at(ws), nbytes, _stream(dev)))
     return logp, entropy, norm, best, index
 
 
@@ -575,6 +589,6 @@ def class_logprobs_backward(grad_logp, grad_entropy, logits, labels, norm, entro
     if y is None:
         args[2] = None
     dz = torch.empty((n, c), dtype=z.dtype, device=dev)
-    with torch.cuda.device(dev):
-        check(load().dg_class_logprobs_bwd(ptr(z), _abi.TYPES[z.dtype], ptr(y), n, c, z.stride(0), *(ptr(t) for t in args), ptr(dz), stream_ptr(dev)))
+    with _abi.on_device(dev):
+        check(load().dg_class_logprobs_bwd(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), *(_at(t) for t in args), dz.data_ptr(), _stream(dev)))
     return dz
