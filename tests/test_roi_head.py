@@ -312,3 +312,410 @@ def test_class_logprobs(n, c, top, dtype):
            _logp64(z, y, 0, g, torch.zeros_like(gh))["dz"], "dz of logp alone")
     none = ops.class_logprobs(Z, None, top)
     assert none[0] is None and torch.equal(none[4], index) and torch.equal(none[1].nan_to_num(7.0), entropy.nan_to_num(7.0))
+
+
+# ------------------------------------------------------------------ layouts, offsets, streams, graphs
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_roi_attention_layouts(dtype):
+    """Heads first, one fused buffer of q, k and v, odd offsets (copied), expanded batches: the bits of the dense call."""
+    from vision_amd import ops
+    B, N, H, D = 2, 77, 4, 64
+    q, k, v, do = (t.cuda() for t in _attn_inputs(11, B, N, N, H, H, D, dtype))
+    out, lse = ops.roi_attention(q, k, v)
+    grads = ops.roi_attention_backward(do, q, k, v, out, lse)
+    views = []
+    views.append([t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v, do)])
+    fused = torch.stack([q, k, v, do], 2)
+    views.append([fused[:, :, i] for i in range(4)])
+    odd = [torch.empty(t.numel() + 1, dtype=dtype, device="cuda")[1:].view(t.shape).copy_(t) for t in (q, k, v, do)]
+    views.append(odd)
+    wide = [torch.zeros((B, N, H, D + 3), dtype=dtype, device="cuda") for _ in range(4)]
+    for w, t in zip(wide, (q, k, v, do)):
+        w[..., :D] = t
+    views.append([w[..., :D] for w in wide])
+    for a, b, c, g in views:
+        o, s = ops.roi_attention(a, b, c)
+        assert torch.equal(o, out) and torch.equal(s, lse)
+        assert all(torch.equal(x, y) for x, y in zip(ops.roi_attention_backward(g, a, b, c, out, lse), grads))
+    o, _ = ops.roi_attention(q, k[:1].expand(B, N, H, D), v[:1].expand(B, N, H, D))
+    o2, _ = ops.roi_attention(q, k[:1].repeat(B, 1, 1, 1), v[:1].repeat(B, 1, 1, 1))
+    assert torch.equal(o, o2)
+    one = do[:, :, :, :1].expand(B, N, H, D)                              # what sum().backward() hands over
+    assert all(torch.equal(x, y) for x, y in zip(ops.roi_attention_backward(one, q, k, v, out, lse),
+                                                 ops.roi_attention_backward(one.contiguous(), q, k, v, out, lse)))
+
+
+@pytest.mark.gpu
+def test_roi_attention_far_rows():
+    """Keys and values whose rows lie so far apart that offsets pass 2^32 bytes and 2^31 values; one more stride and the call
+    goes by a copy."""
+    from vision_amd import ops
+    q, k, v, do = (t.cuda() for t in _attn_inputs(12, 1, 5, 520, 1, 1, 64, torch.bfloat16))
+    out, lse = ops.roi_attention(q, k, v)
+    want = ops.roi_attention_backward(do, q, k, v, out, lse)
+    for step in (1 << 22, (1 << 22) + 8):
+        big = torch.empty((2, 520, step), dtype=torch.bfloat16, device="cuda")
+        K, V = big[0, None, :, None, :64], big[1, None, :, None, :64]
+        K.copy_(k)
+        V.copy_(v)
+        o, s = ops.roi_attention(q, K, V)
+        assert torch.equal(o, out) and torch.equal(s, lse)
+        assert all(torch.equal(x, y) for x, y in zip(ops.roi_attention_backward(do, q, K, V, out, lse), want))
+        del big, K, V
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_roi_attention_nan_behind_mask(dtype):
+    """What a mask hides from a row does not reach it, whatever it holds; what a row does see and is not finite makes it NaN."""
+    from vision_amd import ops
+    B, N, M, H, D = 1, 70, 90, 2, 64
+    q, k, v, do = _attn_inputs(13, B, N, M, H, H, D, dtype)
+    g = _gen(14)
+    mask = torch.rand((B, N, M), generator=g) < 0.5
+    bad_keys, bad_rows = [3, 40, 88], [7, 33]
+    mask[:, :35, bad_keys] = False               # the first half sees none of them
+    mask[:, 35:, bad_keys[0]] = True
+    clean = mask.clone()
+    clean[:, 35:] = False                        # the rows that stay finite, for the reference
+    clean[:, bad_rows] = False
+    K, V, Q, G = k.clone(), v.clone(), q.clone(), do.clone()
+    K[:, 3, 0, 5], V[:, 3, 1, 6] = math.nan, math.inf
+    K[:, 40] = math.inf
+    V[:, 88] = math.nan
+    Q[:, 7] = math.nan
+    G[:, 33, :, 2] = math.inf
+    want = _attn64(q, k, v, None, None, mask, None, do)
+    Qc, Kc, Vc, Gc, Mc = map(_dev, (Q, K, V, G, mask))
+    out, lse = ops.roi_attention(Qc, Kc, Vc, mask=Mc)
+    rows = [i for i in range(35) if i != 7]
+    _close(out[:, rows], tuple(t[:, rows] for t in want["out"]), "rows that see no bad key")
+    assert torch.isnan(out[:, 7]).all() and torch.isnan(out[:, 35:]).all()
+    dq, dk, dv = ops.roi_attention_backward(Gc, Qc, Kc, Vc, out, lse, mask=Mc)
+    rows = [i for i in rows if i != 33]
+    _close(dq[:, rows], tuple(t[:, rows] for t in want["dq"]), "dq of those rows")
+    # keys that only good rows see
+    seen_bad = mask[0, 35:].any(0) | mask[0, bad_rows].any(0)
+    good = [j for j in range(M) if not bool(seen_bad[j])]
+    mask[:, :, :5] = mask[:, :, :5]
+    only = torch.zeros_like(mask)
+    only[:, rows] = mask[:, rows]
+    ref = _attn64(q, k, v, None, None, only, None, do)
+    if good:
+        _close(dk[:, good], tuple(t[:, good] for t in ref["dk"]), "dk")
+        _close(dv[:, good], tuple(t[:, good] for t in ref["dv"]), "dv")
+    # the same with every later row masked off for every key: all good rows' gradients, none of the bad ones'
+    Mc[:, 35:] = False
+    Mc[:, bad_rows] = False
+    out, lse = ops.roi_attention(Qc, Kc, Vc, mask=Mc)
+    dq, dk, dv = ops.roi_attention_backward(Gc, Qc, Kc, Vc, out, lse, mask=Mc)
+    keys = [j for j in range(M) if j not in bad_keys]
+    _close(dk[:, keys], tuple(t[:, keys] for t in ref["dk"]), "dk, bad rows off")
+    _close(dv, ref["dv"], "dv, bad rows off")
+    assert float(dk[:, bad_keys].abs().max()) == 0.0 and float(dq[:, bad_rows].abs().max()) == 0.0 and float(out[:, bad_rows].abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_roi_attention_scale_and_large_scores():
+    """Scores far apart and far from zero: the running maximum follows, nothing overflows; a scale of one's own."""
+    from vision_amd import ops
+    q, k, v, do = _attn_inputs(15, 1, 40, 300, 1, 1, 32, torch.float32)
+    k = k * torch.linspace(0.1, 30.0, 300)[None, :, None, None]          # the largest scores come last
+    for scale in (None, 1.0, 1e-3):
+        want = _attn64(q, k, v, None, None, None, scale, do)
+        out, lse = ops.roi_attention(q.cuda(), k.cuda(), v.cuda(), scale=scale)
+        _close(out, want["out"], "out")
+        _close(lse, want["lse"], "lse")
+        for n, g in zip(("dq", "dk", "dv"), ops.roi_attention_backward(do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, scale=scale)):
+            _close(g, want[n], n)
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """Every operator on a stream of its own, and captured into two graphs that are replayed in turn with eager work between."""
+    from vision_amd import ops
+    g = _gen(16)
+    B, N, H, D, C = 2, 150, 4, 64, 1000
+    plan = ops.rope_plan((16, 16))
+    ins = [[torch.randn((B, N, H, D), generator=g).bfloat16().cuda() for _ in range(4)] + [torch.rand((B, N, 2), generator=g).cuda() * 40,
+           torch.tensor([N, N - 40 - i]).int().cuda(), torch.randn((B * N, C), generator=g).cuda(), torch.randint(0, C, (B * N,), generator=g).cuda(),
+           torch.rand((B, N, N), generator=g).cuda() < 0.5] for i in range(2)]
+
+    def work(q, k, v, do, pos, counts, z, y, mask):
+        a, b = ops.rope_axes(q, pos, plan, k=k)
+        out, lse = ops.roi_attention(a, b, v, counts, counts, mask)
+        grads = ops.roi_attention_backward(do, a, b, v, out, lse, counts, counts, mask)
+        logp, h, norm, best, index = ops.class_logprobs(z, y, 5)
+        dz = ops.class_logprobs_backward(logp, h, z, y, norm, h)
+        return [a, b, out, lse, *grads, logp, h, best, index, dz]
+
+    eager = [[t.clone() for t in work(*i)] for i in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        on_side = work(*ins[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(on_side, eager[0]))
+    graphs, outs = [], []
+    for i in ins:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(work(*i))
+        graphs.append(gr)
+    for r in range(3):
+        for i in (0, 1):
+            for t in outs[i]:
+                t.zero_()
+            graphs[i].replay()
+            work(*ins[1 - i])                    # eager work between
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(outs[i], eager[i])), (r, i)
+    graphs[0].replay()                           # both at once, on two streams
+    with torch.cuda.stream(side):
+        graphs[1].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for i in (0, 1) for x, y in zip(outs[i], eager[i]))
+
+
+# ------------------------------------------------------------------ gradients through autograd
+def _slope(f, xs, ds, h=1e-6):
+    """central difference of a 64-bit function along ds"""
+    up, down = f(*[x + h * d for x, d in zip(xs, ds)]), f(*[x - h * d for x, d in zip(xs, ds)])
+    return float((up - down) / (2 * h))
+
+
+@pytest.mark.gpu
+def test_roi_attention_gradient_against_differences():
+    """The gradient's product with a direction against the difference quotient of the 64-bit definition.  The quotient's own error
+    is h^2 / 6 times a third derivative plus 2^-52 |f| / h: below 1e-6 of the sum of magnitudes here; the rest is the bound of
+    each gradient's elements."""
+    from vision_amd import fast_rcnn
+    B, N, M, H, Hk, D = 2, 20, 30, 4, 2, 16
+    q, k, v, do = _attn_inputs(21, B, N, M, H, Hk, D, torch.float32)
+    mask = torch.rand((B, N, M), generator=_gen(22)) < 0.6
+    qc, kc = torch.tensor([20, 11]), torch.tensor([30, 25])
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    out = fast_rcnn.roi_attention(*leaves, q_counts=qc, k_counts=kc, mask=mask)
+    assert out.is_cuda and out.requires_grad
+    grads = torch.autograd.grad(out, leaves, do.cuda())
+    want = _attn64(q, k, v, qc, kc, mask, None, do)
+    f = lambda a, b, c: (_attn64(a, b, c, qc, kc, mask, None)["out"][0] * do.double()).sum()    # noqa: E731
+    g = _gen(23)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        _close(grads[i], want[name], name)
+        d = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+        d[i] = torch.randn(d[i].shape, generator=g, dtype=torch.float64)
+        slope, mine = _slope(f, (q.double(), k.double(), v.double()), d), float((grads[i].cpu().double() * d[i]).sum())
+        size = float((want[name][0].abs() * d[i].abs()).sum())
+        assert abs(slope - mine) <= float((want[name][1] * d[i].abs()).sum()) + 1e-6 * size, name
+    cpu = [t.clone().requires_grad_(True) for t in (q, k, v)]              # tensors on the CPU go in and come back
+    o = fast_rcnn.roi_attention(*cpu, q_counts=qc, k_counts=kc, mask=mask)
+    assert not o.is_cuda and torch.equal(o, out.detach().cpu())
+    (o * do).sum().backward()
+    assert all(torch.equal(t.grad, x.cpu()) for t, x in zip(cpu, grads))
+    only_v = v.cuda().requires_grad_(True)
+    (dv,) = torch.autograd.grad(fast_rcnn.roi_attention(q.cuda(), k.cuda(), only_v, qc, kc, mask), (only_v,), do.cuda())
+    assert torch.equal(dv, grads[2])
+
+
+@pytest.mark.gpu
+def test_rope_and_logprobs_gradient():
+    from vision_amd import fast_rcnn, ops
+    g = _gen(31)
+    q, k = torch.randn((2, 9, 3, 32), generator=g).cuda().requires_grad_(True), torch.randn((2, 9, 1, 32), generator=g).cuda().requires_grad_(True)
+    pos = torch.rand((2, 9, 3), generator=g).cuda() * 50
+    plan = ops.rope_plan((4, 6, 6))
+    a, b = fast_rcnn.rope_axes(q, k, pos, plan)
+    da, db = torch.randn(a.shape, generator=g).cuda().requires_grad_(True), torch.randn(b.shape, generator=g).cuda()
+    dq, dk = torch.autograd.grad((a, b), (q, k), (da, db), create_graph=True)
+    assert torch.equal(dq.detach(), ops.rope_axes(da.detach(), pos, plan, inverse=True)) and torch.equal(dk.detach(), ops.rope_axes(db, pos, plan, inverse=True))
+    (twice,) = torch.autograd.grad(dq, (da,), q.detach())                  # linear: its second derivative is the turn itself
+    assert torch.equal(twice, a.detach())
+    (only,) = torch.autograd.grad(fast_rcnn.rope_axes(q, k, pos, plan)[1], (k,), db)
+    assert torch.equal(only, dk.detach())
+    z = torch.randn((12, 37), generator=g)
+    y = torch.randint(0, 37, (12,), generator=g)
+    y[3] = -1
+    w, wh = torch.randn(12, generator=g), torch.randn(12, generator=g)
+    Z = z.cuda().requires_grad_(True)
+    r = fast_rcnn.class_logprobs(Z, y, top=4)
+    assert not r.top_logp.requires_grad and r.top_index.dtype == torch.int64
+    (dz,) = torch.autograd.grad((r.logp, r.entropy), (Z,), (w.cuda(), wh.cuda()), retain_graph=True)
+    want = _logp64(z, y, 4, w, wh)
+    _close(dz, want["dz"], "dz")
+    f = lambda x: (_logp64(x, y, 0)["logp"][0] * w.double()).sum() + (_logp64(x, y, 0)["entropy"][0] * wh.double()).sum()    # noqa: E731
+    d = torch.randn(z.shape, generator=g, dtype=torch.float64)
+    # the quotient's own error: below 1e-6 of the sum of magnitudes, as above
+    assert abs(_slope(f, (z.double(),), (d,)) - float((dz.cpu().double() * d).sum())) <= float((want["dz"][1] * d.abs()).sum()) + 1e-6 * float((want["dz"][0] * d).abs().sum())
+    (one,) = torch.autograd.grad(r.entropy, (Z,), wh.cuda())
+    _close(one, _logp64(z, y, 0, torch.zeros(12), wh)["dz"], "dz of the entropy alone")
+
+
+@pytest.mark.gpu
+def test_head_together():
+    """Boxes of two frames turned by their positions, related to each other where they overlap, classified, and a training loss
+    back through all of it: the chain's gradients are the operators' own, one after the other, and its loss and its gradient agree
+    with the definitions in 64 bits.  Every stage is exact to 2^-15 of the magnitudes that it sums (checked above: at most 64 values
+    a product, 60 keys, 30 classes); through three stages forward and back, each norm-preserving up to a factor of 4 (logits by a
+    projection of norm below 4), the loss's slope along a direction stays within 2^-15 x 6 x 4^3 < 2^-6 of its magnitudes."""
+    from tools import workloads as wl
+    from vision_amd import fast_rcnn, ops
+    B, N, H, D, C = 2, 60, 4, 64, 30
+    boxes = torch.stack([torch.from_numpy(wl.random_boxes(50 + i, N)) for i in range(B)])
+    pos = torch.stack([torch.tensor([5.0, 6.0])[:, None].expand(B, N), (boxes[..., 1] + boxes[..., 3]) * 10, (boxes[..., 0] + boxes[..., 2]) * 10], 2)
+    counts = torch.tensor([N, 41]).int()
+    over = torch.stack([ops.iou_pairwise(b.cuda(), b.cuda()) > 0.05 for b in boxes])
+    g = _gen(41)
+    q, k, v = (torch.randn((B, N, H, D), generator=g) for _ in range(3))
+    proj = torch.randn((H * D, C), generator=g) / math.sqrt(H * D)
+    y = torch.randint(0, C, (B, N), generator=g)
+    y[1, 41:] = -1                               # padded rows carry no label
+    plan = ops.rope_plan((8, 12, 12))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    a, b = fast_rcnn.rope_axes(leaves[0], leaves[1], pos, plan)
+    out = fast_rcnn.roi_attention(a, b, leaves[2], counts, counts, over)
+    z = out.reshape(B * N, H * D) @ proj.cuda()
+    r = fast_rcnn.class_logprobs(z, y.reshape(-1), top=3)
+    loss = -r.logp.sum() / int((y >= 0).sum()) - 0.01 * r.entropy.sum()
+    grads = torch.autograd.grad(loss, leaves)
+    # the same by hand
+    ones = torch.full((B * N,), -1.0 / int((y >= 0).sum()), device="cuda")
+    logp, h, norm, best, index = ops.class_logprobs(z.detach(), y.reshape(-1), 3)
+    assert torch.equal(logp, r.logp.detach()) and torch.equal(index, r.top_index)
+    dz = ops.class_logprobs_backward(ones, torch.full_like(ones, -0.01), z.detach(), y.reshape(-1), norm, h)
+    dout = (dz @ proj.cuda().T).view(B, N, H, D)
+    o, lse = ops.roi_attention(a.detach(), b.detach(), leaves[2].detach(), counts, counts, over)
+    da, db, dv = ops.roi_attention_backward(dout, a.detach(), b.detach(), leaves[2].detach(), o, lse, counts, counts, over)
+    dq, dk = ops.rope_axes(da, pos.cuda(), plan, k=db, inverse=True)
+    assert all(torch.equal(x, w) for x, w in zip(grads, (dq, dk, dv)))
+    # and in 64 bits
+    mask = over.cpu()
+
+    def f(Q, K, V):
+        ang = pos.double()[..., plan.axis.cpu().long()] * plan.turns.cpu() * 2 * math.pi
+        c, s = torch.cos(ang)[:, :, None], torch.sin(ang)[:, :, None]
+        turn = lambda t: torch.cat([t[..., :32] * c - t[..., 32:] * s, t[..., :32] * s + t[..., 32:] * c], -1)   # noqa: E731
+        w = _attn64(turn(Q), turn(K), V, counts, counts, mask, None)["out"][0].reshape(B * N, H * D) @ proj.double()
+        lp = _logp64(w, y.reshape(-1), 0)
+        return -lp["logp"][0].sum() / int((y >= 0).sum()) - 0.01 * lp["entropy"][0].sum()
+    xs = [t.double() for t in (q, k, v)]
+    exact = float(f(*xs))
+    assert abs(float(loss.detach()) - exact) <= 2.0 ** -6 * abs(exact)
+    for i in range(3):
+        d = [torch.zeros_like(t) for t in xs]
+        d[i] = torch.randn(xs[i].shape, generator=g, dtype=torch.float64)
+        mine = grads[i].cpu().double() * d[i]
+        assert abs(_slope(f, xs, d) - float(mine.sum())) <= 2.0 ** -6 * float(mine.abs().sum()), i
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals_of_the_library():
+    """On the host, before any launch."""
+    import ctypes as C
+    from vision_amd import _abi
+    lib = _abi.load()
+
+    def shape(**kw):
+        s = _abi.AttnShape(2, 8, 8, 4, 2, 64)
+        for t, heads in (("q", 4), ("k", 2), ("v", 2), ("g", 4)):
+            for a, n in (("batch", 8 * heads * 64), ("row", heads * 64), ("head", 64)):
+                setattr(s, f"{t}_stride_{a}", n)
+        s.scale, s.dtype = 0.125, _abi.BF16
+        for a, b in kw.items():
+            setattr(s, a, b)
+        return s
+    p = C.c_void_p(4096)                         # never touched: every call below ends before a launch
+
+    def fwd(s, q=p, ws=None, n=0):
+        return lib.dg_roi_attn_fwd(s, q, p, p, None, None, None, p, p, ws, n, None)
+    for kw, word in ((dict(d=12), "head size"), (dict(d=136), "head size"), (dict(q_heads=3), "multiple of k_heads"), (dict(k_heads=0), "multiple of k_heads"),
+                     (dict(dtype=_abi.F16), "type"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                     (dict(batch=-1), "negative"), (dict(nq=1 << 40), "2^28"), (dict(masks=3), "masks"), (dict(masks=1), "null"),
+                     (dict(q_stride_row=33), "16 bytes"), (dict(k_stride_row=-64), "16 bytes"), (dict(v_stride_row=1 << 23), "2^22")):
+        assert fwd(shape(**kw)) == _abi.EINVAL, kw
+        assert word in _abi.last_error(), (kw, _abi.last_error())
+    assert fwd(shape(), q=C.c_void_p(4098)) == _abi.EINVAL and "16 bytes" in _abi.last_error()
+    assert fwd(shape(), q=None) == _abi.EINVAL and "null" in _abi.last_error()
+    long = shape(nk=100000)
+    need = lib.dg_roi_attn_workspace_bytes(long, 0)
+    assert need > 0 and fwd(long, ws=p, n=need - 1) == _abi.ENOMEM and "workspace" in _abi.last_error()
+    assert fwd(shape(batch=0)) == _abi.OK and fwd(shape(nq=0)) == _abi.OK
+    assert lib.dg_roi_attn_workspace_bytes(shape(d=12), 1) == 0
+    assert lib.dg_roi_attn_bwd(shape(), p, p, p, p, p, p, None, None, None, p, p, None, p, 1 << 30, None) == _abi.EINVAL     # dk without dv
+
+    def rope(**kw):
+        s = _abi.RopeShape(1, 4, 2, 1, 64, 16, 2)
+        s.pos_dtype = _abi.F32
+        for a, b in kw.items():
+            setattr(s, a, b)
+        return lib.dg_rope_axes(s, p, p, p, p, p, 0, p, p, None)
+    for kw, word in ((dict(pairs=33), "do not fit"), (dict(pairs=0), "do not fit"), (dict(d=7), "even"), (dict(axes=17), "axes"), (dict(pairing=2), "pairing"),
+                     (dict(dtype=_abi.F64), "type"), (dict(pos_dtype=_abi.BF16), "positions"), (dict(n=-1), "token"), (dict(q_heads=0, k_heads=0), "head count")):
+        assert rope(**kw) == _abi.EINVAL, kw
+        assert word in _abi.last_error(), (kw, _abi.last_error())
+    assert rope(n=0) == _abi.OK
+
+    def logp(n=4, c=10, top=2, dtype=_abi.F32, z=p, y=p, logp_=p, ws=None, nbytes=0):
+        return lib.dg_class_logprobs(z, dtype, y, n, c, c, top, logp_, p, p, p, p, p, ws, nbytes, None)
+    for kw, word in ((dict(top=11), "alternatives"), (dict(c=100, top=33), "alternatives"), (dict(c=0, top=0), "classes"), (dict(dtype=_abi.F64), "type"),
+                     (dict(n=-1), "row count"), (dict(z=None), "null"), (dict(logp_=None), "null"), (dict(z=C.c_void_p(4097)), "aligned")):
+        assert logp(**kw) == _abi.EINVAL, kw
+        assert word in _abi.last_error(), (kw, _abi.last_error())
+    need = lib.dg_class_logprobs_workspace_bytes(1, 131072, 8)
+    assert need > 0 and logp(n=1, c=131072, top=8, ws=p, nbytes=need - 1) == _abi.ENOMEM
+    assert logp(n=0) == _abi.OK and logp(n=0, y=None) == _abi.OK
+    assert lib.dg_class_logprobs_bwd(p, _abi.F32, None, 4, 10, 10, p, p, p, None, p, None) == _abi.EINVAL     # a gradient of logp without labels
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="only meaningful on a host without a GPU")
+def test_no_cpu_fallback_of_the_head():
+    from vision_amd import _abi, fast_rcnn, ops
+    t = torch.zeros((1, 4, 2, 32))
+    for call in (lambda: ops.roi_attention(t, t, t), lambda: fast_rcnn.roi_attention(t, t, t), lambda: ops.rope_plan((8, 8)),
+                 lambda: ops.class_logprobs(torch.zeros((2, 5)), torch.zeros(2, dtype=torch.int64)), lambda: fast_rcnn.class_logprobs(torch.zeros((2, 5)))):
+        with pytest.raises(_abi.DetGeomError):
+            call()
+
+
+@pytest.mark.gpu
+def test_refusals_of_the_front_end():
+    from vision_amd import fast_rcnn, ops
+    t = torch.zeros((2, 6, 4, 32), device="cuda")
+    k = torch.zeros((2, 9, 2, 32), device="cuda")
+    out, lse = ops.roi_attention(t, k, k)
+    bad = [
+        lambda: ops.roi_attention(t[0], k, k), lambda: ops.roi_attention(t, k, k[:, :5]), lambda: ops.roi_attention(t, k[:1], k[:1]),
+        lambda: ops.roi_attention(t.half(), k.half(), k.half()), lambda: ops.roi_attention(t, k.bfloat16(), k), lambda: ops.roi_attention(t[:, :, :3], k, k),
+        lambda: ops.roi_attention(t[..., :12], k[..., :12], k[..., :12]), lambda: ops.roi_attention(t, k, k, scale=0.0), lambda: ops.roi_attention(t, k, k, scale=-1.0),
+        lambda: ops.roi_attention(t, k, k, q_counts=torch.zeros(3)), lambda: ops.roi_attention(t, k, k, k_counts=torch.zeros((2, 1))),
+        lambda: ops.roi_attention(t, k, k, mask=torch.zeros((2, 6, 9))), lambda: ops.roi_attention(t, k, k, mask=torch.zeros((3, 6, 9), dtype=torch.bool)),
+        lambda: ops.roi_attention(t, k, k, mask=torch.zeros((6, 8), dtype=torch.bool)),
+        lambda: ops.roi_attention_backward(t[:, :5], t, k, k, out, lse), lambda: ops.roi_attention_backward(t, t, k, k, out, lse.transpose(1, 2)),
+        lambda: ops.roi_attention_backward(t.bfloat16(), t, k, k, out, lse),
+        lambda: ops.rope_plan(()), lambda: ops.rope_plan((0, 0)), lambda: ops.rope_plan((8, -1)), lambda: ops.rope_plan((8,), theta=0.0),
+        lambda: ops.rope_plan((8,), ladder="x"), lambda: ops.rope_plan((8,), pairing="x"),
+        lambda: ops.rope_axes(t, torch.zeros((2, 6, 3)), ops.rope_plan((8, 8))), lambda: ops.rope_axes(t, torch.zeros((2, 6, 2)), ops.rope_plan((8, 9))),
+        lambda: ops.rope_axes(t, torch.zeros((2, 6, 2)), ops.rope_plan((8, 8)), k=k), lambda: ops.rope_axes(t.double(), torch.zeros((2, 6, 2)), ops.rope_plan((8, 8))),
+        lambda: ops.rope_axes(t, torch.zeros((2, 6, 2), device="cuda", requires_grad=True), ops.rope_plan((8, 8))),
+        lambda: fast_rcnn.rope_axes(t, t, torch.zeros((2, 6, 2), requires_grad=True), ops.rope_plan((8, 8))),
+        lambda: ops.class_logprobs(t, torch.zeros(2)), lambda: ops.class_logprobs(t[0, 0], torch.zeros(3, dtype=torch.int64)),
+        lambda: ops.class_logprobs(t[0, 0], torch.zeros(4, dtype=torch.int64), top=33), lambda: ops.class_logprobs(t[0, 0], torch.zeros(4, dtype=torch.int64), top=-1),
+        lambda: ops.class_logprobs(t[0, 0].double()), lambda: ops.class_logprobs_backward(None, torch.zeros(3), t[0, 0], None, torch.zeros((4, 2)), torch.zeros(4)),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            print("not refused:", i)
+    # nothing to do is no error
+    assert ops.roi_attention(t[:0], k[:0], k[:0])[0].shape == (0, 6, 4, 32)
+    o, s = ops.roi_attention(t, k[:, :0], k[:, :0])
+    assert float(o.abs().max()) == 0.0 and bool(torch.isinf(s).all())
+    dq, dk, dv = ops.roi_attention_backward(t, t, k[:, :0], k[:, :0], o, s)
+    assert float(dq.abs().max()) == 0.0 and dk.shape == (2, 0, 2, 32)
+    o, s = ops.roi_attention(t[:, :0], k, k)
+    dq, dk, dv = ops.roi_attention_backward(t[:, :0], t[:, :0], k, k, o, s)
+    assert dq.shape == (2, 0, 4, 32) and float(dk.abs().max()) == 0.0 and float(dv.abs().max()) == 0.0
+    assert ops.rope_axes(t[:, :0], torch.zeros((2, 0, 2)), ops.rope_plan((8, 8))).shape == (2, 0, 4, 32)
+    assert ops.class_logprobs(t[0, 0, :0], torch.zeros(0, dtype=torch.int64), 3)[4].shape == (0, 3)
+    assert ops.class_logprobs_backward(torch.zeros(0), None, t[0, 0, :0], torch.zeros(0, dtype=torch.int64), torch.zeros((0, 2)), torch.zeros(0)).shape == (0, 32)
