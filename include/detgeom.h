@@ -379,8 +379,8 @@ int dg_rope_axes(const dg_rope_shape *shape, const void *q, const void *k, const
 /* ---------------------------------------------------------------- the RoI head: log probabilities of labels
  * NO COUNTERPART IN THE REFERENCE (its classifiers end in torch's own loss).  logits (n, c): rows `stride` values apart, dense
  * classes; DG_F32, DG_BF16 or DG_F16.  labels (n) int64: a negative one gives none (logp 0, no gradient), one at or above c gives
- * NaN (logp, and the row's gradient) and sets bit 0 of *status (device int32, zeroed by the caller); labels may be NULL (then logp
- * and status may be).  Outputs, fp32: logp (n) = z_y - lse, entropy (n; may be NULL) of the row's distribution in nats, norm
+ * NaN (logp, and the row's gradient) and sets bit 0 of *status (device int32, zeroed by the caller, or NULL); labels may be NULL (then logp
+ * may be).  Outputs, fp32: logp (n) = z_y - lse, entropy (n; may be NULL) of the row's distribution in nats, norm
  * (n, 2) = the row's maximum m and log sum e^(z-m), whose sum is lse = log sum e^z, and the `top` (0 to 32, at most c) classes of the
  * largest logits, best first, equal logits by the lowest index, NaN last: top_logp (n, top), top_index (n, top) int64.  -inf is a
  * masked class; a row of nothing else gives logp = -inf, norm = (-inf, 0), entropy 0, no gradient.  A NaN or +inf makes its row's

@@ -402,55 +402,57 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         }
 }
 
-// Joins the splits of a row by their log-sums.  A row has 32 lanes of four values; up to 16 splits eight rows share a workgroup, more
-// of them are dealt to the workgroup's eight lane groups, which then add up through LDS.
+// Joins the splits of a row by their log-sums, four values of d a thread.  Up to 16 splits (MANY false) a row has 32 threads, eight
+// rows a workgroup; with more (few rows, a long walk) a workgroup has 32 values of one row, and its 32 groups of eight threads deal
+// the splits among themselves and add up through LDS (126 splits of 16 rows: 68 us by a wave a row, 11 by a workgroup a row, 7 so).
 #define AT_JOIN_FEW 16
 template <typename T, bool MANY>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, int64_t rows)
 {
     typedef typename at_vec<T>::quad quad;
-    __shared__ __attribute__((aligned(16))) f32x4 red[MANY ? 8 : 1][32];
-    __shared__ float tot8[8], max8[8];
-    const int grp = threadIdx.x >> 5, sub = threadIdx.x & 31;
-    const int64_t row = MANY ? blockIdx.x : (int64_t)blockIdx.x * 8 + grp;
+    constexpr int LANES = MANY ? 8 : 32, GROUPS = AT_THREADS / LANES;
+    __shared__ __attribute__((aligned(16))) f32x4 red[MANY ? GROUPS : 1][LANES];
+    __shared__ float tots[GROUPS], tops[AT_WAVES];
+    const int grp = threadIdx.x / LANES, sub = threadIdx.x % LANES, cuts = MANY ? (a.d + 31) / 32 : 1;
+    const int64_t row = MANY ? blockIdx.x / cuts : (int64_t)blockIdx.x * GROUPS + grp;
+    const int d = (MANY ? (int)(blockIdx.x % cuts) * 32 : 0) + sub * 4;
     if (row >= rows) return;                      // MANY: the whole workgroup
     const int n = (int)(row % a.nq), hq = (int)(row / a.nq % a.hq), b = (int)(row / a.nq / a.hq);
     if (n >= at_count(a.qc, b, a.nq)) return;     // written by the first kernel
-    const float *ls = a.part + row * a.splits, *po = a.part + rows * a.splits + row * a.splits * a.d;
-    const int s0 = MANY ? grp : 0, step = MANY ? 8 : 1;
+    const float *ls = a.part + row * a.splits, *po = a.part + rows * a.splits + row * a.splits * a.d + d;
     float m = -INFINITY;
-    for (int s = MANY ? (int)threadIdx.x : sub; s < a.splits; s += MANY ? AT_THREADS : 32) m = fmaxf(m, ls[s]);
+    for (int s = MANY ? (int)threadIdx.x : sub; s < a.splits; s += MANY ? AT_THREADS : LANES) m = fmaxf(m, ls[s]);
 #pragma unroll
-    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
+    for (int x = MANY ? 32 : LANES / 2; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x, 64));
     if (MANY) {
-        if (sub == 0) max8[grp] = m;
+        if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = m;
         __syncthreads();
 #pragma unroll
-        for (int g = 0; g < 8; ++g) m = fmaxf(m, max8[g]);
+        for (int w = 0; w < AT_WAVES; ++w) m = fmaxf(m, tops[w]);
     }
     const float base = m == -INFINITY ? 0.f : m;
-    const bool in = sub * 4 < a.d;
+    const bool in = d < a.d;
     float tot = 0.f;
     f32x4 v = (f32x4)(0.f);
 #pragma unroll 4
-    for (int s = s0; s < a.splits; s += step) {
+    for (int s = MANY ? grp : 0; s < a.splits; s += MANY ? GROUPS : 1) {
         const float w = __builtin_amdgcn_exp2f(ls[s] - base);
         tot += w;
-        if (in) v += *(const f32x4 *)(po + (int64_t)s * a.d + sub * 4) * w;
+        if (in) v += *(const f32x4 *)(po + (int64_t)s * a.d) * w;
     }
     if (MANY) {
         red[grp][sub] = v;
-        if (sub == 0) tot8[grp] = tot;
+        if (sub == 0) tots[grp] = tot;
         __syncthreads();
         if (grp) return;
-        for (int g = 1; g < 8; ++g) {
+        for (int g = 1; g < GROUPS; ++g) {
             v += red[g][sub];
-            tot += tot8[g];
+            tot += tots[g];
         }
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
-    if (in) *(quad *)(a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d + sub * 4) = __builtin_convertvector(v * inv, quad);
-    if (sub == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
+    if (in) *(quad *)(a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d + d) = __builtin_convertvector(v * inv, quad);
+    if (d == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
 }
 
 // ------------------------------------------------------------------ backward
@@ -751,9 +753,10 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
         }
 }
 
-// sums a gradient's splits in their order: rows (b, h, n) of the partial sums -> (b, n, h); rows behind a count are left alone
+// sums a gradient's splits in their order: rows (b, h, n) of the partial sums -> (b, n, h); rows behind a count are left alone; a second
+// gradient of the same shape (dv) follows the first one's partial sums
 template <typename T>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict__ part, T *__restrict__ out, const int32_t *__restrict__ counts, int64_t rows, int heads,
+__global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict__ part, T *__restrict__ out, T *__restrict__ out2, const int32_t *__restrict__ counts, int64_t rows, int heads,
                                                          int nmax, int d, int splits)
 {
     typedef typename at_vec<T>::quad quad;
@@ -761,11 +764,11 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict
     if (row >= rows) return;
     const int x = (int)(i - row * (d / 4)) * 4, n = (int)(row % nmax), hh = (int)(row / nmax % heads), b = (int)(row / nmax / heads);
     if (n >= at_count(counts, b, nmax)) return;
-    const float *p = part + row * splits * d + x;
+    const float *p = part + ((blockIdx.y ? rows : 0) + row) * splits * d + x;
     f32x4 v = (f32x4)(0.f);
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(p + (int64_t)s * d);
-    *(quad *)(out + (((int64_t)b * nmax + n) * heads + hh) * d + x) = __builtin_convertvector(v, quad);
+    *(quad *)((blockIdx.y ? out2 : out) + (((int64_t)b * nmax + n) * heads + hh) * d + x) = __builtin_convertvector(v, quad);
 }
 
 // pair mask -> bits: a word of 32 keys per thread
@@ -903,7 +906,7 @@ static int at_forward(const dg_attn_shape *s, const void *q, const void *k, cons
     a.o = (T *)out; a.lse = lse; a.part = (float *)ws;
     a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
     AT_LAUNCH(k_attn_fwd, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
-    if (p.qsplits > AT_JOIN_FEW) hipLaunchKernelGGL((k_attn_join<T, true>), dim3((unsigned)p.rows), dim3(AT_THREADS), 0, st, a, p.rows);
+    if (p.qsplits > AT_JOIN_FEW) hipLaunchKernelGGL((k_attn_join<T, true>), dim3((unsigned)(p.rows * dg_cdiv(s->d, 32))), dim3(AT_THREADS), 0, st, a, p.rows);
     else if (p.qsplits > 1) hipLaunchKernelGGL((k_attn_join<T, false>), dim3((unsigned)dg_cdiv(p.rows, 8)), dim3(AT_THREADS), 0, st, a, p.rows);
     DG_CHECK_LAUNCH("k_attn_fwd");
     return DG_OK;
@@ -945,7 +948,7 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
         a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
         AT_LAUNCH(k_attn_dq, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
         if (p.qsplits > 1)
-            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d / 4, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, qc, p.rows,
+            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d / 4, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, (T *)nullptr, qc, p.rows,
                                (int)s->q_heads, (int)s->nq, (int)s->d, (int)p.qsplits);
     }
     if (s->nk > 0 && dk) {
@@ -953,12 +956,9 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
         a.tiles = (int)p.ktiles; a.splits = (int)p.ksplits; a.per = (int)p.kper;
         AT_LAUNCH(k_attn_dkv, s->batch * s->k_heads * p.ktiles * p.ksplits, a);
         if (p.ksplits > 1) {
-            const int64_t rows = s->batch * s->k_heads * s->nk, half = rows * p.ksplits * s->d;
-            const dim3 grid((unsigned)dg_cdiv(rows * s->d / 4, AT_THREADS));
-            hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dk, (const int32_t *)nullptr, rows, (int)s->k_heads,
-                               (int)s->nk, (int)s->d, (int)p.ksplits);
-            hipLaunchKernelGGL((k_attn_sum<T>), grid, dim3(AT_THREADS), 0, st, (const float *)a.part + half, (T *)dv, (const int32_t *)nullptr, rows, (int)s->k_heads,
-                               (int)s->nk, (int)s->d, (int)p.ksplits);
+            const int64_t rows = s->batch * s->k_heads * s->nk;
+            hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(rows * s->d / 4, AT_THREADS), 2), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dk, (T *)dv,
+                               (const int32_t *)nullptr, rows, (int)s->k_heads, (int)s->nk, (int)s->d, (int)p.ksplits);
         }
     }
     DG_CHECK_LAUNCH("k_attn_dkv");

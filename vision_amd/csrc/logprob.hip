@@ -129,7 +129,7 @@ __device__ __forceinline__ void lp_write(const lp_args &a, int64_t row, const lp
     if (a.y) {
         const int64_t y = a.y[row];
         float v = 0.f;                            // a negative label: no class given
-        if (y >= a.c) { v = __builtin_nanf(""); atomicOr(a.status, 1); }
+        if (y >= a.c) { v = __builtin_nanf(""); if (a.status) atomicOr(a.status, 1); }
         else if (y >= 0) v = nm.of((float)((const T *)a.z)[row * a.stride + y]);
         a.logp[row] = v;
     }
@@ -438,7 +438,7 @@ extern "C" int dg_class_logprobs(const void *logits, int dtype, const int64_t *l
     const int rc = lp_check(n, c, stride, dtype, top, "class_logprobs");
     if (rc != DG_OK) return rc;
     if (n == 0) return DG_OK;
-    DG_REQUIRE(logits && norm && (!labels || (logp && status)) && (!top || (top_logp && top_index)), "class_logprobs: null pointer");
+    DG_REQUIRE(logits && norm && (!labels || logp) && (!top || (top_logp && top_index)), "class_logprobs: null pointer");
     DG_REQUIRE((((uintptr_t)logits) & (dtype == DG_F32 ? 3 : 1)) == 0, "class_logprobs: logits are not aligned to their type");
     const size_t need = dg_class_logprobs_workspace_bytes(n, c, top);
     if (ws_bytes < need || (need && !ws)) { dg_set_error("class_logprobs: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }

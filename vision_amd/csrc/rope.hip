@@ -16,8 +16,8 @@ struct rp_args {
     const double *turns;
     const int32_t *axis;
     int64_t xs[2][3], ps[2];                      // strides in values: batch, token, head; pos: batch, token
-    int64_t tokens;
-    int n, heads[2], d, pairs, axes, tok, units;  // tok: tokens of a workgroup, units: pieces of a head
+    u32 tokens, n, heads[2], d, pairs, tok, units;   // tok: tokens of a workgroup, units: pieces of a head
+    int axes;
     float sign;
 };
 
@@ -29,11 +29,9 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
 {
     typedef rp_piece<T, VEC> piece;
     extern __shared__ float2 cs[];                // [tok][pairs]
-    const int64_t t0 = (int64_t)blockIdx.x * a.tok;
-    const int nt = (int)min((int64_t)a.tok, a.tokens - t0);
-    for (int i = threadIdx.x; i < nt * a.pairs; i += 256) {
-        const int t = i / a.pairs, j = i - t * a.pairs;
-        const int64_t tok = t0 + t, b = tok / a.n, n = tok - b * a.n;
+    const u32 t0 = blockIdx.x * (u32)a.tok, nt = min((u32)a.tok, a.tokens - t0);       // tokens number fewer than 2^31
+    for (u32 i = threadIdx.x; i < nt * a.pairs; i += 256) {
+        const u32 t = i / a.pairs, j = i - t * a.pairs, b = (t0 + t) / a.n, n = t0 + t - b * a.n;
         const int ax = min(max(a.axis[j], 0), a.axes - 1);
         double r = (double)((const P *)a.pos)[b * a.ps[0] + n * a.ps[1] + ax] * a.turns[j];
         r -= rint(r);
@@ -42,17 +40,16 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
         cs[i] = make_float2(c, s * a.sign);
     }
     __syncthreads();
-    const int per = a.units * (a.heads[0] + a.heads[1]), turning = (HALVES ? a.pairs : 2 * a.pairs) / VEC;
-    for (int i = threadIdx.x; i < nt * per; i += 256) {
-        const int t = i / per, r = i - t * per, hh = r / a.units, u = r - hh * a.units;
-        const int w = hh >= a.heads[0], h = w ? hh - a.heads[0] : hh;
-        const int64_t tok = t0 + t, b = tok / a.n, n = tok - b * a.n;
+    const u32 per = a.units * (a.heads[0] + a.heads[1]), turning = (HALVES ? a.pairs : 2 * a.pairs) / VEC;
+    for (u32 i = threadIdx.x; i < nt * per; i += 256) {
+        const u32 t = i / per, r = i - t * per, hh = r / a.units, u = r - hh * a.units;
+        const u32 w = hh >= a.heads[0], h = w ? hh - a.heads[0] : hh, b = (t0 + t) / a.n, n = t0 + t - b * a.n;
         const T *x = (const T *)a.x[w] + b * a.xs[w][0] + n * a.xs[w][1] + h * a.xs[w][2];
-        T *y = (T *)a.y[w] + (tok * a.heads[w] + h) * a.d;
+        T *y = (T *)a.y[w] + ((int64_t)(t0 + t) * a.heads[w] + h) * a.d;
         const float2 *c = cs + t * a.pairs;
         if (HALVES) {
             if (u < turning) {
-                const int j = u * VEC;
+                const u32 j = u * VEC;
                 const piece p = *(const piece *)(x + j), q = *(const piece *)(x + a.pairs + j);
                 piece o, s;
 #pragma unroll
@@ -65,11 +62,11 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
                 *(piece *)(y + j) = o;
                 *(piece *)(y + a.pairs + j) = s;
             } else {
-                const int j = 2 * a.pairs + (u - turning) * VEC;
+                const u32 j = 2 * a.pairs + (u - turning) * VEC;
                 *(piece *)(y + j) = *(const piece *)(x + j);
             }
         } else {
-            const int j = u * VEC;
+            const u32 j = u * VEC;
             piece p = *(const piece *)(x + j);
             if (u < turning) {
 #pragma unroll
@@ -101,7 +98,7 @@ static void rp_launch(const rp_args &a0, bool halves, hipStream_t st)
     while (a.tok < 16 && a.tok * a.pairs < 256) a.tok *= 2;
     const dim3 grid((unsigned)dg_cdiv(a.tokens, a.tok)), block(256);
     const size_t lds = (size_t)a.tok * a.pairs * sizeof(float2);
-    const int rest = a.d - 2 * a.pairs;
+    const u32 rest = a.d - 2 * a.pairs;
     if (halves) {
         a.units = wide ? (a.pairs + rest) / V : a.pairs + rest;
         if (wide) hipLaunchKernelGGL((k_rope_axes<T, P, V, true>), grid, block, lds, st, a);
@@ -135,8 +132,8 @@ extern "C" int dg_rope_axes(const dg_rope_shape *s, const void *q, const void *k
     a.pos = pos; a.turns = turns; a.axis = axis;
     for (int i = 0; i < 3; ++i) { a.xs[0][i] = s->q_stride[i]; a.xs[1][i] = s->k_stride[i]; }
     a.ps[0] = s->pos_stride[0]; a.ps[1] = s->pos_stride[1];
-    a.tokens = tokens; a.n = (int)s->n; a.heads[0] = (int)s->q_heads; a.heads[1] = (int)s->k_heads;
-    a.d = (int)s->d; a.pairs = (int)s->pairs; a.axes = (int)s->axes; a.sign = inverse ? -1.f : 1.f;
+    a.tokens = (u32)tokens; a.n = (u32)s->n; a.heads[0] = (u32)s->q_heads; a.heads[1] = (u32)s->k_heads;
+    a.d = (u32)s->d; a.pairs = (u32)s->pairs; a.axes = (int)s->axes; a.sign = inverse ? -1.f : 1.f;
     const bool halves = s->pairing == DG_ROPE_HALVES, p64 = s->pos_dtype == DG_F64;
     hipStream_t st = (hipStream_t)stream;
     if (s->dtype == DG_F32) p64 ? rp_launch<float, double>(a, halves, st) : rp_launch<float, float>(a, halves, st);
