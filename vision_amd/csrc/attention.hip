@@ -133,16 +133,16 @@ __device__ __forceinline__ int at_xcd_id(int per)  // per: tiles x splits of a p
     return whole * per + x * q + min(x, r) + j - (whole >> 3) * per;
 }
 
-// Images of different counts: the workgroups that come first take the images with the most pairs of rows and keys, so that what
-// runs last is short.  i-th image in that order (equal ones by index); every wave finds it for itself from the counts.
-__device__ __forceinline__ int at_image(int i, int batch, const int32_t *qc, const int32_t *kc, int nq, int nk)
+// Images of different counts: the workgroups that come first take the images with the longest walk (keys in the forward and dq
+// kernels, rows in the other), so that what runs last is short.  i-th image in that order (equal ones by index); every wave finds it
+// for itself from the counts.
+__device__ __forceinline__ int at_image(int i, int batch, const int32_t *counts, int n)
 {
-    if ((!qc && !kc) || batch < 2 || batch > 64) return i;
-    const int lane = threadIdx.x & 63;
-    const float w = lane < batch ? (float)at_count(qc, lane, nq) * (float)at_count(kc, lane, nk) : -1.f;
+    if (!counts || batch < 2 || batch > 64) return i;
+    const int lane = threadIdx.x & 63, w = lane < batch ? at_count(counts, lane, n) : -1;
     int rank = 0;
     for (int j = 0; j < batch; ++j) {
-        const float o = __uint_as_float((u32)__builtin_amdgcn_readlane((int)__float_as_uint(w), j));
+        const int o = __builtin_amdgcn_readlane(w, j);
         rank += o > w || (o == w && j < lane);
     }
     return __ffsll((unsigned long long)__ballot(lane < batch && rank == i)) - 1;
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.kc, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
 
@@ -502,7 +502,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
     __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.kc, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int R = G * nq, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
 
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
     __shared__ __attribute__((aligned(16))) char vt[VL ? 32 * AT_WAVES * tile::RB : 16];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
-    const int b = at_image(bh / a.hk, a.batch, a.qc, a.kc, a.nq, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
+    const int b = at_image(bh / a.hk, a.batch, a.qc, a.nq), hk = bh % a.hk, G = a.hq / a.hk;
     const int nq = at_count(a.qc, b, a.nq), nk = at_count(a.kc, b, a.nk);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5;
     // the walk: row tiles of each query head of the group in turn; none where all keys lie behind the image's last one (zeros)
