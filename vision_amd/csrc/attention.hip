@@ -234,6 +234,11 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // ------------------------------------------------------------------ forward
 // A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of 64.  K and V tiles are double
 // buffered in LDS; the next tile's global loads are in flight while this one is computed.
+// The wave that has scores to multiply goes first, then one that has values to, then the vector work: with equal priorities the two
+// waves of a SIMD drift into the same phase and the matrix unit waits (16000 x 128: forward 1101 -> 1040 us, dq 1575 -> 1511, dk, dv
+// 2253 -> 2140; no difference at 64, where three or four waves share a SIMD).
+#define AT_PRIO(p) __builtin_amdgcn_s_setprio(p)
+
 // Never taken (d is 8 at least): it parts a turn of the loop between the products and the exponentials.  In one piece the scheduler
 // keeps so many operands of later products in registers that others are spilled (16001 x 128: dk, dv 2545 -> 2220 us, dq 1650 -> 1530).
 #define AT_PART(when) if ((when) && a.d <= 0) break
@@ -324,12 +329,14 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         for (int u = 0; u < U; ++u) mnext[u] = MASK ? at_word(mp, kb + KT + 32 * u, k1) : 0;
         const char *K = lds[buf][0], *V = lds[buf][1];
         f32x16 s[U];
+        AT_PRIO(2);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             s[u] = (f32x16)(0.f);
 #pragma unroll
             for (int g = 0; g < NG; ++g) s[u] = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s[u]);
         }
+        AT_PRIO(0);
         if (MASK || !more) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -362,7 +369,9 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
                 s[u][e] = p;
                 l += p;
             }
+            AT_PRIO(1);
             at_acc_t<DP>(o, V, u * 32, s[u], lane, (const T *)nullptr);
+            AT_PRIO(0);
         }
         if (more) store(buf ^ 1);
 #pragma unroll
@@ -571,11 +580,13 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             f32x16 s = (f32x16)(0.f), dp = (f32x16)(stat[1]);
+            AT_PRIO(2);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 s = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
                 dp = at_mma(tile::row_frag(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
             }
+            AT_PRIO(0);
             const int left = k1 - kb - u * 32;
             const u32 w = (MASK ? mw[u] : left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u) >> (4 * h);
             AT_PART(DP == 128);
@@ -585,7 +596,9 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
                 if (MASK || !more) ds = w & (1u << (8 * (e >> 2) + (e & 3))) ? ds : 0.f;
                 s[e] = ds;
             }
+            AT_PRIO(1);
             at_acc_t<DP>(o, K, u * 32, s, lane, (const T *)nullptr);
+            AT_PRIO(0);
         }
         if (more) store(buf ^ 1);
 #pragma unroll
@@ -704,6 +717,7 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
         asm volatile("" : "+v"(ln));
         const int lr = ln & 31, lh = ln >> 5;
         f32x16 s = (f32x16)(0.f), dp;
+        AT_PRIO(2);
 #pragma unroll
         for (int g = 0; g < NG; ++g) s = at_mma(tile::row_frag(Q, lr, 2 * g + lh), kf[g], s);
 #pragma unroll
@@ -711,6 +725,7 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
 #pragma unroll
         for (int g = 0; g < NG; ++g)
             dp = at_mma(tile::row_frag(GO, lr, 2 * g + lh), VL ? *(const frag *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
+        AT_PRIO(0);
         AT_PART(DP >= 64);
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -(*(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh])[e & 3]));
@@ -724,10 +739,10 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
             }
             dp[e] = ds;
         }
-        
+        AT_PRIO(1);
         at_acc_t<DP>(ov, GO, 0, s, ln, (const T *)nullptr);
-        
         at_acc_t<DP>(ok, Q, 0, dp, ln, (const T *)nullptr);
+        AT_PRIO(0);
         if (more) store(buf ^ 1);
         __syncthreads();
     }
