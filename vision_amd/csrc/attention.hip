@@ -236,8 +236,8 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // buffered in LDS; the next tile's global loads are in flight while this one is computed.
 // The wave that has scores to multiply goes first, then one that has values to, then the vector work: with equal priorities the two
 // waves of a SIMD drift into the same phase and the matrix unit waits (16000 x 128: forward 1101 -> 1040 us, dq 1575 -> 1511, dk, dv
-// 2253 -> 2140; no difference at 64, where three or four waves share a SIMD).
-#define AT_PRIO(p) __builtin_amdgcn_s_setprio(p)
+// 2253 -> 2140).  Up to 64, where three or four waves share a SIMD, it only keeps the scheduler from mixing the phases (dk, dv 101 -> 126).
+#define AT_PRIO(p) do { if (DP == 128) __builtin_amdgcn_s_setprio(p); } while (0)
 
 // Never taken (d is 8 at least): it parts a turn of the loop between the products and the exponentials.  In one piece the scheduler
 // keeps so many operands of later products in registers that others are spilled (16001 x 128: dk, dv 2545 -> 2220 us, dq 1650 -> 1530).
