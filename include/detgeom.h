@@ -338,9 +338,8 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * A row i sees key j if i < q_counts[image], j < k_counts[image] (device int32, held to [0, n]; NULL = all) and mask[image][i][j] != 0
  * (device bytes, a row's keys dense, strides of image and row in bytes; shape->masks of them, NULL with 0 = all).  What lies behind a count is
  * never read.  A row that sees nothing gives out = 0, lse = -inf and has no gradient; so do the rows behind q_counts, and dk = dv = 0
- * behind k_counts: every element of every output is written.  With a mask, a key that a row may not see does not reach it whatever
- * its values are; a row that sees a key or value holding a NaN or an infinity (and with a mask, in the backward pass, a row
- * holding one in q or grad_out) gives NaN.
+ * behind k_counts: every element of every output is written.  A pair that a count or a mask excludes adds nothing, whatever its values
+ * are.  A NaN or an infinity in what a row does see makes that row's results NaN or infinite, and with a mask NaN.
  * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
  * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products.  Results are the
  * same in every run (no atomics). */

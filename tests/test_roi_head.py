@@ -197,6 +197,7 @@ ROPE_CASES = [
     (3, 19, 5, 1, 22, (3, 4), "axis", "halves", torch.float32),
     (1, 1000, 8, 8, 128, (16, 24, 24), "axis", "halves", torch.float32),
     (2, 5, 2, 0, 32, (0, 16), "axis", "halves", torch.float32),
+    (2, 16, 4, 2, 64, (8, 8), "axis", "neighbours", torch.float64),
 ]
 
 
@@ -268,7 +269,7 @@ def _logp64(z, y, top, g=None, gh=None):
     return r
 
 
-LOGP_CASES = [(1, 1, 1), (1, 2, 2), (5, 21, 3), (300, 81, 5), (257, 33, 32), (64, 512, 8), (33, 513, 8), (7, 1000, 32), (40, 4096, 4), (3, 4097, 8),
+LOGP_CASES = [(1, 1, 1), (1, 2, 2), (5, 21, 3), (300, 81, 5), (20, 200, 6), (257, 33, 32), (64, 512, 8), (33, 513, 8), (7, 1000, 32), (40, 4096, 4), (3, 4097, 8),
               (2, 20011, 5), (1, 131072, 8), (600, 5003, 1), (1, 70001, 0)]
 
 
@@ -719,3 +720,57 @@ def test_refusals_of_the_front_end():
     assert ops.rope_axes(t[:, :0], torch.zeros((2, 0, 2)), ops.rope_plan((8, 8))).shape == (2, 0, 4, 32)
     assert ops.class_logprobs(t[0, 0, :0], torch.zeros(0, dtype=torch.int64), 3)[4].shape == (0, 3)
     assert ops.class_logprobs_backward(torch.zeros(0), None, t[0, 0, :0], torch.zeros(0, dtype=torch.int64), torch.zeros((0, 2)), torch.zeros(0)).shape == (0, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_class_logprobs_large_gradient(dtype):
+    """2^24 scores and more, dense, rows apart, and a gradient that starts off its 16 bytes."""
+    import ctypes as C
+    from vision_amd import _abi, ops
+    n, c = 520, 32771
+    rng = torch.Generator(device="cuda").manual_seed(9)
+    z = (torch.randn((n, c), generator=rng, device="cuda") * 3).to(dtype)
+    y = torch.randint(0, c, (n,), generator=rng, device="cuda")
+    g, gh = torch.randn((n,), generator=rng, device="cuda"), torch.randn((n,), generator=rng, device="cuda")
+    want = _logp64(z, y, 2, g, gh)
+    cpu = lambda t: tuple(x.cpu() for x in t)      # noqa: E731
+    logp, entropy, norm, best, index = ops.class_logprobs(z, y, 2)
+    _close(logp, cpu(want["logp"]), "logp")
+    _close(entropy, cpu(want["entropy"]), "entropy")
+    assert torch.equal(index, want["index"])
+    dz = ops.class_logprobs_backward(g, gh, z, y, norm, entropy)
+    _close(dz, cpu(want["dz"]), "dz")
+    wide = torch.zeros((n, c + 5), dtype=dtype, device="cuda")
+    wide[:, 2:c + 2] = z
+    assert torch.equal(ops.class_logprobs_backward(g, gh, wide[:, 2:c + 2], y, norm, entropy), dz)
+    m = 40                                        # the first rows once more through the C ABI, one value off
+    off = torch.full((m * c + 2,), 7.0, dtype=dtype, device="cuda")
+    rc = _abi.load().dg_class_logprobs_bwd(z.data_ptr(), _abi.TYPES[dtype], y.data_ptr(), m, c, c, norm.data_ptr(), entropy.data_ptr(), g.data_ptr(), gh.data_ptr(),
+                                           off[1:].data_ptr(), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == _abi.OK
+    torch.cuda.synchronize()
+    assert torch.equal(off[1:-1].view(m, c), dz[:m]) and float(off[0]) == 7.0 and float(off[-1]) == 7.0
+
+
+@pytest.mark.gpu
+def test_class_logprobs_status_and_bad_rows():
+    """A label outside the classes is told by the status word and by NaN; a NaN or +inf makes its row NaN and no other."""
+    import ctypes as C
+    from vision_amd import _abi, ops
+    for c in (10, 700):
+        z = torch.randn((6, c), generator=_gen(3)).cuda()
+        z[1, 4], z[2, 5] = math.nan, math.inf
+        y = torch.tensor([0, 1, 2, -5, c, 3]).cuda()
+        logp, entropy, norm, best, index = ops.class_logprobs(z, y, 3)
+        assert torch.isnan(logp[[1, 2, 4]]).all() and torch.isfinite(logp[[0, 3, 5]]).all() and float(logp[3]) == 0.0
+        assert torch.isnan(entropy[[1, 2]]).all() and torch.isfinite(entropy[[0, 3, 4, 5]]).all()
+        assert torch.equal(index[1], torch.sort(torch.where(torch.isnan(z[1]), -math.inf, z[1]), descending=True, stable=True).indices[:3])     # NaN last
+        dz = ops.class_logprobs_backward(torch.ones(6), torch.ones(6), z, y, norm, entropy)
+        assert torch.isnan(dz[[1, 2, 4]]).all() and torch.isfinite(dz[[0, 3, 5]]).all()
+        out = [torch.empty(6, device="cuda"), torch.empty(6, device="cuda"), torch.empty((6, 2), device="cuda")]
+        for labels, bit in ((y, 1), (y.clamp(max=c - 1), 0)):
+            status = torch.zeros(1, dtype=torch.int32, device="cuda")
+            rc = _abi.load().dg_class_logprobs(z.data_ptr(), _abi.F32, labels.data_ptr(), 6, c, c, 0, *(t.data_ptr() for t in out), None, None, status.data_ptr(), None, 0,
+                                               C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            assert rc == _abi.OK and int(status.item()) == bit

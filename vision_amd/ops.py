@@ -433,7 +433,7 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
     defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  No reference
     counterpart.  For a gradient: fast_rcnn.roi_attention."""
     dev, q, k, v, qc, kc, mask, masks, ms = _attn_args(q, k, v, q_counts, k_counts, mask)
-    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, scale, q.dtype, 0)
+    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, None if scale is None else float(scale), q.dtype, 0)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
     ws = _scratch(nbytes, dev)
@@ -455,7 +455,7 @@ def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         raise ValueError("roi_attention_backward: lse must be (B,Hq,Nq) float32")
     g, out = _vec16(g), _vec16(out)
-    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, scale, q.dtype, 1)
+    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, None if scale is None else float(scale), q.dtype, 1)
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
     dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
     dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
