@@ -53,6 +53,13 @@ __device__ __forceinline__ float lp_wave_max(float v)
     return __uint_as_float((u32)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
 }
 
+// every lane's value to the lane behind it (the first lane's result is no one's)
+__device__ __forceinline__ u64 lp_behind(u64 v)
+{
+    const u32 lo = (u32)__builtin_amdgcn_update_dpp(0, (int)(u32)v, 0x138, 0xf, 0xf, false), hi = (u32)__builtin_amdgcn_update_dpp(0, (int)(u32)(v >> 32), 0x138, 0xf, 0xf, false);
+    return ((u64)hi << 32) | lo;                  // wave_shr:1
+}
+
 // the best keys seen by a wave, ascending (best first): lane i holds the i-th
 struct lp_list {
     u64 list = LP_NONE, thr = LP_NONE;
@@ -61,7 +68,7 @@ struct lp_list {
         u64 some = __ballot(key < thr);
         while (some) {
             const int l = __ffsll((unsigned long long)some) - 1;
-            const u64 c = lp_lane(key, l), up = __shfl_up(list, 1, 64);
+            const u64 c = lp_lane(key, l), up = lp_behind(list);
             list = list < c ? list : (lane == 0 || up < c) ? c : up;
             thr = lp_lane(list, keep - 1);
             if (lane == l) key = LP_NONE;
