@@ -99,26 +99,31 @@ def nms(rects, scores):
 class _RoIAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_counts, k_counts, mask, scale):
-        out, lse = ops.roi_attention(q, k, v, q_counts, k_counts, mask, scale)
-        ctx.save_for_backward(q, k, v, out, lse, q_counts, k_counts, mask)
-        ctx.scale = scale
+        args = ops._attn_args(q, k, v, q_counts, k_counts, mask)
+        out, lse = ops._attn_forward(args, scale)
+        ctx.save_for_backward(*args[1:7], out, lse)     # as they were laid out for the kernels
+        ctx.rest = args[0], args[7], args[8], scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, out, lse, q_counts, k_counts, mask = ctx.saved_tensors
+        *args, out, lse = ctx.saved_tensors
+        dev, masks, ms, scale = ctx.rest
         need = ctx.needs_input_grad
-        dq, dk, dv = ops.roi_attention_backward(grad_out, q, k, v, out, lse, q_counts, k_counts, mask, ctx.scale, need[0], need[1] or need[2])
+        dq, dk, dv = ops._attn_backward((dev, *args, masks, ms), grad_out, out, lse, scale, need[0], need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 
 def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
     """ops.roi_attention's out, with a gradient for q, k and v.  Tensors on the CPU are copied in and the result back."""
     dev = ops._abi.device_of(q, k, v)
-    was_cpu = not any(t.is_cuda for t in (q, k, v))
-    qc, kc, m = (c if c is None else torch.as_tensor(c).to(dev) for c in (q_counts, k_counts, mask))
-    out = _RoIAttentionFn.apply(q.to(dev), k.to(dev), v.to(dev), qc, kc, m, scale)
+    was_cpu = not (q.is_cuda or k.is_cuda or v.is_cuda)
+    if not (q.device == dev and k.device == dev and v.device == dev):
+        q, k, v = q.to(dev), k.to(dev), v.to(dev)
+    if mask is not None and not isinstance(mask, torch.Tensor):
+        mask = torch.as_tensor(mask)
+    out = _RoIAttentionFn.apply(q, k, v, q_counts, k_counts, mask, scale)
     return out.cpu() if was_cpu else out
 
 
@@ -157,19 +162,21 @@ def rope_axes(q, k, pos, plan):
 class _ClassLogprobsFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, top):
-        logp, entropy, norm, best, index = ops.class_logprobs(logits, labels, top)
+        dev, z, y = ops._logits(logits, labels, "class_logprobs")
+        logp, entropy, norm, best, index = ops._logprobs(dev, z, y, top)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, labels, norm, entropy)
+        ctx.save_for_backward(z, y, norm, entropy)
         ctx.mark_non_differentiable(best, index)
         return logp, entropy, best, index
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, gh, _best, _index):
-        logits, labels, norm, entropy = ctx.saved_tensors
+        z, y, norm, entropy = ctx.saved_tensors
         if g is None and gh is None:
             return None, None, None
-        return ops.class_logprobs_backward(g, gh, logits, labels, norm, entropy), None, None
+        g, gh = (t if t is None else t.contiguous() for t in (g, gh))
+        return ops._logprobs_backward(z.device, z, y, norm, entropy, g, gh), None, None
 
 
 ClassLogprobs = namedtuple("ClassLogprobs", "logp entropy top_logp top_index")
@@ -181,6 +188,5 @@ def class_logprobs(logits, labels=None, top=0):
     Tensors on the CPU are copied in and the results back."""
     dev = ops._abi.device_of(logits)
     was_cpu = not logits.is_cuda
-    y = labels if labels is None else torch.as_tensor(labels).to(device=dev, dtype=torch.int64)
-    r = _ClassLogprobsFn.apply(logits.to(dev), y, int(top))
-    return ClassLogprobs(*(t.cpu() if was_cpu and t is not None else t for t in r))
+    r = _ClassLogprobsFn.apply(logits.to(dev) if was_cpu else logits, labels, int(top))
+    return ClassLogprobs(*(t if t is None else t.cpu() for t in r)) if was_cpu else ClassLogprobs(*r)

@@ -432,7 +432,11 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
     lse (B,Hq,Nq) float32.  A row sees the keys before k_counts (B) of its image for which mask (B or 1,Nq,Nk) is not 0; scale
     defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  No reference
     counterpart.  For a gradient: fast_rcnn.roi_attention."""
-    dev, q, k, v, qc, kc, mask, masks, ms = _attn_args(q, k, v, q_counts, k_counts, mask)
+    return _attn_forward(_attn_args(q, k, v, q_counts, k_counts, mask), scale)
+
+
+def _attn_forward(args, scale):
+    dev, q, k, v, qc, kc, mask, masks, ms = args
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, None if scale is None else float(scale), q.dtype, 0)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
@@ -446,15 +450,20 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
 def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=None, mask=None, scale=None, need_q=True, need_kv=True):
     """Gradients of roi_attention from its inputs, out and lse, with the probabilities recomputed: dq (B,Nq,Hq,D), dk and dv
     (B,Nk,Hk,D), rows behind a count 0.  need_q / need_kv False leaves those out (None)."""
-    dev, q, k, v, qc, kc, mask, masks, ms = _attn_args(q, k, v, q_counts, k_counts, mask)
+    args = _attn_args(q, k, v, q_counts, k_counts, mask)
+    dev, q = args[0], args[1]
     if not (grad_out.device == dev and out.device == dev and lse.device == dev):
         grad_out, out, lse = grad_out.to(dev), out.to(dev), lse.to(dev)
-    g, out, lse = grad_out, out.contiguous(), lse.contiguous()
-    if g.shape != q.shape or out.shape != q.shape or g.dtype != q.dtype or out.dtype != q.dtype:
+    if grad_out.shape != q.shape or out.shape != q.shape or grad_out.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError("roi_attention_backward: grad_out and out must have q's shape and type")
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         raise ValueError("roi_attention_backward: lse must be (B,Hq,Nq) float32")
-    g, out = _vec16(g), _vec16(out)
+    return _attn_backward(args, grad_out, _vec16(out.contiguous()), lse.contiguous(), scale, need_q, need_kv)
+
+
+def _attn_backward(args, g, out, lse, scale, need_q, need_kv):
+    dev, q, k, v, qc, kc, mask, masks, ms = args
+    g = _vec16(g)
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, None if scale is None else float(scale), q.dtype, 1)
     dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
     dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
@@ -563,10 +572,12 @@ def class_logprobs(logits, labels=None, top=0):
     norm (n,2) (the row's maximum and the log of its sum of exponentials above it: what the gradient needs), top_logp (n,top),
     top_index (n,top) int64: the most probable classes, best first, equal logits by the lowest index (top 0 to 32).  A negative label gives none (logp 0, no gradient); a label of C or more gives NaN.  -inf is a masked class.
     No reference counterpart.  For a gradient: fast_rcnn.class_logprobs."""
-    dev, z, y = _logits(logits, labels, "class_logprobs")
+    return _logprobs(*_logits(logits, labels, "class_logprobs"), int(top))
+
+
+def _logprobs(dev, z, y, top):
     n, c = z.shape
     f32 = dict(dtype=torch.float32, device=dev)
-    top = int(top)
     if not 0 <= top <= min(32, c):
         raise ValueError("class_logprobs: top must be 0 to 32 and no more than the classes")
     logp = torch.empty((n,), **f32) if y is not None else None
@@ -591,9 +602,13 @@ def class_logprobs_backward(grad_logp, grad_entropy, logits, labels, norm, entro
         if t is not None and t.shape != shape:
             raise ValueError("class_logprobs_backward: norm (n,2), entropy and the gradients (n)")
         args.append(t)
-    if y is None:
-        args[2] = None
+    return _logprobs_backward(dev, z, y, *args)
+
+
+def _logprobs_backward(dev, z, y, norm, entropy, g, gh):
+    n, c = z.shape
     dz = torch.empty((n, c), dtype=z.dtype, device=dev)
     with _abi.on_device(dev):
-        check(load().dg_class_logprobs_bwd(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), *(_at(t) for t in args), dz.data_ptr(), _stream(dev)))
+        check(load().dg_class_logprobs_bwd(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), norm.data_ptr(), entropy.data_ptr(),
+                                           _at(g) if y is not None else None, _at(gh), dz.data_ptr(), _stream(dev)))
     return dz
