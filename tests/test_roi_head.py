@@ -774,3 +774,19 @@ def test_class_logprobs_status_and_bad_rows():
             rc = _abi.load().dg_class_logprobs(z.data_ptr(), _abi.F32, labels.data_ptr(), 6, c, c, 0, *(t.data_ptr() for t in out), None, None, status.data_ptr(), None, 0,
                                                C.c_void_p(torch.cuda.current_stream().cuda_stream))
             assert rc == _abi.OK and int(status.item()) == bit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,c,first", [(3, 4000, 2500), (300, 20000, 9000)])
+def test_class_logprobs_best_behind_nan(n, c, first):
+    """The classes of a row that begins with more NaN than are looked at in one turn are still ranked before the NaN."""
+    from vision_amd import ops
+    z = torch.randn(n, c, generator=_gen(61))
+    z[:, :first] = math.nan
+    z[:, first::7] = -math.inf
+    index = ops.class_logprobs(_dev(z), None, 5)[4].cpu()
+    assert torch.equal(index, torch.sort(torch.where(torch.isnan(z), -math.inf, z), dim=1, descending=True, stable=True).indices[:, :5])
+    z[:, first:] = -math.inf
+    z[:, first + 100:] = math.nan
+    index = ops.class_logprobs(_dev(z), None, 5)[4].cpu()
+    assert torch.equal(index, first + torch.arange(5).expand(n, 5))

@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 8 : 6)) void k_logprob_walk(
                 least = lp_wave_max(x);
                 if (lane == __ffsll((unsigned long long)__ballot(x == least)) - 1) x = -INFINITY;
             }
-        } else if (!__any(mx > least)) continue;  // later classes rank behind equal ones
+        } else if (!__any(!(mx <= least))) continue; // later classes rank behind equal ones (before a list of NaN all do)
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const int64_t p = p0 + u * (64 * WPR) + tid;
