@@ -790,3 +790,19 @@ def test_class_logprobs_best_behind_nan(n, c, first):
     z[:, first + 100:] = math.nan
     index = ops.class_logprobs(_dev(z), None, 5)[4].cpu()
     assert torch.equal(index, first + torch.arange(5).expand(n, 5))
+
+
+@pytest.mark.gpu
+def test_roi_attention_empty_views():
+    """No rows or no keys, cut from tensors whose strides are no multiples of 16 bytes."""
+    from vision_amd import ops
+    x = torch.randn(3, 5, 2, 13, dtype=torch.float32, device="cuda")
+    full, none = x[..., 5:13], x[:, :0, :, 5:13]
+    out, lse = ops.roi_attention(full, none, none)
+    assert out.shape == full.shape and bool((out == 0).all()) and bool((lse == -math.inf).all())
+    dq, dk, dv = ops.roi_attention_backward(full, full, none, none, out, lse)
+    assert bool((dq == 0).all()) and dk.shape == dv.shape == none.shape
+    out, lse = ops.roi_attention(none, full, full)
+    assert out.shape == none.shape and lse.shape == (3, 2, 0)
+    dq, dk, dv = ops.roi_attention_backward(none, none, full, full, out, lse)
+    assert dq.shape == none.shape and bool((dk == 0).all()) and bool((dv == 0).all())

@@ -378,7 +378,7 @@ def _strides_fit(shape, strides, e):
 
 def _vec16(t):
     """t, or a copy of it, such that _strides_fit and its first value lies on a multiple of 16 bytes"""
-    if t.numel() == 0 or (t.data_ptr() % 16 == 0 and _strides_fit(t.shape, t.stride(), t.element_size())):
+    if t.data_ptr() % 16 == 0 and _strides_fit(t.shape, t.stride(), t.element_size()):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
