@@ -347,7 +347,7 @@ typedef struct dg_attn_shape {   /* host */
     int64_t batch, nq, nk, q_heads, k_heads, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3];   /* batch, row, head; g: of grad_out (backward) */
     int64_t masks, mask_stride[2];                                /* 0: no mask, 1: one for all images, batch: one each; batch, row */
-    float scale;                                                  /* positive, finite */
+    float scale;                                                  /* positive, at most 1e30 */
     int32_t dtype;
 } dg_attn_shape;
 size_t dg_roi_attn_workspace_bytes(const dg_attn_shape *shape, int backward);

@@ -792,6 +792,44 @@ def test_class_logprobs_best_behind_nan(n, c, first):
     assert torch.equal(index, first + torch.arange(5).expand(n, 5))
 
 
+def test_attention_refuses_what_no_launch_holds():
+    """On the host: a launch has fewer than 2^32 threads, and a scale times log2 e has to be a 32-bit number."""
+    from vision_amd import _abi
+    lib = _abi.load()
+    for kw, word in ((dict(scale=2.5e38), "scale"), (dict(batch=1 << 23), "too many tiles"), (dict(batch=1 << 20, nq=2000), "too many tiles"),
+                     (dict(batch=1 << 20, nk=2000), "too many tiles")):
+        s = _abi.AttnShape(2, 8, 8, 4, 2, 64)
+        s.scale, s.dtype = 0.125, _abi.BF16
+        for a, b in kw.items():
+            setattr(s, a, b)
+        assert lib.dg_roi_attn_workspace_bytes(s, 1) == 0 and word in _abi.last_error(), (kw, _abi.last_error())
+
+
+@pytest.mark.gpu
+def test_more_blocks_than_one_axis_of_a_launch_holds():
+    """2^32 threads and more: the tokens and rows behind them are computed as those before."""
+    from vision_amd import ops
+    n, d = (1 << 28) + 37, 2                     # 16 tokens a block
+    plan = ops.rope_plan((1,), device="cuda")
+    q = torch.empty(1, n, 1, d, dtype=torch.bfloat16, device="cuda")
+    q[..., 0], q[..., 1] = 1.0, -2.0
+    pos = torch.zeros(n, 1, device="cuda")
+    pos[:, 0] = torch.arange(n, device="cuda") % 1021
+    out = ops.rope_axes(q, pos, plan)
+    for a in (0, (1 << 28) - 50, n - 60):
+        assert torch.equal(out[:, a:a + 60], ops.rope_axes(q[:, a:a + 60], pos[a:a + 60], plan))
+    del q, pos, out
+    for c, top in ((300, 1), (600, 0)):          # 4 rows a block
+        n = (1 << 26) + 9
+        z = torch.randn(1, c, generator=_gen(62)).bfloat16().cuda()
+        one = ops.class_logprobs(z, torch.full((1,), 7, device="cuda"), top)
+        y = torch.full((n,), 7, dtype=torch.int64, device="cuda")
+        y[-1] = -1
+        many = ops.class_logprobs(z.expand(n, c), y, top)
+        assert bool((many[0][:-1] == one[0]).all()) and float(many[0][-1]) == 0.0
+        assert all(bool((a == b).all()) for a, b in zip(many[1:], one[1:]))
+
+
 @pytest.mark.gpu
 def test_roi_attention_empty_views():
     """No rows or no keys, cut from tensors whose strides are no multiples of 16 bytes."""

@@ -855,14 +855,15 @@ static int at_check(const dg_attn_shape *s, const char *who)
     DG_REQUIRE(s->batch >= 0 && s->nq >= 0 && s->nk >= 0, "%s: negative size", who);
     DG_REQUIRE(s->k_heads >= 1 && s->q_heads >= 1 && s->q_heads % s->k_heads == 0, "%s: q_heads must be a positive multiple of k_heads", who);
     DG_REQUIRE(s->d >= 8 && s->d <= 128 && s->d % 8 == 0, "%s: head size %lld is not a multiple of 8 from 8 to 128", who, (long long)s->d);
-    DG_REQUIRE(s->scale > 0.f && s->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
+    DG_REQUIRE(s->scale > 0.f && s->scale <= 1e30f, "%s: scale must be positive and at most 1e30", who);
     DG_REQUIRE(s->masks == 0 || s->masks == 1 || s->masks == s->batch, "%s: masks is 0, 1 (for all images) or the batch", who);
     const int64_t most = 1ll << 28;
     DG_REQUIRE(s->batch <= most && s->nk <= most && s->q_heads <= most && s->nq <= most && s->nq * (s->q_heads / s->k_heads) <= most &&
                    s->batch * s->q_heads <= most, "%s: more than 2^28 rows or keys", who);
     const at_plan p = at_plan_of(s);
-    DG_REQUIRE(s->batch * s->k_heads * p.qtiles * p.qsplits < (1ll << 31) && s->batch * s->k_heads * p.ktiles * p.ksplits < (1ll << 31) &&
-                   dg_cdiv(p.rows, 4) < (1ll << 31) && dg_cdiv(s->masks * s->nq * p.words, AT_THREADS) < (1ll << 31), "%s: more than 2^31 tiles", who);
+    const int64_t blocks = (1ll << 32) / AT_THREADS;         // a launch holds fewer than 2^32 threads
+    DG_REQUIRE(s->batch * s->k_heads * p.qtiles * p.qsplits < blocks && s->batch * s->k_heads * p.ktiles * p.ksplits < blocks &&
+                   dg_cdiv(p.rows, 8) < blocks && dg_cdiv(s->masks * s->nq * p.words, AT_THREADS) < blocks, "%s: too many tiles for one launch", who);
     return DG_OK;
 }
 

@@ -23,6 +23,14 @@ void dg_set_error(const char *fmt, ...);
         if (e_ != hipSuccess) { dg_set_error("%s: launch failed: %s", name, hipGetErrorString(e_)); return DG_EHIP; } \
     } while (0)
 
+// blocks that may number more than a launch's 2^32 threads in x allow: in two dimensions; a kernel counts with dg_block()
+static inline dim3 dg_grid(int64_t blocks)
+{
+    const int64_t x = 1ll << 22;
+    return blocks <= x ? dim3((unsigned)blocks) : dim3((unsigned)x, (unsigned)((blocks + x - 1) / x));
+}
+__device__ __forceinline__ u32 dg_block() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 // communicator handle of include/detgeom.h (comm.hip owns it; kmeans.hip keeps the captured chunk of its sharded loop here)
 struct dg_comm {
     void *comm = nullptr;            // ncclComm_t

@@ -148,7 +148,7 @@ template <typename T, int L>
 __global__ __launch_bounds__(256) void k_logprob_small(const lp_args a)
 {
     const int sub = threadIdx.x & (L - 1);
-    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const int64_t row = (int64_t)dg_block() * (256 / L) + threadIdx.x / L;
     if (row >= a.n) return;                       // whole groups: shuffles stay among the lanes of a row
     const T *z = (const T *)a.z + row * a.stride;
     float v[8];
@@ -218,7 +218,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 8 : 6)) void k_logprob_walk(
     __shared__ float sums[4][3];
     __shared__ u64 lists[4][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tid = WPR == 4 ? threadIdx.x : lane;
-    const int64_t part = WPR == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int64_t part = WPR == 4 ? dg_block() : (int64_t)dg_block() * 4 + wave;
     const int64_t row = part / a.splits, sp = part - row * a.splits;
     if (row >= a.n) return;                       // WPR == 1: whole waves, and no barrier follows
     const int keep = a.top;
@@ -349,7 +349,7 @@ __global__ __launch_bounds__(256) void k_logprob_bwd(const T *__restrict__ z, co
                                                      const float *__restrict__ gh, T *__restrict__ dz)
 {
     typedef T vec __attribute__((ext_vector_type(VEC)));
-    const int64_t end = n * c, first = ((int64_t)blockIdx.x * (256 * UN) + threadIdx.x) * VEC;
+    const int64_t end = n * c, first = ((int64_t)dg_block() * (256 * UN) + threadIdx.x) * VEC;
     vec x[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
@@ -426,7 +426,7 @@ extern "C" size_t dg_class_logprobs_workspace_bytes(int64_t n, int64_t c, int64_
 template <typename T> static void lp_forward(lp_args &a, hipStream_t st)
 {
     if (a.c <= 512) {
-#define LP_SMALL(L) hipLaunchKernelGGL((k_logprob_small<T, L>), dim3((unsigned)dg_cdiv(a.n, 256 / L)), dim3(256), 0, st, a)
+#define LP_SMALL(L) hipLaunchKernelGGL((k_logprob_small<T, L>), dg_grid(dg_cdiv(a.n, 256 / L)), dim3(256), 0, st, a)
         if (a.c <= 32) LP_SMALL(4);
         else if (a.c <= 64) LP_SMALL(8);
         else if (a.c <= 128) LP_SMALL(16);
@@ -435,7 +435,7 @@ template <typename T> static void lp_forward(lp_args &a, hipStream_t st)
         return;
     }
     // a wave a row where rows alone give every SIMD four waves, or where a row is short; four waves a row elsewhere
-    if (a.splits == 1 && (a.c <= 4096 || a.n >= 4096)) hipLaunchKernelGGL((k_logprob_walk<T, 1>), dim3((unsigned)dg_cdiv(a.n, 4)), dim3(256), 0, st, a);
+    if (a.splits == 1 && (a.c <= 4096 || a.n >= 4096)) hipLaunchKernelGGL((k_logprob_walk<T, 1>), dg_grid(dg_cdiv(a.n, 4)), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((k_logprob_walk<T, 4>), dim3((unsigned)(a.n * a.splits)), dim3(256), 0, st, a);
     if (a.splits > 1) hipLaunchKernelGGL((k_logprob_join<T>), dim3((unsigned)a.n), dim3(64), 0, st, a);
 }
@@ -476,7 +476,7 @@ static int lp_backward(const void *z, const int64_t *y, int64_t n, int64_t c, in
     const bool many = wide && n * c >= (1ll << 24);
     const int64_t blocks = dg_cdiv(n * c, 256 * (many ? 4 * V : wide ? V : 1));
     DG_REQUIRE(blocks < (1ll << 31), "class_logprobs_bwd: too large");
-#define LP_BWD(VEC, DENSE, UN) hipLaunchKernelGGL((k_logprob_bwd<T, VEC, DENSE, UN>), dim3((unsigned)blocks), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz)
+#define LP_BWD(VEC, DENSE, UN) hipLaunchKernelGGL((k_logprob_bwd<T, VEC, DENSE, UN>), dg_grid(blocks), dim3(256), 0, st, (const T *)z, y, n, c, stride, norm, entropy, g, gh, (T *)dz)
     if (many && dense) LP_BWD(V, true, 4);
     else if (many) LP_BWD(V, false, 4);
     else if (wide && dense) LP_BWD(V, true, 1);

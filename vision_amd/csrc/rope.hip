@@ -30,7 +30,9 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
 {
     typedef rp_piece<T, VEC> piece;
     extern __shared__ float2 cs[];                // [tok][pairs]
-    const u32 t0 = blockIdx.x * (u32)a.tok, nt = min((u32)a.tok, a.tokens - t0);       // tokens number fewer than 2^31
+    const u32 t0 = dg_block() * a.tok;            // tokens number fewer than 2^31
+    if (t0 >= a.tokens) return;
+    const u32 nt = min(a.tok, a.tokens - t0);
     for (u32 i = threadIdx.x; i < nt * a.pairs; i += 256) {
         const u32 t = i / a.pairs, j = i - t * a.pairs, b = (t0 + t) / a.n, n = t0 + t - b * a.n;
         const int ax = min(max(a.axis[j], 0), a.axes - 1);
@@ -97,7 +99,7 @@ static void rp_launch(const rp_args &a0, bool halves, hipStream_t st)
     }
     a.tok = 1;
     while (a.tok < 16 && a.tok * a.pairs < 256) a.tok *= 2;
-    const dim3 grid((unsigned)dg_cdiv(a.tokens, a.tok)), block(256);
+    const dim3 grid = dg_grid(dg_cdiv(a.tokens, a.tok)), block(256);
     const size_t lds = (size_t)a.tok * a.pairs * sizeof(float2);
     const u32 rest = a.d - 2 * a.pairs;
     if (halves) {
