@@ -794,24 +794,28 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict
     *(quad *)((blockIdx.y ? out2 : out) + (((int64_t)b * nmax + n) * heads + hh) * d + x) = __builtin_convertvector(v, quad);
 }
 
-// pair mask -> bits, once for all heads and passes over it: a word of 32 keys per thread (4 x 509 x 509: the bytes read by every lane
-// for itself cost the three kernels 47, 53 and 71 us, the bits 38, 44 and 59, and 6 to make them)
-__global__ __launch_bounds__(AT_THREADS) void k_attn_bits(const uint8_t *__restrict__ mask, int64_t sb, int64_t sr, u32 *__restrict__ bits, int64_t n, int nq, int nk, int words)
+// pair mask -> bits, once for all heads and passes over it (4 x 509 x 509: the bytes read by every lane for itself cost the three
+// kernels 47, 53 and 71 us, the bits 38, 44 and 59; 4 to make them).  A workgroup has 1024 keys of a row, a wave 256: a byte a lane, a ballot for 64.
+__global__ __launch_bounds__(AT_THREADS) void k_attn_bits(const uint8_t *__restrict__ mask, int64_t sb, int64_t sr, u32 *__restrict__ bits, u32 blocks, int nq, int nk, int words)
 {
-    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x;
-    if (i >= n) return;
-    const int w = (int)(i % words), k0 = w * 32;
-    const int64_t r = i / words;
-    const uint8_t *m = mask + r / nq * sb + r % nq * sr + k0;
-    u32 x = 0;
-    if (nk - k0 >= 32) {
-        uint8_t v[32];
-        __builtin_memcpy(v, m, 32);
+    const u32 id = dg_block(), cuts = (nk + 1023) / 1024, r = id / cuts;
+    if (id >= blocks) return;
+    const int lane = threadIdx.x & 63, k0 = (int)(id - r * cuts) * 1024 + (int)(threadIdx.x >> 6) * 256;
+    const uint8_t *m = mask + (int64_t)(r / nq) * sb + (int64_t)(r % nq) * sr;
+    uint8_t v[4];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x |= v[j] ? 1u << j : 0u;
-    } else
-        for (int j = 0; j < nk - k0; ++j) x |= m[j] ? 1u << j : 0u;
-    bits[i] = x;
+    for (int j = 0; j < 4; ++j) {
+        const int k = k0 + 64 * j + lane;
+        v[j] = k < nk ? m[k] : 0;
+    }
+    u32 x = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const u64 w = __ballot(v[j] != 0);
+        if (lane >> 1 == j) x = (u32)(w >> (32 * (lane & 1)));
+    }
+    const int w = (k0 >> 5) + lane;
+    if (lane < 8 && w < words) bits[(int64_t)r * words + w] = x;
 }
 
 // ------------------------------------------------------------------ host
@@ -863,7 +867,7 @@ static int at_check(const dg_attn_shape *s, const char *who)
     const at_plan p = at_plan_of(s);
     const int64_t blocks = (1ll << 32) / AT_THREADS;         // a launch holds fewer than 2^32 threads
     DG_REQUIRE(s->batch * s->k_heads * p.qtiles * p.qsplits < blocks && s->batch * s->k_heads * p.ktiles * p.ksplits < blocks &&
-                   dg_cdiv(p.rows, 8) < blocks && dg_cdiv(s->masks * s->nq * p.words, AT_THREADS) < blocks, "%s: too many tiles for one launch", who);
+                   dg_cdiv(p.rows, 8) < blocks && s->masks * s->nq * dg_cdiv(s->nk, 1024) < (1ll << 31), "%s: too many tiles for one launch", who);
     return DG_OK;
 }
 
@@ -904,9 +908,9 @@ static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, 
 template <typename T> static void *at_bits(const dg_attn_shape *s, const at_plan &p, const uint8_t *mask, at_args<T> &a, void *ws, hipStream_t st)
 {
     if (!p.bits) return ws;
-    const int64_t n = s->masks * s->nq * p.words;
-    hipLaunchKernelGGL(k_attn_bits, dim3((unsigned)dg_cdiv(n, AT_THREADS)), dim3(AT_THREADS), 0, st, mask, s->mask_stride[0], s->mask_stride[1], (u32 *)ws, n, (int)s->nq,
-                       (int)s->nk, (int)p.words);
+    const int64_t n = s->masks * s->nq * dg_cdiv(s->nk, 1024);
+    hipLaunchKernelGGL(k_attn_bits, dg_grid(n), dim3(AT_THREADS), 0, st, mask, s->mask_stride[0], s->mask_stride[1], (u32 *)ws, (u32)n, (int)s->nq, (int)s->nk,
+                       (int)p.words);
     a.bits = (const u32 *)ws;
     a.words = (int)p.words;
     a.bs = s->masks > 1 ? s->nq * p.words : 0;
