@@ -332,8 +332,8 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
 /* ---------------------------------------------------------------- the RoI head: attention over an image's boxes or cells
  * NO COUNTERPART IN THE REFERENCE (its Fast R-CNN sketch classifies every RoI by itself, rcnn/fast_rcnn.py:379-384).
  * q (batch, nq, q_heads, d), k and v (batch, nk, k_heads, d): strides of the first three axes in values, the last axis dense;
- * pointers and strides multiples of 16 bytes, rows at most 2^22 values apart.  Query head h reads key head h / (q_heads / k_heads).  Types: DG_F32, DG_BF16 (one
- * for all of q, k, v, out and the gradients).  d: a multiple of 8 from 8 to 128.
+ * pointers and strides multiples of 16 bytes, rows at most 2^22 values apart.  Query head h reads key head
+ * h / (q_heads / k_heads).  Types: DG_F32, DG_BF16 (one for all of q, k, v, out and the gradients).  d: a multiple of 8 from 8 to 128.
  *   s_ij = scale * q_i . k_j,  p_i = softmax over the keys that row i may see,  out_i = sum_j p_ij v_j,  lse_i = log sum_j exp s_ij
  * A row i sees key j if i < q_counts[image], j < k_counts[image] (device int32, held to [0, n]; NULL = all) and mask[image][i][j] != 0
  * (device bytes, a row's keys dense, strides of image and row in bytes; shape->masks of them, NULL with 0 = all).  What lies behind a count is
@@ -341,8 +341,9 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * behind k_counts: every element of every output is written.  A pair that a count or a mask excludes adds nothing, whatever its values
  * are.  A NaN or an infinity in what a row does see makes that row's results NaN or infinite, and with a mask NaN.
  * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
- * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products.  Results are the
- * same in every run (no atomics). */
+ * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products, in DG_F32 products
+ * are formed from three bf16 parts of each operand, which keeps their 24 bits; a DG_F32 value of 3.39e38 or more counts as infinite.
+ * Results are the same in every run (no atomics). */
 typedef struct dg_attn_shape {   /* host */
     int64_t batch, nq, nk, q_heads, k_heads, d;
     int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3];   /* batch, row, head; g: of grad_out (backward) */

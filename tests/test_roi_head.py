@@ -844,3 +844,43 @@ def test_roi_attention_empty_views():
     assert out.shape == none.shape and lse.shape == (3, 2, 0)
     dq, dk, dv = ops.roi_attention_backward(none, none, full, full, out, lse)
     assert dq.shape == none.shape and bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_roi_attention_largest_values_behind_mask(dtype, D):
+    """Keys and rows that a mask hides from all, filled with a type's largest and lowest value: as if they held zeros."""
+    from vision_amd import ops
+    B, N, M, H = 2, 70, 90, 2
+    q, k, v, do = _attn_inputs(71, B, N, M, H, H, D, dtype)
+    mask = torch.rand((B, N, M), generator=_gen(72)) < 0.5
+    keys, rows = [0, 17, 63, 89], [5, 31, 69]
+    mask[:, :, keys] = False
+    mask[:, rows] = False
+    got = []
+    for fill in ((0.0, 0.0), (torch.finfo(dtype).max, torch.finfo(dtype).min)):
+        Q, K, V, G = q.clone(), k.clone(), v.clone(), do.clone()
+        K[:, keys, 0], K[:, keys, 1], V[:, keys, 0], V[:, keys, 1] = fill[0], fill[1], fill[1], fill[0]
+        Q[:, rows, 0], Q[:, rows, 1], G[:, rows, 0], G[:, rows, 1] = fill[0], fill[1], fill[1], fill[0]
+        Q, K, V, G, m = map(_dev, (Q, K, V, G, mask))
+        out, lse = ops.roi_attention(Q, K, V, mask=m)
+        got.append((out, lse, *ops.roi_attention_backward(G, Q, K, V, out, lse, mask=m)))
+    for name, a, b in zip(("out", "lse", "dq", "dk", "dv"), *got):
+        assert torch.equal(a, b), name
+
+
+@pytest.mark.gpu
+def test_roi_attention_keeps_the_bits_of_float32():
+    """Values that differ in their last bits only: products of 32-bit operands in three parts keep them.  v is 1 + j 2^-20 for key j and
+    one key is seen by each row, so that out is that v exactly; with two keys of equal score it is their mean, rounded once or twice."""
+    from vision_amd import ops
+    n, d = 96, 64
+    q = torch.zeros(1, n, 1, d, device="cuda")
+    v = (1.0 + torch.arange(n, dtype=torch.float32)[:, None] * 2.0 ** -20 + torch.arange(d) * 2.0 ** -23).view(1, n, 1, d).cuda()
+    eye = torch.eye(n, dtype=torch.bool, device="cuda")
+    out, _ = ops.roi_attention(q, q, v, mask=eye)
+    assert torch.equal(out, v)
+    out, _ = ops.roi_attention(q, q, v, mask=eye | eye.roll(1, 1))
+    want = (v.double() + v.double().roll(-1, 1)) / 2
+    assert float((out.double() - want).abs().max()) <= 2.0 ** -23

@@ -17,6 +17,7 @@
 #include "common.hpp"
 #include <math.h>
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -35,13 +36,56 @@ template <typename T> struct at_vec;
 template <> struct at_vec<__bf16> { typedef bf16x8 frag; typedef bf16x4 quad; };
 template <> struct at_vec<float> { typedef f32x4 frag; typedef f32x4 quad; };
 
-// a block of contraction values: 16 bytes per lane of each operand, lanes 0..31 the first chunk, lanes 32..63 the second
-__device__ __forceinline__ f32x16 at_mma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 at_mma(f32x4 a, f32x4 b, f32x16 c)
+// Operands of the matrix cores: eight contraction values of a lane, lanes 0..31 the first eight of a block of sixteen, lanes
+// 32..63 the second.  A value of 32 bits goes in as three of 16: x = h + m + l, each the rounding of what the ones before left, which is
+// exact but for numbers that end below 2^-126.  Of the nine products the six from 2^-16 up are formed; what is left out is less than 2^-25 of
+// |x y|, half a rounding in 32 bits.  Six instructions of 32 cycles for sixteen contraction values; the 32-bit matrix instruction
+// would take 512 cycles for them.
+template <typename T> struct at_parts { static constexpr int N = sizeof(T) == 4 ? 3 : 1; };
+template <typename T> struct at_op { bf16x8 p[at_parts<T>::N]; };
+__device__ __forceinline__ f32x16 at_mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 at_mma(const at_op<__bf16> &a, const at_op<__bf16> &b, f32x16 c) { return at_mfma(a.p[0], b.p[0], c); }
+__device__ __forceinline__ f32x16 at_mma(const at_op<float> &a, const at_op<float> &b, f32x16 c)
+{
+    c = at_mfma(a.p[2], b.p[0], c);
+    c = at_mfma(a.p[0], b.p[2], c);
+    c = at_mfma(a.p[1], b.p[1], c);
+    c = at_mfma(a.p[1], b.p[0], c);
+    c = at_mfma(a.p[0], b.p[1], c);
+    return at_mfma(a.p[0], b.p[0], c);
+}
+__device__ __forceinline__ void at_cut(f32x8 x, at_op<__bf16> &o) { o.p[0] = __builtin_convertvector(x, bf16x8); }
+// x - h for the two values of a pair: a dot product of two terms with (-1, 0) or (0, -1), exact (as is the difference of the two numbers),
+// one instruction where a conversion back and a difference are two.  (-1, 0) comes from a register: as a constant of the
+// instruction, which is of 32 bits, -1 would stand in the other half.
+__device__ __forceinline__ void at_less(bf16x2 h, float &x, float &y)
+{
+    u32 c;
+    asm("s_mov_b32 %0, 0xbf80" : "=s"(c));
+    x = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, c), x, false);
+    y = __builtin_amdgcn_fdot2_f32_bf16(h, (bf16x2){(__bf16)0.f, (__bf16)-1.f}, y, false);
+}
+__device__ __forceinline__ void at_cut(f32x8 x, at_op<float> &o)
 {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-    return c;
+    for (int i = 0; i < 3; ++i) {
+        const bf16x8 h = __builtin_convertvector(x, bf16x8);
+        o.p[i] = h;
+#pragma unroll
+        for (int e = 0; e < 8 && i < 2; e += 2) {
+            float a = x[e], b = x[e + 1];
+            at_less((bf16x2){h[e], h[e + 1]}, a, b);
+            x[e] = a;
+            x[e + 1] = b;
+        }
+    }
+}
+// eight values of a row in memory
+__device__ __forceinline__ void at_read(const __bf16 *p, bool in, at_op<__bf16> &o) { o.p[0] = in ? *(const bf16x8 *)p : (bf16x8)(0.f); }
+__device__ __forceinline__ void at_read(const float *p, bool in, at_op<float> &o)
+{
+    const f32x4 a = in ? *(const f32x4 *)p : (f32x4)(0.f), b = in ? *(const f32x4 *)(p + 4) : (f32x4)(0.f);
+    at_cut(__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7), o);
 }
 // the value of this lane and of the one 32 away, in either order
 __device__ __forceinline__ void at_both(float v, float &x, float &y)
@@ -52,57 +96,63 @@ __device__ __forceinline__ void at_both(float v, float &x, float &y)
     y = __uint_as_float(r[1]);
 }
 
-// A tile of rows in LDS, DP values wide, in 16-byte chunks whose place inside the row is swizzled by the row.  LDS gives 256 bytes
-// a clock to reads; sixteen lanes that read the same chunk of sixteen successive rows, and thirty-two that read four chunks of four
-// successive rows (the transposing read), both cover all 256 bytes modulo 256.  Measured on 16001 rows x 128: a swizzle for 128
-// bytes a clock spent 40% of the LDS's active cycles on conflicts.
-template <typename T, int DP> struct at_tile {
-    static constexpr int RB = DP * (int)sizeof(T), CPR = RB / 16;
+// A tile of ROWS rows in LDS, DP values wide, a plane of bf16 for each part, in 16-byte chunks whose place inside the row is
+// swizzled by the row.  LDS gives 256 bytes a clock to reads; sixteen lanes that read the same chunk of sixteen successive rows, and
+// thirty-two that read four chunks of four successive rows (the transposing read), both cover all 256 bytes modulo 256.  Measured on
+// 16001 rows x 128: a swizzle for 128 bytes a clock spent 40% of the LDS's active cycles on conflicts.
+template <typename T, int DP, int ROWS> struct at_tile {
+    static constexpr int RB = DP * 2, CPR = RB / 16, N = at_parts<T>::N, PLANE = ROWS * RB, BYTES = N * PLANE;
     static __device__ __forceinline__ int swz(int row)
     {
         return CPR >= 16 ? ((row & 3) << 2) | ((row >> 2) & 3) : CPR == 8 ? ((row & 2) << 1) | ((row >> 2) & 3) : (row >> 2) & 3;
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * RB + ((chunk ^ swz(row)) << 4); }
     // rows of the tile as an operand: row l & 31, chunk 2 g + l / 32
-    static __device__ __forceinline__ typename at_vec<T>::frag row_frag(const char *t, int row, int chunk)
+    static __device__ __forceinline__ at_op<T> row(const char *t, int row, int chunk)
     {
-        return *(const typename at_vec<T>::frag *)(t + at(row, chunk));
+        at_op<T> o;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o.p[i] = *(const bf16x8 *)(t + i * PLANE + at(row, chunk));
+        return o;
+    }
+    // 16 bytes of a row in memory
+    static __device__ __forceinline__ void put(char *t, int row, int c16, u32x4 x)
+    {
+        if (N == 1) { *(u32x4 *)(t + at(row, c16)) = x; return; }
+        f32x4 v = __builtin_bit_cast(f32x4, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bf16x4 h = __builtin_convertvector(v, bf16x4);
+            *(bf16x4 *)(t + i * PLANE + at(row, c16 >> 1) + (c16 & 1) * 8) = h;
+            float a = v[0], b = v[1], c = v[2], d = v[3];
+            at_less((bf16x2){h[0], h[1]}, a, b);
+            at_less((bf16x2){h[2], h[3]}, c, d);
+            v = (f32x4){a, b, c, d};
+        }
+    }
+    // acc[db] (32 values of d x 32 columns) += tile[rows base..base+31][d]^T * w, w in the result layout (rows = the tile's rows)
+    static __device__ __forceinline__ void acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane)
+    {
+        const int h = lane >> 5, j = lane & 15, row0 = base + 4 * h + (j >> 2), part = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            at_op<T> b;                           // bf16: one rounding to 8 bits; the sum stays in 32
+            at_cut(s ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7), b);
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db) {
+                typedef __attribute__((address_space(3))) s16x4 *lp;
+                at_op<T> a;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + i * PLANE + at(row0 + 16 * s, db * 4 + part) + (j & 1) * 8));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + i * PLANE + at(row0 + 16 * s + 8, db * 4 + part) + (j & 1) * 8));
+                    a.p[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                acc[db] = at_mma(a, b, acc[db]);
+            }
+        }
     }
 };
-
-// acc[db] (32 values of d x 32 columns) += tile[rows base..base+31][d]^T * w, w in the result layout (rows = the tile's rows)
-template <int DP> __device__ __forceinline__ void at_acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane, const __bf16 *)
-{
-    typedef at_tile<__bf16, DP> tile;
-    const int h = lane >> 5, j = lane & 15, row0 = base + 4 * h + (j >> 2), part = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1);
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        const f32x8 ws = s ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
-        const bf16x8 b = __builtin_convertvector(ws, bf16x8);       // one rounding to 8 bits; the sum stays in 32
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-            typedef __attribute__((address_space(3))) s16x4 *lp;
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + tile::at(row0 + 16 * s, db * 4 + part) + (j & 1) * 8));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + tile::at(row0 + 16 * s + 8, db * 4 + part) + (j & 1) * 8));
-            const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-            acc[db] = at_mma(a, b, acc[db]);
-        }
-    }
-}
-template <int DP> __device__ __forceinline__ void at_acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane, const float *)
-{
-    typedef at_tile<float, DP> tile;
-    const int h = lane >> 5, d = lane & 31;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int row = base + 8 * (r >> 2) + 4 * h + (r & 3);
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-            const float a = *(const float *)(t + tile::at(row, db * 8 + (d >> 2)) + (d & 3) * 4);
-            acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w[r], acc[db], 0, 0, 0);
-        }
-    }
-}
 
 // what a call is made of, on the device's side
 template <typename T> struct at_args {
@@ -158,14 +208,14 @@ __device__ __forceinline__ u32 at_word(const u32 *row, int kb, int k1)
 
 template <typename T> __device__ __forceinline__ u32x4 at_load_chunk(const T *p) { return *(const u32x4 *)p; }
 
-// A workgroup's loader of row tiles: thread t takes chunk t % CPR of rows t / CPR, + STEP, ...  Buffer loads: the tile's address is
+// A workgroup's loader of row tiles: thread t takes 16 bytes, t % CPR, of rows t / CPR, + STEP, ...  Buffer loads: the tile's address is
 // uniform, a lane's offset inside it fixed, and a lane with nothing to load (a row behind the end, a chunk behind d) asks for an
 // offset out of range and gets zeros.  A tile spans less than 2^31 bytes (at_aligned).
 #define AT_OUT 0x7fffffff
 #define AT_VM0 0x0f70                             // s_waitcnt vmcnt(0), the other counters free
 template <typename T, int DP, int ROWS, bool LEAN = false> struct at_loader {
-    typedef at_tile<T, DP> tile;
-    static constexpr int STEP = AT_THREADS / tile::CPR, NL = ROWS / STEP > 0 ? ROWS / STEP : 1;
+    typedef at_tile<T, DP, ROWS> tile;
+    static constexpr int CPR = DP * (int)sizeof(T) / 16, STEP = AT_THREADS / CPR, NL = ROWS / STEP > 0 ? ROWS / STEP : 1;
     const T *base;
     int64_t stride;
     int bytes, row0_, c16_, off_;                 // bytes: of a row; off: of the first row's chunk
@@ -175,8 +225,8 @@ template <typename T, int DP, int ROWS, bool LEAN = false> struct at_loader {
     }
     __device__ __forceinline__ void place(int t, int &row0, int &c16, int &off) const
     {
-        row0 = t / tile::CPR;
-        c16 = t % tile::CPR;
+        row0 = t / CPR;
+        c16 = t % CPR;
         off = c16 * 16 < bytes ? row0 * (int)(stride * (int)sizeof(T)) + c16 * 16 : AT_OUT;
     }
     // LEAN: a thread's place is formed anew in every turn, where keeping it would cost registers that are not there
@@ -205,12 +255,13 @@ template <typename T, int DP, int ROWS, bool LEAN = false> struct at_loader {
         place(row0, c16, off);
 #pragma unroll
         for (int i = 0; i < NL; ++i)
-            if (ROWS >= STEP || row0 < ROWS) *(u32x4 *)(lds + tile::at(row0 + i * STEP, c16)) = r[i];
+            if (ROWS >= STEP || row0 < ROWS) tile::put(lds, row0 + i * STEP, c16, r[i]);
     }
 };
 
 // with a pair mask, a row of K, V, Q or dO that some rows may not see must not reach them through 0 * NaN: non-finite values
-// are put to zero in the staged copy, and the caller marks the row so that those who do see it get NaN
+// are put to zero in the staged copy, and the caller marks the row so that those who do see it get NaN.  Values of 32 bits that round to
+// infinity as their first part count with them
 template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 {
     bool bad = false;
@@ -222,7 +273,7 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
             if (hi) x[i] &= 0x0000ffffu;
             bad |= lo | hi;
         } else {
-            const bool b = (x[i] & 0x7f800000u) == 0x7f800000u;
+            const bool b = (x[i] & 0x7fffffffu) >= 0x7f7f8000u;
             if (b) x[i] = 0;
             bad |= b;
         }
@@ -234,8 +285,10 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 // ------------------------------------------------------------------ forward
 // The wave that has scores to multiply goes first, then one that has values to, then the vector work: with equal priorities the two
 // waves of a SIMD drift into the same phase and the matrix unit waits (16000 x 128: forward 1101 -> 1040 us, dq 1575 -> 1511, dk, dv
-// 2253 -> 2140).  Up to 64, where three or four waves share a SIMD, it only keeps the scheduler from mixing the phases (dk, dv 101 -> 126).
-#define AT_PRIO(p) do { if (DP == 128) __builtin_amdgcn_s_setprio(p); } while (0)
+// 2253 -> 2140).  In bf16 up to 64, where three
+// or four waves share a SIMD, it only keeps the scheduler from mixing the phases (dk, dv 101 -> 126); in fp32, whose products are six times as
+// many, it helps there too (8 x 2000 x 64: forward 375 -> 353, dk, dv 668 -> 643).
+#define AT_PRIO(p) do { if (DP == 128 || sizeof(T) == 4) __builtin_amdgcn_s_setprio(p); } while (0)
 
 // Never taken (d is 8 at least): it parts a turn of the loop between the products and the exponentials.  In one piece the scheduler
 // keeps so many operands of later products in registers that others are spilled (16001 x 128: dk, dv 2545 -> 2220 us, dq 1650 -> 1530).
@@ -248,22 +301,22 @@ template <typename T> __device__ __forceinline__ bool at_scrub(u32x4 &x)
 template <typename T, int DP> struct at_shape {
     static constexpr int BYTES = sizeof(T) * DP, H = sizeof(T) == 2;
     static constexpr int KT = H && DP == 128 ? 64 : 32, KT_Q = 32;
-    static constexpr int OCC = BYTES > 256 ? 1 : H && DP <= 64 ? 4 : 2, OCC_Q = BYTES > 256 ? 1 : H && DP <= 64 ? 3 : 2, OCC_KV = H ? DP <= 64 ? 3 : 2 : BYTES > 128 ? 1 : 2;
+    static constexpr int OCC = BYTES > 256 ? 1 : H && DP <= 64 ? 4 : 2, OCC_Q = BYTES > 256 ? 1 : H && DP <= 64 ? 3 : 2, OCC_KV = H ? DP <= 64 ? 3 : 2 : BYTES > 256 ? 1 : 2;
 };
 
 // A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of KT.  K and V tiles are double buffered
 // in LDS; the next tile's loads are on their way while this one is computed.  Per 32 x 32 scores a wave spends 8 d / 64 matrix
 // instructions of 32 cycles and about 110 vector instructions (scale, exponential, sum, maximum, rounding): the vector unit bounds
 // 64 values a head, both units together 128.  Measured, bf16: 16 x 2000 rows and keys, 8 heads of 64: 170 us, 771 TFLOP/s; 16000, 8
-// heads of 128: 1040 us, 1008 TFLOP/s (a large matrix product reaches 1195); fp32, 8 x 2000, 8 heads of 64: 590 us, 111 TFLOP/s (153).
+// heads of 128: 1040 us, 1008 TFLOP/s (a large matrix product reaches 1195); fp32, 8 x 2000, 8 heads of 64: 355 us,
+// 185 TFLOP/s (a library's matrix product of 32 bits: 153; by 32-bit matrix instructions it took 590).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd(const at_args<T> a)
 {
-    typedef at_tile<T, DP> tile;
-    typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT, U = KT / 32, TB = KT * tile::RB;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+    constexpr int NG = DP / 16, NB = DP / 32, KT = at_shape<T, DP>::KT, U = KT / 32;
+    typedef at_tile<T, DP, KT> tile;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][tile::BYTES];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = at_image(bh / a.hk, a.batch, a.kc, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
@@ -285,11 +338,11 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
     const bool live = r < R;
     const int gh = live ? r / nq : 0, n = live ? r % nq : 0, hq = hk * G + gh;
     const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2];
-    frag qf[NG];
+    at_op<T> qf[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        const int d = (2 * g + h) * CH;
-        qf[g] = (live && d < a.d) ? *(const frag *)(qp + d) : (frag)(0.f);
+        const int d = (2 * g + h) * 8;
+        at_read(qp + d, live && d < a.d, qf[g]);
     }
     const u32 *mp = MASK ? a.bits + b * a.bs + (int64_t)n * a.words : nullptr;
 
@@ -337,7 +390,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         for (int u = 0; u < U; ++u) {
             s[u] = (f32x16)(0.f);
 #pragma unroll
-            for (int g = 0; g < NG; ++g) s[u] = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s[u]);
+            for (int g = 0; g < NG; ++g) s[u] = at_mma(tile::row(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s[u]);
         }
         AT_PRIO(0);
         if (MASK || !more) {
@@ -373,7 +426,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
                 l += p;
             }
             AT_PRIO(1);
-            at_acc_t<DP>(o, V, u * 32, s[u], lane, (const T *)nullptr);
+            tile::acc_t(o, V, u * 32, s[u], lane);
             AT_PRIO(0);
         }
         if (more) store(buf ^ 1);
@@ -506,15 +559,14 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
 
 // dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp).
 // Three products a tile.  Measured, bf16: 16 x 2000, 8 heads of 64: 247 us, 796 TFLOP/s; 16000, 8 heads of 128: 1511 us, 1041 TFLOP/s;
-// fp32, 8 x 2000, 8 heads of 64: 810 us, 121 TFLOP/s.
+// fp32, 8 x 2000, 8 heads of 64: 480 us, 205 TFLOP/s (by 32-bit matrix instructions 810).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_dq(const at_args<T> a)
 {
-    typedef at_tile<T, DP> tile;
-    typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = at_shape<T, DP>::KT_Q, U = KT / 32, TB = KT * tile::RB;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+    constexpr int NG = DP / 16, NB = DP / 32, KT = at_shape<T, DP>::KT_Q, U = KT / 32;
+    typedef at_tile<T, DP, KT> tile;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][tile::BYTES];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = at_image(bh / a.hk, a.batch, a.kc, a.nk), hk = bh % a.hk, G = a.hq / a.hk;
@@ -534,13 +586,12 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
     const bool live = r < R;
     const int gh = live ? r / nq : 0, n = live ? r % nq : 0, hq = hk * G + gh;
     const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2], *gp = a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2];
-    frag qf[NG], gf[NG];
+    at_op<T> qf[NG], gf[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        const int d = (2 * g + h) * CH;
-        const bool in = live && d < a.d;
-        qf[g] = in ? *(const frag *)(qp + d) : (frag)(0.f);
-        gf[g] = in ? *(const frag *)(gp + d) : (frag)(0.f);
+        const int d = (2 * g + h) * 8;
+        at_read(qp + d, live && d < a.d, qf[g]);
+        at_read(gp + d, live && d < a.d, gf[g]);
     }
     const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
     const f32x2 stat = live ? a.stat[at] : (f32x2){INFINITY, 0.f};
@@ -589,8 +640,8 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
             AT_PRIO(2);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                s = at_mma(tile::row_frag(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
-                dp = at_mma(tile::row_frag(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
+                s = at_mma(tile::row(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
+                dp = at_mma(tile::row(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
             }
             AT_PRIO(0);
             const int left = k1 - kb - u * 32;
@@ -603,7 +654,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
                 s[e] = ds;
             }
             AT_PRIO(1);
-            at_acc_t<DP>(o, K, u * 32, s, lane, (const T *)nullptr);
+            tile::acc_t(o, K, u * 32, s, lane);
             AT_PRIO(0);
         }
         if (more) store(buf ^ 1);
@@ -630,15 +681,14 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
 // dk, dv: a workgroup owns 128 keys (a wave: 32, one per lane pair) and walks the rows; Q and dO tiles are read as rows (scores,
 // dp) and transposed (dk, dv).  Four products a tile, and 2 x 32 x d accumulators a wave, which bound how many waves share a SIMD.
 // Measured, bf16: 16 x 2000, 8 heads of 64: 408 us, 642 TFLOP/s; 16000, 8 heads of 128: 2140 us, 980 TFLOP/s; fp32, 8 x 2000, 8 heads of
-// 64: 1084 us, 121 TFLOP/s.
+// 64: 630 us, 208 TFLOP/s (by 32-bit matrix instructions 1084).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
-    typedef at_tile<T, DP> tile;
-    typedef typename at_vec<T>::frag frag;
     typedef typename at_vec<T>::quad quad;
-    constexpr int CH = 16 / (int)sizeof(T), NG = tile::CPR / 2, NB = DP / 32, KT = AT_RT, TB = KT * tile::RB;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][TB];
+    constexpr int NG = DP / 16, NB = DP / 32, KT = AT_RT;
+    typedef at_tile<T, DP, KT> tile;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][tile::BYTES];
     __shared__ __attribute__((aligned(16))) float st[2][2][KT];
     constexpr bool LEAN = sizeof(T) == 2 && DP >= 64;
     constexpr bool VL = sizeof(T) == 2 && DP == 128;          // V stays in LDS: its registers are what would keep a second wave off the SIMD
@@ -654,14 +704,14 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
     const bool live = key < nk;
 
     const T *kp = a.k + b * a.ks[0] + (live ? key : 0) * a.ks[1] + hk * a.ks[2], *vp = a.v + b * a.vs[0] + (live ? key : 0) * a.vs[1] + hk * a.vs[2];
-    frag kf[NG], vf[VL ? 1 : NG];
+    at_op<T> kf[NG], vf[VL ? 1 : NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-        const int d = (2 * g + h) * CH;
-        const bool in = live && d < a.d;
-        kf[g] = in ? *(const frag *)(kp + d) : (frag)(0.f);
-        const frag x = in ? *(const frag *)(vp + d) : (frag)(0.f);
-        if (VL) *(frag *)(vt + (wave * NG + g) * 1024 + lane * 16) = x;
+        const int d = (2 * g + h) * 8;
+        at_op<T> x;
+        at_read(kp + d, live && d < a.d, kf[g]);
+        at_read(vp + d, live && d < a.d, x);
+        if (VL) *(at_op<T> *)(vt + (wave * NG + g) * 1024 + lane * 16) = x;
         else vf[VL ? 0 : g] = x;
     }
 
@@ -727,12 +777,12 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
         f32x16 s = (f32x16)(0.f), dp;
         AT_PRIO(2);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) s = at_mma(tile::row_frag(Q, lr, 2 * g + lh), kf[g], s);
+        for (int g = 0; g < NG; ++g) s = at_mma(tile::row(Q, lr, 2 * g + lh), kf[g], s);
 #pragma unroll
         for (int e = 0; e < 16; ++e) dp[e] = (*(const f32x4 *)&st[buf][1][2 * (e & ~3) + 4 * lh])[e & 3];
 #pragma unroll
         for (int g = 0; g < NG; ++g)
-            dp = at_mma(tile::row_frag(GO, lr, 2 * g + lh), VL ? *(const frag *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
+            dp = at_mma(tile::row(GO, lr, 2 * g + lh), VL ? *(const at_op<T> *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
         AT_PRIO(0);
         AT_PART(DP >= 64);
 #pragma unroll
@@ -748,8 +798,8 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
             dp[e] = ds;
         }
         AT_PRIO(1);
-        at_acc_t<DP>(ov, GO, 0, s, ln, (const T *)nullptr);
-        at_acc_t<DP>(ok, Q, 0, dp, ln, (const T *)nullptr);
+        tile::acc_t(ov, GO, 0, s, ln);
+        tile::acc_t(ok, Q, 0, dp, ln);
         AT_PRIO(0);
         if (more) store(buf ^ 1);
         __syncthreads();
