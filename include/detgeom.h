@@ -343,6 +343,8 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
  * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products, in DG_F32 products
  * are formed from three bf16 parts of each operand, which keeps their 24 bits; a DG_F32 value of 3.39e38 or more counts as infinite.
+ * rest (like out, bf16; may be NULL; DG_BF16 only): what rounding took from out, for the backward pass, whose delta is a sum of products
+ * with out that cancels where a row sees few keys: without it dq and dk are off by up to 2^-8 of the terms of that sum.
  * Results are the same in every run (no atomics). */
 typedef struct dg_attn_shape {   /* host */
     int64_t batch, nq, nk, q_heads, k_heads, d;
@@ -353,11 +355,11 @@ typedef struct dg_attn_shape {   /* host */
 } dg_attn_shape;
 size_t dg_roi_attn_workspace_bytes(const dg_attn_shape *shape, int backward);
 int dg_roi_attn_fwd(const dg_attn_shape *shape, const void *q, const void *k, const void *v, const int32_t *q_counts,
-                    const int32_t *k_counts, const uint8_t *mask, void *out, float *lse, void *ws, size_t ws_bytes, dg_stream_t s);
-/* out, lse: what the forward pass gave for the same inputs.  dq == NULL, or dk and dv both NULL: not computed */
+                    const int32_t *k_counts, const uint8_t *mask, void *out, float *lse, void *rest, void *ws, size_t ws_bytes, dg_stream_t s);
+/* out, lse, rest: what the forward pass gave for the same inputs.  dq == NULL, or dk and dv both NULL: not computed */
 int dg_roi_attn_bwd(const dg_attn_shape *shape, const void *grad_out, const void *q, const void *k, const void *v, const void *out,
-                    const float *lse, const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv,
-                    void *ws, size_t ws_bytes, dg_stream_t s);
+                    const float *lse, const void *rest, const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq,
+                    void *dk, void *dv, void *ws, size_t ws_bytes, dg_stream_t s);
 
 /* ---------------------------------------------------------------- the RoI head: rotary positions over several axes
  * NO COUNTERPART IN THE REFERENCE.  q (batch, n, q_heads, d), k (batch, n, k_heads, d; either may have 0 heads and be NULL): strides

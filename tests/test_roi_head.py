@@ -629,7 +629,7 @@ def test_refusals_of_the_library():
     p = C.c_void_p(4096)                         # never touched: every call below ends before a launch
 
     def fwd(s, q=p, ws=None, n=0):
-        return lib.dg_roi_attn_fwd(s, q, p, p, None, None, None, p, p, ws, n, None)
+        return lib.dg_roi_attn_fwd(s, q, p, p, None, None, None, p, p, None, ws, n, None)
     for kw, word in ((dict(d=12), "head size"), (dict(d=136), "head size"), (dict(q_heads=3), "multiple of k_heads"), (dict(k_heads=0), "multiple of k_heads"),
                      (dict(dtype=_abi.F16), "type"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
                      (dict(batch=-1), "negative"), (dict(nq=1 << 40), "2^28"), (dict(masks=3), "masks"), (dict(masks=1), "null"),
@@ -643,7 +643,7 @@ def test_refusals_of_the_library():
     assert need > 0 and fwd(long, ws=p, n=need - 1) == _abi.ENOMEM and "workspace" in _abi.last_error()
     assert fwd(shape(batch=0)) == _abi.OK and fwd(shape(nq=0)) == _abi.OK
     assert lib.dg_roi_attn_workspace_bytes(shape(d=12), 1) == 0
-    assert lib.dg_roi_attn_bwd(shape(), p, p, p, p, p, p, None, None, None, p, p, None, p, 1 << 30, None) == _abi.EINVAL     # dk without dv
+    assert lib.dg_roi_attn_bwd(shape(), p, p, p, p, p, p, None, None, None, None, p, p, None, p, 1 << 30, None) == _abi.EINVAL     # dk without dv
 
     def rope(**kw):
         s = _abi.RopeShape(1, 4, 2, 1, 64, 16, 2)
@@ -884,3 +884,62 @@ def test_roi_attention_keeps_the_bits_of_float32():
     out, _ = ops.roi_attention(q, q, v, mask=eye | eye.roll(1, 1))
     want = (v.double() + v.double().roll(-1, 1)) / 2
     assert float((out.double() - want).abs().max()) <= 2.0 ** -23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("n,D", [(1, 64), (2, 32), (3, 64), (5, 128), (7, 64)])
+def test_roi_attention_gradient_of_few_keys(n, D, masked):
+    """n keys of equal score: p is 1 / n (1 before it is divided, so without a rounding to bf16), the sum of ds over them 0, and dq, the
+    sum of ds k over equal k, 0 too; ds is what is left of dp - delta.  delta comes from out and its rest, 2^-16 of |do| |out| apart, ds
+    goes into its products as two parts, 2^-16 of it, and 32-bit sums of D terms add D 2^-24 of their magnitudes."""
+    from vision_amd import fast_rcnn, ops
+    N, u2 = 150, 2.0 ** -16
+    q, k, v, do = (t.double() for t in _attn_inputs(81, 2, N, 40 if masked else n, 2, 1, D, torch.bfloat16))
+    k[:] = k[:, :1]
+    mask = None
+    if masked:
+        mask = torch.zeros((2, N, 40), dtype=torch.bool)
+        mask[:, :, torch.randperm(40, generator=_gen(82))[:n]] = True
+    seen = slice(None) if mask is None else mask[0, 0].nonzero()[:, 0]
+    V = v[:, seen, 0]                             # (2, n, D)
+    o = V.mean(1)[:, None, None]                  # (2, 1, 1, D)
+    dp = torch.einsum("bihd,bjd->bihj", do, V)
+    ds = (dp - (do * o).sum(-1, keepdim=True)) / n
+    mag = torch.einsum("bihd,bjd->bihj", do.abs(), V.abs()) + (do.abs() * o.abs()).sum(-1, keepdim=True)
+    eds = ds.abs() * (u2 + 16 * E32) + ((do.abs() * o.abs()).sum(-1, keepdim=True) * u2 + (D + 8) * E32 * mag) / n + 8 * E32 * dp.abs() / n
+    sc = D ** -0.5
+    dk = torch.einsum("bihj,bihd->bjd", ds, q) * sc
+    edk = torch.einsum("bihj,bihd->bjd", eds + 2 * N * E32 * ds.abs(), q.abs()) * sc + 2.0 ** -8 * dk.abs()
+    edq = (eds + n * E32 * ds.abs()).sum(-1, keepdim=True) * k[:, :1, :1].abs() * sc
+    Q, K, W, G = (t.to(torch.bfloat16).cuda() for t in (q, k, v, do))
+    out, lse, rest = ops.roi_attention(Q, K, W, mask=_dev(mask), rest=True)
+    a = ops.roi_attention_backward(G, Q, K, W, out, lse, mask=_dev(mask), rest=rest)
+    Q, K, W = (t.requires_grad_(True) for t in (Q, K, W))
+    b = torch.autograd.grad(fast_rcnn.roi_attention(Q, K, W, mask=_dev(mask)), (Q, K, W), G)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    _close(a[0], (torch.zeros_like(q), edq), "dq")
+    _close(a[1][:, seen, 0], (dk, edk), "dk")
+
+
+@pytest.mark.gpu
+def test_roi_attention_rest():
+    """out + rest is the output in 16 bits, also where splits are joined; rows that see nothing have none; float32 has none."""
+    from vision_amd import ops
+    for case in ((2, 100, 70, 4, 2, 64, True, None), (1, 3, 5000, 2, 1, 128, True, None), (1, 70, 3000, 2, 2, 40, False, "shared")):
+        q, k, v, _ = _attn_inputs(91, *case[:6], torch.bfloat16)
+        qc, kc, m = _attn_masks(case, 91)
+        one = ops.roi_attention(*map(_dev, (q, k, v, qc, kc, m)), rest=True)
+        two = ops.roi_attention(*map(_dev, (q, k, v, qc, kc, m)))
+        assert torch.equal(one[0], two[0]) and torch.equal(one[1], two[1]) and len(two) == 2
+        out, rest = one[0].cpu().double(), one[2].cpu().double()
+        assert bool((rest.abs() <= 2.0 ** -8 * out.abs()).all()) and float(rest.abs().max()) > 0.0
+        if qc is not None:
+            assert all(float(rest[b, int(qc[b]):].abs().sum()) == 0.0 for b in range(case[0]))
+        want = _attn64(q, k, v, qc, kc, m, None)["out"]
+        p_only = want[1] - 2.0 ** -8 * want[0].abs() + 2.0 ** -16 * want[0].abs()       # without the rounding of out
+        _close(torch.from_numpy((out + rest).numpy()), (want[0], p_only), "out + rest")
+    q = torch.randn(1, 4, 1, 8, device="cuda")
+    assert ops.roi_attention(q, q, q, rest=True)[2] is None
+    with pytest.raises(ValueError, match="rest"):
+        ops.roi_attention_backward(q, q, q, q, *ops.roi_attention(q, q, q), rest=q)

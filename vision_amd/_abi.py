@@ -98,8 +98,8 @@ SIGNATURES = {
     "dg_voc_ap_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "dg_voc_ap_f32": (C.c_int, [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _f32, _vp, _vp, _vp, _sz, _vp]),
     "dg_roi_attn_workspace_bytes": (_sz, [C.POINTER(AttnShape), C.c_int]),
-    "dg_roi_attn_fwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 9 + [_sz, _vp]),
-    "dg_roi_attn_bwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 13 + [_sz, _vp]),
+    "dg_roi_attn_fwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 10 + [_sz, _vp]),
+    "dg_roi_attn_bwd": (C.c_int, [C.POINTER(AttnShape)] + [_vp] * 14 + [_sz, _vp]),
     "dg_rope_axes": (C.c_int, [C.POINTER(RopeShape)] + [_vp] * 5 + [C.c_int] + [_vp] * 3),
     "dg_class_logprobs_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "dg_class_logprobs": (C.c_int, [_vp, C.c_int, _vp, _i64, _i64, _i64, _i64] + [_vp] * 7 + [_sz, _vp]),

@@ -65,20 +65,24 @@ __device__ __forceinline__ void at_less(bf16x2 h, float &x, float &y)
     x = __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, c), x, false);
     y = __builtin_amdgcn_fdot2_f32_bf16(h, (bf16x2){(__bf16)0.f, (__bf16)-1.f}, y, false);
 }
+// the next part of x, which is left with the rest
+__device__ __forceinline__ bf16x8 at_next(f32x8 &x)
+{
+    const bf16x8 h = __builtin_convertvector(x, bf16x8);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        float a = x[e], b = x[e + 1];
+        at_less((bf16x2){h[e], h[e + 1]}, a, b);
+        x[e] = a;
+        x[e + 1] = b;
+    }
+    return h;
+}
 __device__ __forceinline__ void at_cut(f32x8 x, at_op<float> &o)
 {
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        const bf16x8 h = __builtin_convertvector(x, bf16x8);
-        o.p[i] = h;
-#pragma unroll
-        for (int e = 0; e < 8 && i < 2; e += 2) {
-            float a = x[e], b = x[e + 1];
-            at_less((bf16x2){h[e], h[e + 1]}, a, b);
-            x[e] = a;
-            x[e + 1] = b;
-        }
-    }
+    o.p[0] = at_next(x);
+    o.p[1] = at_next(x);
+    o.p[2] = __builtin_convertvector(x, bf16x8);
 }
 // eight values of a row in memory
 __device__ __forceinline__ void at_read(const __bf16 *p, bool in, at_op<__bf16> &o) { o.p[0] = in ? *(const bf16x8 *)p : (bf16x8)(0.f); }
@@ -130,14 +134,20 @@ template <typename T, int DP, int ROWS> struct at_tile {
             v = (f32x4){a, b, c, d};
         }
     }
-    // acc[db] (32 values of d x 32 columns) += tile[rows base..base+31][d]^T * w, w in the result layout (rows = the tile's rows)
-    static __device__ __forceinline__ void acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane)
+    // acc[db] (32 values of d x 32 columns) += tile[rows base..base+31][d]^T * w, w in the result layout (rows = the tile's rows); FINE:
+    // in bf16 w goes in as two parts
+    template <bool FINE = false> static __device__ __forceinline__ void acc_t(f32x16 (&acc)[DP / 32], const char *t, int base, const f32x16 &w, int lane)
     {
         const int h = lane >> 5, j = lane & 15, row0 = base + 4 * h + (j >> 2), part = ((lane >> 4) & 1) * 2 + ((j & 3) >> 1);
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            at_op<T> b;                           // bf16: one rounding to 8 bits; the sum stays in 32
-            at_cut(s ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7), b);
+            f32x8 x = s ? __builtin_shufflevector(w, w, 8, 9, 10, 11, 12, 13, 14, 15) : __builtin_shufflevector(w, w, 0, 1, 2, 3, 4, 5, 6, 7);
+            at_op<T> b;                           // bf16: one rounding to 8 bits (FINE: to 16); the sum stays in 32
+            bf16x8 low = (bf16x8)(0.f);
+            if (FINE && N == 1) {
+                b.p[0] = at_next(x);
+                low = __builtin_convertvector(x, bf16x8);
+            } else at_cut(x, b);
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) {
                 typedef __attribute__((address_space(3))) s16x4 *lp;
@@ -148,6 +158,7 @@ template <typename T, int DP, int ROWS> struct at_tile {
                     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(t + i * PLANE + at(row0 + 16 * s + 8, db * 4 + part) + (j & 1) * 8));
                     a.p[i] = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                 }
+                if (FINE && N == 1) acc[db] = at_mfma(a.p[0], low, acc[db]);
                 acc[db] = at_mma(a, b, acc[db]);
             }
         }
@@ -158,7 +169,7 @@ template <typename T, int DP, int ROWS> struct at_tile {
 template <typename T> struct at_args {
     const T *q, *k, *v, *g;                       // g: gradient of the output (backward)
     T *o, *dk;                                    // o: output / dq; dk, dv
-    T *dv;
+    T *dv, *rest;                                 // rest: what rounding took from the output (bf16; may be NULL)
     float *lse;                                   // forward: output (b, hq, nq)
     const f32x2 *stat;                            // backward: (b, hq, nq) pairs of a row's log-sum in base 2 and -delta
     float *part;                                  // partial results of a split call
@@ -169,6 +180,15 @@ template <typename T> struct at_args {
     int words, batch, nq, nk, hq, hk, d, tiles, splits, per;    // per: rows or keys of a split, a multiple of the tile
     float c, scale, slack;                        // c = scale * log2(e); slack = 8 / c
 };
+
+// four values of the output, and what rounding took from them
+template <typename T> __device__ __forceinline__ void at_out(const at_args<T> &a, T *o, f32x4 x)
+{
+    typedef typename at_vec<T>::quad quad;
+    const quad r = __builtin_convertvector(x, quad);
+    *(quad *)o = r;
+    if (sizeof(T) == 2 && a.rest) *(quad *)(a.rest + (o - a.o)) = __builtin_convertvector(x - __builtin_convertvector(r, f32x4), quad);
+}
 
 __device__ __forceinline__ int at_count(const int32_t *c, int b, int n) { return c ? min(max(c[b], 0), n) : n; }
 
@@ -313,7 +333,6 @@ template <typename T, int DP> struct at_shape {
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd(const at_args<T> a)
 {
-    typedef typename at_vec<T>::quad quad;
     constexpr int NG = DP / 16, NB = DP / 32, KT = at_shape<T, DP>::KT, U = KT / 32;
     typedef at_tile<T, DP, KT> tile;
     __shared__ __attribute__((aligned(16))) char lds[2][2][tile::BYTES];
@@ -328,7 +347,10 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         for (int p = tix; p < G * pad; p += a.tiles) {
             const int hq = hk * G + p / pad, n = nq + p % pad;
             T *o = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
-            for (int d = threadIdx.x; d < a.d; d += AT_THREADS) o[d] = (T)0.f;
+            for (int d = threadIdx.x; d < a.d; d += AT_THREADS) {
+                o[d] = (T)0.f;
+                if (a.rest) a.rest[o - a.o + d] = (T)0.f;
+            }
             if (threadIdx.x == 0) a.lse[((int64_t)b * a.hq + hq) * a.nq + n] = -INFINITY;
         }
     }
@@ -462,8 +484,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int d = i * 32 + 2 * e + 4 * h;
-            if (d < a.d)
-                *(quad *)(op + d) = __builtin_convertvector(((f32x4){o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv}), quad);
+            if (d < a.d) at_out(a, op + d, (f32x4){o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv});
         }
 }
 
@@ -474,7 +495,6 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
 template <typename T, bool MANY>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, int64_t rows)
 {
-    typedef typename at_vec<T>::quad quad;
     constexpr int LANES = MANY ? 8 : 32, GROUPS = AT_THREADS / LANES;
     __shared__ __attribute__((aligned(16))) f32x4 red[MANY ? GROUPS : 1][LANES];
     __shared__ float tots[GROUPS], tops[AT_WAVES];
@@ -482,7 +502,8 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, in
     const int64_t row = MANY ? blockIdx.x / cuts : (int64_t)blockIdx.x * GROUPS + grp;
     const int d = (MANY ? (int)(blockIdx.x % cuts) * 32 : 0) + sub * 4;
     if (row >= rows) return;                      // MANY: the whole workgroup
-    const int n = (int)(row % a.nq), hq = (int)(row / a.nq % a.hq), b = (int)(row / a.nq / a.hq);
+    const u32 bh = (u32)row / a.nq, b = bh / a.hq;
+    const int n = (int)((u32)row - bh * a.nq), hq = (int)(bh - b * a.hq);
     if (n >= at_count(a.qc, b, a.nq)) return;     // written by the first kernel
     const float *ls = a.part + row * a.splits, *po = a.part + rows * a.splits + row * a.splits * a.d + d;
     float m = -INFINITY;
@@ -516,22 +537,28 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, in
         }
     }
     const float inv = tot == 0.f ? 0.f : 1.f / tot;
-    if (in) *(quad *)(a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d + d) = __builtin_convertvector(v * inv, quad);
+    if (in) at_out(a, a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d + d, v * inv);
     if (d == 0) a.lse[row] = tot == 0.f ? -INFINITY : (base + __builtin_amdgcn_logf(tot)) * AT_LN2;
 }
 
 // ------------------------------------------------------------------ backward
-// delta_i = do_i . o_i and the rows' log-sums in base 2; a row that sees nothing gets +inf there, so that its p is 0.  Bound by memory:
-// 8 x 2000 x 8 x 64 bf16: 11 us, 6.0 TB/s.
+// How ds enters its products in bf16.  The sum of ds over a row's keys is 0, so dq and dk are what is left of larger terms, the more so
+// the fewer keys a row sees.  With few keys (and under a pair mask, which may leave few) ds goes in as two parts, 16 bits; elsewhere one
+// rounding to 8 bits is of no more weight than that of the result.
+enum { AT_PLAIN, AT_FINE, AT_MASKED };
+// delta_i = do_i . o_i and the rows' log-sums in base 2; a row that sees nothing gets +inf there, so that its p is 0.  From the output as
+// rounded to bf16 alone delta would be off by 2^-8 of its terms, which where few keys are seen is as much as ds itself (one key: ds is 0);
+// with what rounding took, by 2^-16.  Bound by memory: 8 images of 1000 to 2000 rows x 8 x 64 bf16: 11 us, 3.6 TB/s.
 template <typename T, bool MASK>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, const T *__restrict__ out, const float *__restrict__ lse, f32x2 *__restrict__ stat,
-                                                           int64_t rows)
+                                                           u32 rows)
 {
     constexpr int CH = 16 / (int)sizeof(T), LPR = 128 / CH, RPB = AT_THREADS / LPR;
     const int sub = threadIdx.x % LPR;
-    const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;     // (b, n, hq), heads innermost as in memory
+    const u32 row = blockIdx.x * RPB + threadIdx.x / LPR;     // (b, n, hq), heads innermost as in memory; fewer than 2^28 (at_check)
     if (row >= rows) return;
-    const int hq = (int)(row % a.hq), n = (int)(row / a.hq % a.nq), b = (int)(row / a.hq / a.nq);
+    const u32 bn = row / a.hq, b = bn / a.nq;
+    const int hq = (int)(row - bn * a.hq), n = (int)(bn - b * a.nq);
     const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
     const bool live = n < at_count(a.qc, b, a.nq);
     float sum = 0.f;
@@ -539,9 +566,14 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
     const int d = sub * CH;
     if (live && d < a.d) {
         const typename at_vec<T>::frag x = *(const typename at_vec<T>::frag *)(a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2] + d);
-        const typename at_vec<T>::frag y = *(const typename at_vec<T>::frag *)(out + row * a.d + d);
+        const typename at_vec<T>::frag y = *(const typename at_vec<T>::frag *)(out + (int64_t)row * a.d + d);
 #pragma unroll
         for (int i = 0; i < CH; ++i) sum = fmaf((float)x[i], (float)y[i], sum);
+        if (sizeof(T) == 2 && a.rest) {
+            const typename at_vec<T>::frag z = *(const typename at_vec<T>::frag *)(a.rest + (int64_t)row * a.d + d);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) sum = fmaf((float)x[i], (float)z[i], sum);
+        }
         if (MASK) {
             u32x4 xs = __builtin_bit_cast(u32x4, x), qs = at_load_chunk(a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2] + d);
             bad = (int)at_scrub<T>(xs) | (int)at_scrub<T>(qs);
@@ -560,9 +592,10 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
 // dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp).
 // Three products a tile.  Measured, bf16: 16 x 2000, 8 heads of 64: 247 us, 796 TFLOP/s; 16000, 8 heads of 128: 1511 us, 1041 TFLOP/s;
 // fp32, 8 x 2000, 8 heads of 64: 480 us, 205 TFLOP/s (by 32-bit matrix instructions 810).
-template <typename T, int DP, bool MASK>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_dq(const at_args<T> a)
 {
+    constexpr bool MASK = MODE == AT_MASKED, FINE = MODE != AT_PLAIN;
     typedef typename at_vec<T>::quad quad;
     constexpr int NG = DP / 16, NB = DP / 32, KT = at_shape<T, DP>::KT_Q, U = KT / 32;
     typedef at_tile<T, DP, KT> tile;
@@ -654,7 +687,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
                 s[e] = ds;
             }
             AT_PRIO(1);
-            tile::acc_t(o, K, u * 32, s, lane);
+            tile::template acc_t<FINE>(o, K, u * 32, s, lane);
             AT_PRIO(0);
         }
         if (more) store(buf ^ 1);
@@ -682,9 +715,10 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
 // dp) and transposed (dk, dv).  Four products a tile, and 2 x 32 x d accumulators a wave, which bound how many waves share a SIMD.
 // Measured, bf16: 16 x 2000, 8 heads of 64: 408 us, 642 TFLOP/s; 16000, 8 heads of 128: 2140 us, 980 TFLOP/s; fp32, 8 x 2000, 8 heads of
 // 64: 630 us, 208 TFLOP/s (by 32-bit matrix instructions 1084).
-template <typename T, int DP, bool MASK>
-__global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
+template <typename T, int DP, int MODE>
+__global__ __launch_bounds__(AT_THREADS, (MODE == AT_MASKED && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
+    constexpr bool MASK = MODE == AT_MASKED, FINE = MODE != AT_PLAIN;
     typedef typename at_vec<T>::quad quad;
     constexpr int NG = DP / 16, NB = DP / 32, KT = AT_RT;
     typedef at_tile<T, DP, KT> tile;
@@ -799,7 +833,7 @@ __global__ __launch_bounds__(AT_THREADS, (MASK && at_shape<T, DP>::OCC_KV == 3 ?
         }
         AT_PRIO(1);
         tile::acc_t(ov, GO, 0, s, ln);
-        tile::acc_t(ok, Q, 0, dp, ln);
+        tile::template acc_t<FINE>(ok, Q, 0, dp, ln);
         AT_PRIO(0);
         if (more) store(buf ^ 1);
         __syncthreads();
@@ -833,11 +867,12 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_sum(const float *__restrict
                                                          int nmax, int d, int splits)
 {
     typedef typename at_vec<T>::quad quad;
-    const int64_t i = (int64_t)blockIdx.x * AT_THREADS + threadIdx.x, row = i / (d / 4);
+    const u32 i = blockIdx.x * AT_THREADS + threadIdx.x, row = i / (u32)(d / 4);     // a split call has few rows
     if (row >= rows) return;
-    const int x = (int)(i - row * (d / 4)) * 4, n = (int)(row % nmax), hh = (int)(row / nmax % heads), b = (int)(row / nmax / heads);
+    const u32 bh = row / nmax, b = bh / heads;
+    const int x = (int)(i - row * (d / 4)) * 4, n = (int)(row - bh * nmax), hh = (int)(bh - b * heads);
     if (n >= at_count(counts, b, nmax)) return;
-    const float *p = part + ((blockIdx.y ? rows : 0) + row) * splits * d + x;
+    const float *p = part + ((blockIdx.y ? rows : 0) + (int64_t)row) * splits * d + x;
     f32x4 v = (f32x4)(0.f);
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) v += *(const f32x4 *)(p + (int64_t)s * d);
@@ -967,24 +1002,25 @@ template <typename T> static void *at_bits(const dg_attn_shape *s, const at_plan
     return (char *)ws + p.bits;
 }
 
-#define AT_LAUNCH(kernel, grid, a)                                                                                              \
+#define AT_LAUNCH(kernel, mode, grid, a)                                                                                        \
     do {                                                                                                                        \
         const dim3 gr_((unsigned)(grid)), bl_(AT_THREADS);                                                                       \
-        if ((a).d <= 32) { if ((a).bits) hipLaunchKernelGGL((kernel<T, 32, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 32, false>), gr_, bl_, 0, st, a); } \
-        else if ((a).d <= 64) { if ((a).bits) hipLaunchKernelGGL((kernel<T, 64, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 64, false>), gr_, bl_, 0, st, a); } \
-        else { if ((a).bits) hipLaunchKernelGGL((kernel<T, 128, true>), gr_, bl_, 0, st, a); else hipLaunchKernelGGL((kernel<T, 128, false>), gr_, bl_, 0, st, a); } \
+        if ((a).d <= 32) hipLaunchKernelGGL((kernel<T, 32, mode>), gr_, bl_, 0, st, a);                                          \
+        else if ((a).d <= 64) hipLaunchKernelGGL((kernel<T, 64, mode>), gr_, bl_, 0, st, a);                                     \
+        else hipLaunchKernelGGL((kernel<T, 128, mode>), gr_, bl_, 0, st, a);                                                     \
     } while (0)
 
 template <typename T>
 static int at_forward(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *qc, const int32_t *kc, const uint8_t *mask, void *out,
-                      float *lse, void *ws, hipStream_t st)
+                      float *lse, void *rest, void *ws, hipStream_t st)
 {
     const at_plan p = at_plan_of(s);
     at_args<T> a = at_fill<T>(s, q, k, v, qc, kc);
     ws = at_bits(s, p, mask, a, ws, st);
-    a.o = (T *)out; a.lse = lse; a.part = (float *)ws;
+    a.o = (T *)out; a.lse = lse; a.rest = (T *)rest; a.part = (float *)ws;
     a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
-    AT_LAUNCH(k_attn_fwd, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
+    if (a.bits) AT_LAUNCH(k_attn_fwd, true, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
+    else AT_LAUNCH(k_attn_fwd, false, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
     if (p.qsplits > AT_JOIN_FEW) hipLaunchKernelGGL((k_attn_join<T, true>), dim3((unsigned)(p.rows * dg_cdiv(s->d, 32))), dim3(AT_THREADS), 0, st, a, p.rows);
     else if (p.qsplits > 1) hipLaunchKernelGGL((k_attn_join<T, false>), dim3((unsigned)dg_cdiv(p.rows, 8)), dim3(AT_THREADS), 0, st, a, p.rows);
     DG_CHECK_LAUNCH("k_attn_fwd");
@@ -992,40 +1028,47 @@ static int at_forward(const dg_attn_shape *s, const void *q, const void *k, cons
 }
 
 extern "C" int dg_roi_attn_fwd(const dg_attn_shape *s, const void *q, const void *k, const void *v, const int32_t *q_counts, const int32_t *k_counts,
-                               const uint8_t *mask, void *out, float *lse, void *ws, size_t ws_bytes, dg_stream_t stream)
+                               const uint8_t *mask, void *out, float *lse, void *rest, void *ws, size_t ws_bytes, dg_stream_t stream)
 {
     const int rc = at_check(s, "roi_attn_fwd");
     if (rc != DG_OK) return rc;
     if (s->batch == 0 || s->nq == 0) return DG_OK;
     DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v && !mask == !s->masks)), "roi_attn_fwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
-                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && (((uintptr_t)out) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
+                   at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && ((((uintptr_t)out) | ((uintptr_t)rest)) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 0);
     if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_fwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
     DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_fwd: workspace must be 16-byte aligned");
-    return s->dtype == DG_F32 ? at_forward<float>(s, q, k, v, q_counts, k_counts, mask, out, lse, ws, (hipStream_t)stream)
-                              : at_forward<__bf16>(s, q, k, v, q_counts, k_counts, mask, out, lse, ws, (hipStream_t)stream);
+    return s->dtype == DG_F32 ? at_forward<float>(s, q, k, v, q_counts, k_counts, mask, out, lse, rest, ws, (hipStream_t)stream)
+                              : at_forward<__bf16>(s, q, k, v, q_counts, k_counts, mask, out, lse, rest, ws, (hipStream_t)stream);
 }
 
 template <typename T>
-static int at_backward(const dg_attn_shape *s, const void *g, const void *q, const void *k, const void *v, const void *out, const float *lse, const int32_t *qc,
+static int at_backward(const dg_attn_shape *s, const void *g, const void *q, const void *k, const void *v, const void *out, const float *lse, const void *rest, const int32_t *qc,
                        const int32_t *kc, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, hipStream_t st)
 {
     const at_plan p = at_plan_of(s);
     at_args<T> a = at_fill<T>(s, q, k, v, qc, kc);
     ws = at_bits(s, p, mask, a, ws, st);
+    constexpr int FINE = sizeof(T) == 2 ? AT_FINE : AT_PLAIN;
+    // 16 x 500 rows and keys x 64: dq 36 -> 39 us, dk, dv 47 -> 51, for errors of dq, dk of 1.0 instead of 1.45 roundings of the result (2.3 at 10
+    // keys of which a fifth is seen); 16000 x 128: dq 1575 -> 1980, dk, dv 2235 -> 2545, for 1.0 instead of 1.42
+    const bool fine = s->nk <= 512;
     f32x2 *stat = (f32x2 *)ws;
-    a.g = (const T *)g; a.stat = stat; a.part = (float *)((char *)ws + p.stats);
+    a.g = (const T *)g; a.rest = (T *)rest; a.stat = stat; a.part = (float *)((char *)ws + p.stats);
     if (s->nq > 0) {
         const int64_t rpb = AT_THREADS * (16 / (int64_t)sizeof(T)) / 128;
         const dim3 grid((unsigned)dg_cdiv(p.rows, rpb));
-        if (a.bits) hipLaunchKernelGGL((k_attn_delta<T, true>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, p.rows);
-        else hipLaunchKernelGGL((k_attn_delta<T, false>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, p.rows);
+        if (a.bits) hipLaunchKernelGGL((k_attn_delta<T, true>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, (u32)p.rows);
+        else hipLaunchKernelGGL((k_attn_delta<T, false>), grid, dim3(AT_THREADS), 0, st, a, (const T *)out, lse, stat, (u32)p.rows);
     }
     if (s->nq > 0 && dq) {
         a.o = (T *)dq;
         a.tiles = (int)p.qtiles; a.splits = (int)p.qsplits; a.per = (int)p.qper;
-        AT_LAUNCH(k_attn_dq, s->batch * s->k_heads * p.qtiles * p.qsplits, a);
+        const int64_t grid = s->batch * s->k_heads * p.qtiles * p.qsplits;
+        if (a.bits) AT_LAUNCH(k_attn_dq, AT_MASKED, grid, a);
+        else if (fine) AT_LAUNCH(k_attn_dq, FINE, grid, a);
+        else AT_LAUNCH(k_attn_dq, AT_PLAIN, grid, a);
         if (p.qsplits > 1)
             hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d / 4, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, (T *)nullptr, qc, p.rows,
                                (int)s->q_heads, (int)s->nq, (int)s->d, (int)p.qsplits);
@@ -1033,7 +1076,10 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
     if (s->nk > 0 && dk) {
         a.dk = (T *)dk; a.dv = (T *)dv;
         a.tiles = (int)p.ktiles; a.splits = (int)p.ksplits; a.per = (int)p.kper;
-        AT_LAUNCH(k_attn_dkv, s->batch * s->k_heads * p.ktiles * p.ksplits, a);
+        const int64_t grid = s->batch * s->k_heads * p.ktiles * p.ksplits;
+        if (a.bits) AT_LAUNCH(k_attn_dkv, AT_MASKED, grid, a);
+        else if (fine) AT_LAUNCH(k_attn_dkv, FINE, grid, a);
+        else AT_LAUNCH(k_attn_dkv, AT_PLAIN, grid, a);
         if (p.ksplits > 1) {
             const int64_t rows = s->batch * s->k_heads * s->nk;
             hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(rows * s->d / 4, AT_THREADS), 2), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dk, (T *)dv,
@@ -1045,7 +1091,7 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
 }
 
 extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, const void *q, const void *k, const void *v, const void *out, const float *lse,
-                               const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, size_t ws_bytes,
+                               const void *rest, const int32_t *q_counts, const int32_t *k_counts, const uint8_t *mask, void *dq, void *dk, void *dv, void *ws, size_t ws_bytes,
                                dg_stream_t stream)
 {
     const int rc = at_check(s, "roi_attn_bwd");
@@ -1054,11 +1100,11 @@ extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, con
     DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv && (s->nk == 0 || s->nq == 0 || !mask == !s->masks), "roi_attn_bwd: null pointer");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && at_aligned(grad_out, s->g_stride, s, s->nq, s->q_heads) &&
-                   ((((uintptr_t)out) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
+                   ((((uintptr_t)out) | ((uintptr_t)rest) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 1);
     if (ws_bytes < need || (need && !ws)) { dg_set_error("roi_attn_bwd: workspace %zu < %zu bytes", ws_bytes, need); return DG_ENOMEM; }
     DG_REQUIRE((((uintptr_t)ws) & 15) == 0, "roi_attn_bwd: workspace must be 16-byte aligned");
     return s->dtype == DG_F32
-               ? at_backward<float>(s, grad_out, q, k, v, out, lse, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream)
-               : at_backward<__bf16>(s, grad_out, q, k, v, out, lse, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream);
+               ? at_backward<float>(s, grad_out, q, k, v, out, lse, rest, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream)
+               : at_backward<__bf16>(s, grad_out, q, k, v, out, lse, rest, q_counts, k_counts, mask, dq, dk, dv, ws, (hipStream_t)stream);
 }

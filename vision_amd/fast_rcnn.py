@@ -100,18 +100,18 @@ class _RoIAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_counts, k_counts, mask, scale):
         args = ops._attn_args(q, k, v, q_counts, k_counts, mask)
-        out, lse = ops._attn_forward(args, scale)
-        ctx.save_for_backward(*args[1:7], out, lse)     # as they were laid out for the kernels
+        out, lse, rest = ops._attn_forward(args, scale, any(ctx.needs_input_grad))
+        ctx.save_for_backward(*args[1:7], out, lse, rest)     # as they were laid out for the kernels
         ctx.rest = args[0], args[7], args[8], scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        *args, out, lse = ctx.saved_tensors
+        *args, out, lse, rest = ctx.saved_tensors
         dev, masks, ms, scale = ctx.rest
         need = ctx.needs_input_grad
-        dq, dk, dv = ops._attn_backward((dev, *args, masks, ms), grad_out, out, lse, scale, need[0], need[1] or need[2])
+        dq, dk, dv = ops._attn_backward((dev, *args, masks, ms), grad_out, out, lse, rest, scale, need[0], need[1] or need[2])
         return dq, dk if need[1] else None, dv if need[2] else None, None, None, None, None
 
 

@@ -426,42 +426,50 @@ def _attn_args(q, k, v, q_counts, k_counts, mask):
     return dev, _vec16(q), _vec16(k), _vec16(v), qc, kc, mask, mask.shape[0], mask.stride()
 
 
-def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
+def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None, rest=False):
     """Attention over padded sets of RoIs or map cells: q (B,Nq,Hq,D), k and v (B,Nk,Hk,D), float32 or bfloat16, any strides,
     Hq a multiple of Hk (query head h reads key head h // (Hq // Hk)), D a multiple of 8 up to 128 -> out (B,Nq,Hq,D),
     lse (B,Hq,Nq) float32.  A row sees the keys before k_counts (B) of its image for which mask (B or 1,Nq,Nk) is not 0; scale
-    defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  No reference
-    counterpart.  For a gradient: fast_rcnn.roi_attention."""
-    return _attn_forward(_attn_args(q, k, v, q_counts, k_counts, mask), scale)
+    defaults to D ** -0.5.  Rows that see nothing, rows behind q_counts (B) among them: out 0, lse -inf.  rest: -> out,
+    lse, rest, what rounding took from a bfloat16 out (None in float32), for roi_attention_backward.  No reference counterpart.
+    For a gradient: fast_rcnn.roi_attention."""
+    r = _attn_forward(_attn_args(q, k, v, q_counts, k_counts, mask), scale, rest)
+    return r if rest else r[:2]
 
 
-def _attn_forward(args, scale):
+def _attn_forward(args, scale, keep_rest):
     dev, q, k, v, qc, kc, mask, masks, ms = args
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, None if scale is None else float(scale), q.dtype, 0)
     out = torch.empty(q.shape, dtype=q.dtype, device=dev)
     lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
+    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if keep_rest and q.dtype == torch.bfloat16 else None
     ws = _scratch(nbytes, dev)
     with _abi.on_device(dev):
-        check(load().dg_roi_attn_fwd(s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(qc), _at(kc), _at(mask), out.data_ptr(), lse.data_ptr(), _at(ws), nbytes,
-                                     _stream(dev)))
-    return out, lse
+        check(load().dg_roi_attn_fwd(s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(qc), _at(kc), _at(mask), out.data_ptr(), lse.data_ptr(), _at(rest), _at(ws),
+                                     nbytes, _stream(dev)))
+    return out, lse, rest
 
 
-def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=None, mask=None, scale=None, need_q=True, need_kv=True):
+def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=None, mask=None, scale=None, need_q=True, need_kv=True, rest=None):
     """Gradients of roi_attention from its inputs, out and lse, with the probabilities recomputed: dq (B,Nq,Hq,D), dk and dv
-    (B,Nk,Hk,D), rows behind a count 0.  need_q / need_kv False leaves those out (None)."""
+    (B,Nk,Hk,D), rows behind a count 0.  need_q / need_kv False leaves those out (None).  rest: roi_attention's; without it dq and
+    dk of a bfloat16 call are off by up to 2^-8 of grad_out . out where a row sees few keys."""
     args = _attn_args(q, k, v, q_counts, k_counts, mask)
     dev, q = args[0], args[1]
     if not (grad_out.device == dev and out.device == dev and lse.device == dev):
         grad_out, out, lse = grad_out.to(dev), out.to(dev), lse.to(dev)
+    if rest is not None:
+        if rest.shape != q.shape or rest.dtype != q.dtype or q.dtype != torch.bfloat16:
+            raise ValueError("roi_attention_backward: rest must have q's shape and be bfloat16, as q")
+        rest = _vec16(rest.to(dev).contiguous())
     if grad_out.shape != q.shape or out.shape != q.shape or grad_out.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError("roi_attention_backward: grad_out and out must have q's shape and type")
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32:
         raise ValueError("roi_attention_backward: lse must be (B,Hq,Nq) float32")
-    return _attn_backward(args, grad_out, _vec16(out.contiguous()), lse.contiguous(), scale, need_q, need_kv)
+    return _attn_backward(args, grad_out, _vec16(out.contiguous()), lse.contiguous(), rest, scale, need_q, need_kv)
 
 
-def _attn_backward(args, g, out, lse, scale, need_q, need_kv):
+def _attn_backward(args, g, out, lse, rest, scale, need_q, need_kv):
     dev, q, k, v, qc, kc, mask, masks, ms = args
     g = _vec16(g)
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, None if scale is None else float(scale), q.dtype, 1)
@@ -470,7 +478,7 @@ def _attn_backward(args, g, out, lse, scale, need_q, need_kv):
     dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
     ws = _scratch(nbytes, dev)
     with _abi.on_device(dev):
-        check(load().dg_roi_attn_bwd(s, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _at(qc), _at(kc), _at(mask),
+        check(load().dg_roi_attn_bwd(s, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _at(rest), _at(qc), _at(kc), _at(mask),
                                      _at(dq), _at(dk), _at(dv), _at(ws), nbytes, _stream(dev)))
     return dq, dk, dv
 
