@@ -102,6 +102,7 @@ ATTN_CASES = [
     (1, 5000, 40, 2, 2, 64, False, None),        # few keys, many rows: dk, dv split over the rows
     (1, 700, 900, 2, 2, 72, False, "shared"),
     (2, 64, 100, 2, 1, 104, True, "none"),       # a mask that leaves every row empty
+    (1, 90, 700, 2, 1, 24, False, None),         # more keys than those for which ds is cut in two
     (4, 50, 50, 3, 3, 16, "zero", None),         # images with no rows or no keys at all
 ]
 
