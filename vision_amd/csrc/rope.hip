@@ -1,7 +1,7 @@
 // rope.hip — rotary positions over several axes (frame, row, column of a box centre or map cell) for queries and keys.
 //   pair j of a token turns by a = pos[token][axis_j] * f_j:  (u, v) -> (u cos a - v sin a, u sin a + v cos a)
 // The map is a rotation, so its gradient is the turn by -a: the same kernel.  Values are read once and written once: bound by
-// memory: 4 x 30400 tokens, 20 heads of 128 bf16: 214 us, 5.8 TB/s; 16 x 2000, 16 heads of 80 fp32: 73 us, 4.5 TB/s (a copy of 1 GB: 5.0).
+// memory: 4 x 30400 tokens, 20 heads of 128 bf16: 212 us, 5.9 TB/s; 16 x 2000, 16 heads of 80 fp32: 70 us, 4.7 TB/s (a copy of 1 GB: 5.0).
 // The sines of a token are formed once, by the first phase of its workgroup, and serve all heads of q and k from LDS.
 // Angles are held in turns in 64 bits and reduced to [-1/2, 1/2] before they are rounded to 32: a far position (a frame number
 // of 10^5) keeps its angle, where a 32-bit product would be off by a hundredth of a radian.
@@ -20,9 +20,19 @@ struct rp_args {
     u32 tokens, n, heads[2], d, pairs, tok, units;   // tok: tokens of a workgroup, units: pieces of a head
     int axes;
     float sign;
+    bool past;
 };
 
 template <typename T, int VEC> struct rp_piece { T v[VEC]; };
+// past: results that no cache would hold until they are read (with the inputs more than the 256 MB of the last one) are written around
+// it: 16 x 2000, 16 heads of 80 fp32 73.5 -> 70 us, 4 x 30400, 20 heads of 128 bf16 218 -> 212
+template <typename P, typename T> __device__ __forceinline__ void rp_put(T *y, const P &o, bool past)
+{
+    if constexpr (sizeof(P) == 16) {
+        if (past) { __builtin_nontemporal_store(__builtin_bit_cast(rp_u4, o), (rp_u4 *)y); return; }
+    }
+    *(P *)y = o;
+}
 
 // a piece: VEC pairs (halves) or VEC values (neighbours) that turn, or VEC values behind the turned ones, copied as they are
 template <typename T, typename P, int VEC, bool HALVES>
@@ -62,11 +72,11 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
                     o.v[e] = (T)fmaf(pv, k.x, -(qv * k.y));
                     s.v[e] = (T)fmaf(pv, k.y, qv * k.x);
                 }
-                *(piece *)(y + j) = o;
-                *(piece *)(y + a.pairs + j) = s;
+                rp_put(y + j, o, a.past);
+                rp_put(y + a.pairs + j, s, a.past);
             } else {
                 const u32 j = 2 * a.pairs + (u - turning) * VEC;
-                *(piece *)(y + j) = *(const piece *)(x + j);
+                rp_put(y + j, *(const piece *)(x + j), a.past);
             }
         } else {
             const u32 j = u * VEC;
@@ -80,7 +90,7 @@ __global__ __launch_bounds__(256) void k_rope_axes(const rp_args a)
                     p.v[e + 1] = (T)fmaf(pv, k.y, qv * k.x);
                 }
             }
-            *(piece *)(y + j) = p;
+            rp_put(y + j, p, a.past);
         }
     }
 }
@@ -136,6 +146,7 @@ extern "C" int dg_rope_axes(const dg_rope_shape *s, const void *q, const void *k
     for (int i = 0; i < 3; ++i) { a.xs[0][i] = s->q_stride[i]; a.xs[1][i] = s->k_stride[i]; }
     a.ps[0] = s->pos_stride[0]; a.ps[1] = s->pos_stride[1];
     a.tokens = (u32)tokens; a.n = (u32)s->n; a.heads[0] = (u32)s->q_heads; a.heads[1] = (u32)s->k_heads;
+    a.past = tokens * (s->q_heads + s->k_heads) * s->d * (s->dtype == DG_F32 ? 4 : 2) > (1ll << 27);
     a.d = (u32)s->d; a.pairs = (u32)s->pairs; a.axes = (int)s->axes; a.sign = inverse ? -1.f : 1.f;
     const bool halves = s->pairing == DG_ROPE_HALVES, p64 = s->pos_dtype == DG_F64;
     hipStream_t st = (hipStream_t)stream;
