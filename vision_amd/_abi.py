@@ -172,21 +172,6 @@ def ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else None
 
 
-class on_device:
-    """torch.cuda.device(device) that costs nothing where it already is the current one"""
-
-    def __init__(self, device):
-        self.other = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.other is not None:
-            self.other.__enter__()
-
-    def __exit__(self, *exc):
-        if self.other is not None:
-            self.other.__exit__(*exc)
-
-
 # scratch, grown on demand (the C ABI allocates nothing).  One buffer per (device, stream): calls in flight on different
 # streams must not share masks, tickets or RoI lists (INTEGRATION.md section 3).  A buffer is allocated while its stream
 # is current, so the caching allocator hands a replaced buffer's memory out again only in that stream's order.
@@ -214,4 +199,6 @@ def to_dev(x, dtype, device):
     """Host arrays / CPU tensors are copied in; GPU tensors are used in place (contiguous)."""
     if not isinstance(x, torch.Tensor):
         x = torch.as_tensor(x)
+    elif x.dtype == dtype and x.device == device and x.is_contiguous():
+        return x
     return x.to(device=device, dtype=dtype).contiguous()

@@ -152,10 +152,13 @@ def rope_axes(q, k, pos, plan):
     are copied in and the results back."""
     dev = ops._abi.device_of(q, k)
     was_cpu = not (q.is_cuda or k.is_cuda)
-    pos = torch.as_tensor(pos).to(dev)
+    if not isinstance(pos, torch.Tensor) or pos.device != dev:
+        pos = torch.as_tensor(pos, device=dev)
     if pos.requires_grad:
         raise ValueError("rope_axes: positions have no gradient here; detach them")
-    q, k = _RopeFn.apply(q.to(dev), k.to(dev), pos, plan, False)
+    if not (q.device == dev and k.device == dev):
+        q, k = q.to(dev), k.to(dev)
+    q, k = _RopeFn.apply(q, k, pos, plan, False)
     return (q.cpu(), k.cpu()) if was_cpu else (q, k)
 
 

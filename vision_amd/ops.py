@@ -351,10 +351,26 @@ def kmeans_labels_i32(labels_u8):
 
 
 # ------------------------------------------------------------------ RoI head: attention
-def _scratch(nbytes, dev):
-    """Scratch of one call, from the caching allocator in the current stream's order: captured graphs and calls on other
-    streams never share it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+def _scratch(nbytes, like):
+    """Scratch of one call on a tensor's device, from the caching allocator in the current stream's order: captured graphs and
+    calls on other streams never share it."""
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+def _call(dev, fn, *args):
+    """an entry point on its tensors' device, which mostly is the current one"""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args)
+    if rc:
+        check(rc)
+
+
+def _empty_like(t):
+    """half the time of torch.empty(t.shape, dtype=..., device=...), which a small call spends several times"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _at(t):
@@ -414,7 +430,8 @@ def _attn_args(q, k, v, q_counts, k_counts, mask):
     qc, kc = _counts(q_counts, B, dev, "q_counts"), _counts(k_counts, B, dev, "k_counts")
     if mask is None:
         return dev, _vec16(q), _vec16(k), _vec16(v), qc, kc, None, 0, (0, 0)
-    mask = mask.to(dev) if isinstance(mask, torch.Tensor) else torch.as_tensor(mask, device=dev)
+    if not isinstance(mask, torch.Tensor) or mask.device != dev:
+        mask = torch.as_tensor(mask, device=dev)
     if mask.dtype not in (torch.bool, torch.uint8):
         raise ValueError("roi_attention: mask must be bool (or uint8: not 0 = may be seen)")
     if mask.dim() == 2:
@@ -440,13 +457,12 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None, 
 def _attn_forward(args, scale, keep_rest):
     dev, q, k, v, qc, kc, mask, masks, ms = args
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, None if scale is None else float(scale), q.dtype, 0)
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((s.batch, s.q_heads, s.nq), dtype=torch.float32, device=dev)
-    rest = torch.empty(q.shape, dtype=q.dtype, device=dev) if keep_rest and q.dtype == torch.bfloat16 else None
-    ws = _scratch(nbytes, dev)
-    with _abi.on_device(dev):
-        check(load().dg_roi_attn_fwd(s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(qc), _at(kc), _at(mask), out.data_ptr(), lse.data_ptr(), _at(rest), _at(ws),
-                                     nbytes, _stream(dev)))
+    out = _empty_like(q)
+    lse = q.new_empty((s.batch, s.q_heads, s.nq), dtype=torch.float32)
+    rest = _empty_like(q) if keep_rest and q.dtype == torch.bfloat16 else None
+    ws = _scratch(nbytes, q)
+    _call(dev, load().dg_roi_attn_fwd, s, q.data_ptr(), k.data_ptr(), v.data_ptr(), _at(qc), _at(kc), _at(mask), out.data_ptr(), lse.data_ptr(), _at(rest),
+          _at(ws), nbytes, _stream(dev))
     return out, lse, rest
 
 
@@ -473,13 +489,11 @@ def _attn_backward(args, g, out, lse, rest, scale, need_q, need_kv):
     dev, q, k, v, qc, kc, mask, masks, ms = args
     g = _vec16(g)
     s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, None if scale is None else float(scale), q.dtype, 1)
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if need_q else None
-    dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
-    dv = torch.empty(k.shape, dtype=q.dtype, device=dev) if need_kv else None
-    ws = _scratch(nbytes, dev)
-    with _abi.on_device(dev):
-        check(load().dg_roi_attn_bwd(s, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _at(rest), _at(qc), _at(kc), _at(mask),
-                                     _at(dq), _at(dk), _at(dv), _at(ws), nbytes, _stream(dev)))
+    dq = _empty_like(q) if need_q else None
+    dk, dv = (_empty_like(k), _empty_like(k)) if need_kv else (None, None)
+    ws = _scratch(nbytes, q)
+    _call(dev, load().dg_roi_attn_bwd, s, g.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _at(rest), _at(qc), _at(kc),
+          _at(mask), _at(dq), _at(dk), _at(dv), _at(ws), nbytes, _stream(dev))
     return dq, dk, dv
 
 
@@ -535,7 +549,8 @@ def rope_axes(q, pos, plan, k=None, inverse=False):
     dev = _abi.device_of(q, k, pos)
     q = _dense_last(q if q.device == dev else q.to(dev))
     k = None if k is None else _dense_last(k if k.device == dev else k.to(dev))
-    pos = pos.to(dev) if isinstance(pos, torch.Tensor) else torch.as_tensor(pos, device=dev)
+    if not isinstance(pos, torch.Tensor) or pos.device != dev:
+        pos = torch.as_tensor(pos, device=dev)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
         raise ValueError("rope_axes: q (B,N,Hq,D), k (B,N,Hk,D) of one type")
     if q.dtype not in _abi.TYPES:
@@ -553,18 +568,18 @@ def rope_axes(q, pos, plan, k=None, inverse=False):
     pos = _dense_last(pos)
     s = _rope_shape(q.shape, 0 if k is None else k.shape[2], plan.pairs, plan.axes, q.stride(), (0, 0, 0) if k is None else k.stride(),
                     pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2), q.dtype, pos.dtype == torch.float64, plan.pairing)
-    out_q = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    out_k = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=dev)
-    with _abi.on_device(dev):
-        check(load().dg_rope_axes(s, q.data_ptr(), _at(k), pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), 1 if inverse else 0, out_q.data_ptr(),
-                                  _at(out_k), _stream(dev)))
+    out_q = _empty_like(q)
+    out_k = None if k is None else _empty_like(k)
+    _call(dev, load().dg_rope_axes, s, q.data_ptr(), _at(k), pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), 1 if inverse else 0, out_q.data_ptr(),
+          _at(out_k), _stream(dev))
     return out_q if k is None else (out_q, out_k)
 
 
 # ------------------------------------------------------------------ RoI head: log probabilities of labels
 def _logits(z, labels, what):
     dev = _abi.device_of(z, labels)
-    z = z.to(dev) if isinstance(z, torch.Tensor) else torch.as_tensor(z, device=dev)
+    if not isinstance(z, torch.Tensor) or z.device != dev:
+        z = torch.as_tensor(z, device=dev)
     if z.dim() != 2 or z.shape[1] < 1 or z.dtype not in _abi.TYPES:
         raise ValueError(f"{what}: logits must be (n,C), C >= 1, float32, bfloat16 or float16")
     z = _dense_last(z)
@@ -583,20 +598,23 @@ def class_logprobs(logits, labels=None, top=0):
     return _logprobs(*_logits(logits, labels, "class_logprobs"), int(top))
 
 
+@functools.lru_cache(maxsize=1024)
+def _logprobs_scratch(n, c, top):
+    return load().dg_class_logprobs_workspace_bytes(n, c, top)
+
+
 def _logprobs(dev, z, y, top):
     n, c = z.shape
-    f32 = dict(dtype=torch.float32, device=dev)
     if not 0 <= top <= min(32, c):
         raise ValueError("class_logprobs: top must be 0 to 32 and no more than the classes")
-    logp = torch.empty((n,), **f32) if y is not None else None
-    entropy, norm = torch.empty((n,), **f32), torch.empty((n, 2), **f32)
-    best, index = torch.empty((n, top), **f32), torch.empty((n, top), dtype=torch.int64, device=dev)
-    lib = load()
-    nbytes = lib.dg_class_logprobs_workspace_bytes(n, c, top)
-    ws = _scratch(nbytes, dev)
-    with _abi.on_device(dev):
-        check(lib.dg_class_logprobs(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), top, _at(logp), entropy.data_ptr(), norm.data_ptr(),
-                                    best.data_ptr(), index.data_ptr(), None, _at(ws), nbytes, _stream(dev)))
+    f32 = torch.float32
+    entropy, norm = z.new_empty(n, dtype=f32), z.new_empty((n, 2), dtype=f32)
+    logp = _empty_like(entropy) if y is not None else None
+    best, index = z.new_empty((n, top), dtype=f32), z.new_empty((n, top), dtype=torch.int64)
+    nbytes = _logprobs_scratch(n, c, top)
+    ws = _scratch(nbytes, z)
+    _call(dev, load().dg_class_logprobs, z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), top, _at(logp), entropy.data_ptr(), norm.data_ptr(),
+          best.data_ptr(), index.data_ptr(), None, _at(ws), nbytes, _stream(dev))
     return logp, entropy, norm, best, index
 
 
@@ -615,8 +633,7 @@ def class_logprobs_backward(grad_logp, grad_entropy, logits, labels, norm, entro
 
 def _logprobs_backward(dev, z, y, norm, entropy, g, gh):
     n, c = z.shape
-    dz = torch.empty((n, c), dtype=z.dtype, device=dev)
-    with _abi.on_device(dev):
-        check(load().dg_class_logprobs_bwd(z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), norm.data_ptr(), entropy.data_ptr(),
-                                           _at(g) if y is not None else None, _at(gh), dz.data_ptr(), _stream(dev)))
+    dz = _empty_like(z)
+    _call(dev, load().dg_class_logprobs_bwd, z.data_ptr(), _abi.TYPES[z.dtype], _at(y), n, c, z.stride(0), norm.data_ptr(), entropy.data_ptr(),
+          _at(g) if y is not None else None, _at(gh), dz.data_ptr(), _stream(dev))
     return dz
