@@ -96,6 +96,15 @@ def nms(rects, scores):
 
 
 # ------------------------------------------------------------------ RoI head
+def _once(backward):
+    """torch's once_differentiable, without its cost where no graph of the gradient is asked for"""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 class _RoIAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_counts, k_counts, mask, scale):
@@ -106,7 +115,7 @@ class _RoIAttentionFn(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad_out):
         *args, out, lse, rest = ctx.saved_tensors
         dev, masks, ms, scale = ctx.rest
@@ -130,21 +139,21 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None):
 class _RopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, plan, inverse):
+        args = ops._rope_args(q, k, pos, plan)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(pos)
-        ctx.plan, ctx.inverse = plan, inverse
-        return ops.rope_axes(q, pos, plan, k=k, inverse=inverse)
+        ctx.save_for_backward(args[3])
+        ctx.rest = args[0], args[4], inverse
+        return ops._rope_turn(*args, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         (pos,) = ctx.saved_tensors
-        if dq is not None and dk is not None:
-            dq, dk = _RopeFn.apply(dq, dk, pos, ctx.plan, not ctx.inverse)
-        elif dq is not None:
-            dq = _RopeFn.apply(dq, dq[:, :, :0], pos, ctx.plan, not ctx.inverse)[0]
-        elif dk is not None:
-            dk = _RopeFn.apply(dk[:, :, :0], dk, pos, ctx.plan, not ctx.inverse)[1]
-        return dq, dk, None, None, None
+        dev, plan, inverse = ctx.rest
+        if dq is None and dk is None:
+            return None, None, None, None, None
+        g, h = dk[:, :, :0] if dq is None else dq, dq[:, :, :0] if dk is None else dk
+        g, h = _RopeFn.apply(g, h, pos, plan, not inverse) if torch.is_grad_enabled() else ops._rope_turn(dev, g, h, pos, plan, not inverse)
+        return None if dq is None else g, None if dk is None else h, None, None, None
 
 
 def rope_axes(q, k, pos, plan):
@@ -173,7 +182,7 @@ class _ClassLogprobsFn(torch.autograd.Function):
         return logp, entropy, best, index
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, g, gh, _best, _index):
         z, y, norm, entropy = ctx.saved_tensors
         if g is None and gh is None:

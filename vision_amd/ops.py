@@ -546,9 +546,14 @@ def rope_axes(q, pos, plan, k=None, inverse=False):
     tokens as plan says; inverse: back, which is the gradient.  float32, bfloat16 or float16; values behind the plan's pairs are
     copied; float32 or float64 positions are used as they are, whole numbers as float64.  -> the turned q, or (q, k).  No
     reference counterpart.  For a gradient: fast_rcnn.rope_axes."""
+    q, k = _rope_turn(*_rope_args(q, k, pos, plan), inverse)
+    return q if k is None else (q, k)
+
+
+def _rope_args(q, k, pos, plan):
     dev = _abi.device_of(q, k, pos)
-    q = _dense_last(q if q.device == dev else q.to(dev))
-    k = None if k is None else _dense_last(k if k.device == dev else k.to(dev))
+    q = q if q.device == dev else q.to(dev)
+    k = k if k is None or k.device == dev else k.to(dev)
     if not isinstance(pos, torch.Tensor) or pos.device != dev:
         pos = torch.as_tensor(pos, device=dev)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3] or k.dtype != q.dtype)):
@@ -561,18 +566,22 @@ def rope_axes(q, pos, plan, k=None, inverse=False):
         pos = pos.to(torch.float64)
     elif pos.dtype not in (torch.float32, torch.float64):
         pos = pos.to(torch.float32)
-    B, N, Hq, D = q.shape
+    B, N = q.shape[:2]
     plan = plan.to(dev)
     if pos.dim() not in (2, 3) or tuple(pos.shape[-2:]) != (N, plan.axes) or (pos.dim() == 3 and pos.shape[0] not in (1, B)):
         raise ValueError(f"rope_axes: pos must be (B,N,{plan.axes}) or (N,{plan.axes})")
-    pos = _dense_last(pos)
+    return dev, q, k, _dense_last(pos), plan
+
+
+def _rope_turn(dev, q, k, pos, plan, inverse):
+    q, k = _dense_last(q), None if k is None else _dense_last(k)
     s = _rope_shape(q.shape, 0 if k is None else k.shape[2], plan.pairs, plan.axes, q.stride(), (0, 0, 0) if k is None else k.stride(),
                     pos.stride(0) if pos.dim() == 3 and pos.shape[0] > 1 else 0, pos.stride(-2), q.dtype, pos.dtype == torch.float64, plan.pairing)
     out_q = _empty_like(q)
     out_k = None if k is None else _empty_like(k)
     _call(dev, load().dg_rope_axes, s, q.data_ptr(), _at(k), pos.data_ptr(), plan.turns.data_ptr(), plan.axis.data_ptr(), 1 if inverse else 0, out_q.data_ptr(),
           _at(out_k), _stream(dev))
-    return out_q if k is None else (out_q, out_k)
+    return out_q, out_k
 
 
 # ------------------------------------------------------------------ RoI head: log probabilities of labels
