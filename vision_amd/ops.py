@@ -394,9 +394,14 @@ def _strides_fit(shape, strides, e):
 
 def _vec16(t):
     """t, or a copy of it, such that _strides_fit and its first value lies on a multiple of 16 bytes"""
-    if t.data_ptr() % 16 == 0 and _strides_fit(t.shape, t.stride(), t.element_size()):
-        return t
+    if t.data_ptr() % 16 == 0 and ((t.is_contiguous() and t.numel()) or _strides_fit(t.shape, t.stride(), t.element_size())):
+        return t                                 # dense with a head size that the library takes: 16 bytes at a time
     return t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t):
+    """for a key: None says the same in less time where a tensor is dense"""
+    return None if t.is_contiguous() else t.stride()
 
 
 def _counts(c, B, dev, what):
@@ -410,9 +415,11 @@ def _counts(c, B, dev, what):
 
 @functools.lru_cache(maxsize=1024)
 def _attn_plan(q_shape, k_shape, q_stride, k_stride, v_stride, g_stride, masks, mask_stride, scale, dtype, backward):
-    """the call's description for the library and its workspace's size: by shapes alone"""
+    """the call's description for the library and its workspace's size: by shapes alone; a stride None: dense"""
     B, Nq, Hq, D = q_shape
-    s = _abi.AttnShape(B, Nq, k_shape[1], Hq, k_shape[2], D, *q_stride[:3], *k_stride[:3], *v_stride[:3], *g_stride[:3], masks, *mask_stride[:2],
+    dense = [(shape[1] * shape[2] * D, shape[2] * D, D) for shape in (q_shape, k_shape)]
+    strides = [(d if st is None else st)[:3] for st, d in ((q_stride, dense[0]), (k_stride, dense[1]), (v_stride, dense[1]), (g_stride, dense[0]))]
+    s = _abi.AttnShape(B, Nq, k_shape[1], Hq, k_shape[2], D, *strides[0], *strides[1], *strides[2], *strides[3], masks, *mask_stride[:2],
                        D ** -0.5 if scale is None else scale, _abi.TYPES[dtype])
     return s, load().dg_roi_attn_workspace_bytes(s, backward)
 
@@ -456,7 +463,7 @@ def roi_attention(q, k, v, q_counts=None, k_counts=None, mask=None, scale=None, 
 
 def _attn_forward(args, scale, keep_rest):
     dev, q, k, v, qc, kc, mask, masks, ms = args
-    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), (0, 0, 0), masks, ms, None if scale is None else float(scale), q.dtype, 0)
+    s, nbytes = _attn_plan(q.shape, k.shape, _strides(q), _strides(k), _strides(v), None, masks, ms, None if scale is None else float(scale), q.dtype, 0)
     out = _empty_like(q)
     lse = q.new_empty((s.batch, s.q_heads, s.nq), dtype=torch.float32)
     rest = _empty_like(q) if keep_rest and q.dtype == torch.bfloat16 else None
@@ -488,7 +495,7 @@ def roi_attention_backward(grad_out, q, k, v, out, lse, q_counts=None, k_counts=
 def _attn_backward(args, g, out, lse, rest, scale, need_q, need_kv):
     dev, q, k, v, qc, kc, mask, masks, ms = args
     g = _vec16(g)
-    s, nbytes = _attn_plan(q.shape, k.shape, q.stride(), k.stride(), v.stride(), g.stride(), masks, ms, None if scale is None else float(scale), q.dtype, 1)
+    s, nbytes = _attn_plan(q.shape, k.shape, _strides(q), _strides(k), _strides(v), _strides(g), masks, ms, None if scale is None else float(scale), q.dtype, 1)
     dq = _empty_like(q) if need_q else None
     dk, dv = (_empty_like(k), _empty_like(k)) if need_kv else (None, None)
     ws = _scratch(nbytes, q)
