@@ -944,3 +944,29 @@ def test_roi_attention_rest():
     assert ops.roi_attention(q, q, q, rest=True)[2] is None
     with pytest.raises(ValueError, match="rest"):
         ops.roi_attention_backward(q, q, q, q, *ops.roi_attention(q, q, q), rest=q)
+
+
+@pytest.mark.gpu
+def test_gradients_of_gradients_and_of_broadcast_inputs():
+    """A second derivative that is not there is refused, not wrong; a key set expanded over the batch gets the sum of its gradients; a
+    gradient that comes expanded (of a sum) is taken like a dense one."""
+    from vision_amd import fast_rcnn
+    g = _gen(95)
+    q = torch.randn((3, 40, 2, 32), generator=g).cuda().requires_grad_(True)
+    k, v = (torch.randn((1, 50, 2, 32), generator=g).cuda().requires_grad_(True) for _ in range(2))
+    out = fast_rcnn.roi_attention(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1))
+    wide = [t.detach().expand(3, -1, -1, -1).contiguous().requires_grad_(True) for t in (k, v)]
+    ref = fast_rcnn.roi_attention(q, *wide)
+    assert torch.equal(out, ref)
+    a = torch.autograd.grad(out.sum(), (q, k, v))
+    b = torch.autograd.grad(ref, (q, *wide), torch.ones_like(ref))
+    assert torch.equal(a[0], b[0])
+    for x, y in zip(a[1:], b[1:]):                # a sum of three terms of 32 bits, in any order
+        assert bool(((x - y.double().sum(0, keepdim=True)).abs() <= 4 * E32 * y.abs().sum(0, keepdim=True)).all())
+    z = torch.randn((6, 9), generator=g).cuda().requires_grad_(True)
+    r = fast_rcnn.class_logprobs(z, torch.arange(6), 2)
+    for y, x in ((fast_rcnn.roi_attention(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1)), q), (r.logp, z)):
+        w = torch.ones_like(y).requires_grad_(True)
+        (dx,) = torch.autograd.grad(y, (x,), w, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            dx.sum().backward()
