@@ -981,7 +981,12 @@ static at_args<T> at_fill(const dg_attn_shape *s, const void *q, const void *k, 
     at_args<T> a = {};
     a.q = (const T *)q; a.k = (const T *)k; a.v = (const T *)v;
     a.qc = qc; a.kc = kc;
-    for (int i = 0; i < 3; ++i) { a.qs[i] = s->q_stride[i]; a.ks[i] = s->k_stride[i]; a.vs[i] = s->v_stride[i]; a.gs[i] = s->g_stride[i]; }
+    // an axis of one has no stride: whatever the caller's is, it would enter the loaders' 32-bit offsets of rows that are not there
+    const int64_t qn[3] = {s->batch, s->nq, s->q_heads}, kn[3] = {s->batch, s->nk, s->k_heads};
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = qn[i] > 1 ? s->q_stride[i] : 0; a.gs[i] = qn[i] > 1 ? s->g_stride[i] : 0;
+        a.ks[i] = kn[i] > 1 ? s->k_stride[i] : 0; a.vs[i] = kn[i] > 1 ? s->v_stride[i] : 0;
+    }
     a.batch = (int)s->batch; a.nq = (int)s->nq; a.nk = (int)s->nk; a.hq = (int)s->q_heads; a.hk = (int)s->k_heads; a.d = (int)s->d;
     a.scale = s->scale;
     a.c = (float)((double)s->scale * 1.4426950408889634);
