@@ -16,6 +16,7 @@
 // contraction index may be permuted as long as the first operand, read transposed from LDS, is permuted the same way.
 #include "common.hpp"
 #include <math.h>
+#include <type_traits>
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -543,9 +544,12 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_join(const at_args<T> a, in
 
 // ------------------------------------------------------------------ backward
 // How ds enters its products in bf16.  The sum of ds over a row's keys is 0, so dq and dk are what is left of larger terms, the more so
-// the fewer keys a row sees.  With few keys (and under a pair mask, which may leave few) ds goes in as two parts, 16 bits; elsewhere one
-// rounding to 8 bits is of no more weight than that of the result.
-enum { AT_PLAIN, AT_FINE, AT_MASKED };
+// the fewer keys a row sees.  In images of up to AT_FEW keys (and under a pair mask, which may leave few) ds goes in as two parts, 16 bits;
+// elsewhere one rounding to 8 bits is of no more weight than that of the result.  AT_COUNTED: each image's count decides, whatever the
+// padded size: the kernel holds both walks, whole, so that neither's registers bind the other's.
+enum { AT_PLAIN, AT_FINE, AT_COUNTED, AT_MASKED };
+#define AT_FEW 512
+#define AT_CUT(nk) (MODE == AT_COUNTED ? (nk) <= AT_FEW : MODE != AT_PLAIN)
 // delta_i = do_i . o_i and the rows' log-sums in base 2; a row that sees nothing gets +inf there, so that its p is 0.  From the output as
 // rounded to bf16 alone delta would be off by 2^-8 of its terms, which where few keys are seen is as much as ds itself (one key: ds is 0);
 // with what rounding took, by 2^-16.  Bound by memory: 8 images of 1000 to 2000 rows x 8 x 64 bf16: 11 us, 3.6 TB/s.
@@ -595,7 +599,7 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_dq(const at_args<T> a)
 {
-    constexpr bool MASK = MODE == AT_MASKED, FINE = MODE != AT_PLAIN;
+    constexpr bool MASK = MODE == AT_MASKED;
     typedef typename at_vec<T>::quad quad;
     constexpr int NG = DP / 16, NB = DP / 32, KT = at_shape<T, DP>::KT_Q, U = KT / 32;
     typedef at_tile<T, DP, KT> tile;
@@ -618,96 +622,100 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
     const int r = (tix * AT_WAVES + wave) * 32 + (lane & 31);
     const bool live = r < R;
     const int gh = live ? r / nq : 0, n = live ? r % nq : 0, hq = hk * G + gh;
-    const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2], *gp = a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2];
-    at_op<T> qf[NG], gf[NG];
+    auto walk = [&](auto cut) {                   // cut: ds goes in as two parts
+        const T *qp = a.q + b * a.qs[0] + n * a.qs[1] + hq * a.qs[2], *gp = a.g + b * a.gs[0] + n * a.gs[1] + hq * a.gs[2];
+        at_op<T> qf[NG], gf[NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const int d = (2 * g + h) * 8;
-        at_read(qp + d, live && d < a.d, qf[g]);
-        at_read(gp + d, live && d < a.d, gf[g]);
-    }
-    const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
-    const f32x2 stat = live ? a.stat[at] : (f32x2){INFINITY, 0.f};
-    const float lse2 = stat[0];
-    const u32 *mp = MASK ? a.bits + b * a.bs + (int64_t)n * a.words : nullptr;
-
-    const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
-    const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
-    u32x4 kr[kl.NL], vr[kl.NL];
-    auto load = [&](int kb) {
-        kl.load(kr, kb, k1 - kb);
-        vl.load(vr, kb, k1 - kb);
-    };
-    auto store = [&](int buf) {
-        if (MASK) {
-#pragma unroll
-            for (int i = 0; i < kl.NL; ++i)
-                if (at_scrub<T>(kr[i])) vr[i] = AT_NAN4;    // dp of that key becomes NaN
+        for (int g = 0; g < NG; ++g) {
+            const int d = (2 * g + h) * 8;
+            at_read(qp + d, live && d < a.d, qf[g]);
+            at_read(gp + d, live && d < a.d, gf[g]);
         }
-        kl.store(lds[buf][0], kr);
-        vl.store(lds[buf][1], vr);
-    };
+        const int64_t at = ((int64_t)b * a.hq + hq) * a.nq + n;
+        const f32x2 stat = live ? a.stat[at] : (f32x2){INFINITY, 0.f};
+        const float lse2 = stat[0];
+        const u32 *mp = MASK ? a.bits + b * a.bs + (int64_t)n * a.words : nullptr;
 
-    f32x16 o[NB];
+        const int k0 = sp * a.per, k1 = min(nk, k0 + a.per);
+        const at_loader<T, DP, KT> kl(a.k + b * a.ks[0] + hk * a.ks[2], a.ks[1], a.d), vl(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], a.d);
+        u32x4 kr[kl.NL], vr[kl.NL];
+        auto load = [&](int kb) {
+            kl.load(kr, kb, k1 - kb);
+            vl.load(vr, kb, k1 - kb);
+        };
+        auto store = [&](int buf) {
+            if (MASK) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
-    u32 mw[U], mnext[U];                          // MASK: this tile's words and the next one's
-    if (k0 < k1) {
-        load(k0);
-        store(0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) mw[u] = MASK ? at_word(mp, k0 + 32 * u, k1) : 0;
-    }
-    __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
-    __syncthreads();
-    int buf = 0;
-    for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
-        const bool more = kb + KT < k1;
-        if (more) load(kb + KT);
-#pragma unroll
-        for (int u = 0; u < U; ++u) mnext[u] = MASK ? at_word(mp, kb + KT + 32 * u, k1) : 0;
-        const char *K = lds[buf][0], *V = lds[buf][1];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            f32x16 s = (f32x16)(0.f), dp = (f32x16)(stat[1]);
-            AT_PRIO(2);
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                s = at_mma(tile::row(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
-                dp = at_mma(tile::row(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
+                for (int i = 0; i < kl.NL; ++i)
+                    if (at_scrub<T>(kr[i])) vr[i] = AT_NAN4;    // dp of that key becomes NaN
             }
-            AT_PRIO(0);
-            const int left = k1 - kb - u * 32;
-            const u32 w = (MASK ? mw[u] : left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u) >> (4 * h);
-            AT_PART(DP == 128);
+            kl.store(lds[buf][0], kr);
+            vl.store(lds[buf][1], vr);
+        };
+
+        f32x16 o[NB];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse2)) * dp[e];
-                if (MASK || !more) ds = w & (1u << (8 * (e >> 2) + (e & 3))) ? ds : 0.f;
-                s[e] = ds;
-            }
-            AT_PRIO(1);
-            tile::template acc_t<FINE>(o, K, u * 32, s, lane);
-            AT_PRIO(0);
+        for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
+        u32 mw[U], mnext[U];                          // MASK: this tile's words and the next one's
+        if (k0 < k1) {
+            load(k0);
+            store(0);
+#pragma unroll
+            for (int u = 0; u < U; ++u) mw[u] = MASK ? at_word(mp, k0 + 32 * u, k1) : 0;
         }
-        if (more) store(buf ^ 1);
-#pragma unroll
-        for (int u = 0; u < U; ++u) mw[u] = mnext[u];
+        __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
         __syncthreads();
-    }
-    if (!live) return;
-    float *po = a.part + (((int64_t)b * a.hq + hq) * a.nq + n) * a.splits * a.d + (int64_t)sp * a.d;
-    T *op = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
+        int buf = 0;
+        for (int kb = k0; kb < k1; kb += KT, buf ^= 1) {
+            const bool more = kb + KT < k1;
+            if (more) load(kb + KT);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+            for (int u = 0; u < U; ++u) mnext[u] = MASK ? at_word(mp, kb + KT + 32 * u, k1) : 0;
+            const char *K = lds[buf][0], *V = lds[buf][1];
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int d = i * 32 + 2 * e + 4 * h;
-            const f32x4 x = (f32x4){o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]} * a.scale;
-            if (d >= a.d) continue;
-            if (a.splits > 1) *(f32x4 *)(po + d) = x;
-            else *(quad *)(op + d) = __builtin_convertvector(x, quad);
+            for (int u = 0; u < U; ++u) {
+                f32x16 s = (f32x16)(0.f), dp = (f32x16)(stat[1]);
+                AT_PRIO(2);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    s = at_mma(tile::row(K, u * 32 + (lane & 31), 2 * g + h), qf[g], s);
+                    dp = at_mma(tile::row(V, u * 32 + (lane & 31), 2 * g + h), gf[g], dp);
+                }
+                AT_PRIO(0);
+                const int left = k1 - kb - u * 32;
+                const u32 w = (MASK ? mw[u] : left >= 32 ? ~0u : left > 0 ? (1u << left) - 1 : 0u) >> (4 * h);
+                AT_PART(DP == 128);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    float ds = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -lse2)) * dp[e];
+                    if (MASK || !more) ds = w & (1u << (8 * (e >> 2) + (e & 3))) ? ds : 0.f;
+                    s[e] = ds;
+                }
+                AT_PRIO(1);
+                tile::template acc_t<decltype(cut)::value>(o, K, u * 32, s, lane);
+                AT_PRIO(0);
+            }
+            if (more) store(buf ^ 1);
+#pragma unroll
+            for (int u = 0; u < U; ++u) mw[u] = mnext[u];
+            __syncthreads();
         }
+        if (!live) return;
+        float *po = a.part + (((int64_t)b * a.hq + hq) * a.nq + n) * a.splits * a.d + (int64_t)sp * a.d;
+        T *op = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = i * 32 + 2 * e + 4 * h;
+                const f32x4 x = (f32x4){o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]} * a.scale;
+                if (d >= a.d) continue;
+                if (a.splits > 1) *(f32x4 *)(po + d) = x;
+                else *(quad *)(op + d) = __builtin_convertvector(x, quad);
+            }
+    };
+    if (AT_CUT(nk)) walk(std::true_type());
+    else walk(std::false_type());
 }
 
 #define AT_RT 32
@@ -718,7 +726,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(AT_THREADS, (MODE == AT_MASKED && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
-    constexpr bool MASK = MODE == AT_MASKED, FINE = MODE != AT_PLAIN;
+    constexpr bool MASK = MODE == AT_MASKED;
     typedef typename at_vec<T>::quad quad;
     constexpr int NG = DP / 16, NB = DP / 32, KT = AT_RT;
     typedef at_tile<T, DP, KT> tile;
@@ -727,6 +735,7 @@ __global__ __launch_bounds__(AT_THREADS, (MODE == AT_MASKED && at_shape<T, DP>::
     constexpr bool LEAN = sizeof(T) == 2 && DP >= 64;
     constexpr bool VL = sizeof(T) == 2 && DP == 128;          // V stays in LDS: its registers are what would keep a second wave off the SIMD
     __shared__ __attribute__((aligned(16))) char vt[VL ? 32 * AT_WAVES * tile::RB : 16];
+    __shared__ __attribute__((aligned(16))) u32 mws[2][AT_WAVES][MASK ? KT : 4];
 
     const int id = at_xcd_id(a.tiles * a.splits), tix = id % a.tiles, sp = (id / a.tiles) % a.splits, bh = id / a.tiles / a.splits;
     const int b = at_image(bh / a.hk, a.batch, a.qc, a.nq), hk = bh % a.hk, G = a.hq / a.hk;
@@ -737,127 +746,130 @@ __global__ __launch_bounds__(AT_THREADS, (MODE == AT_MASKED && at_shape<T, DP>::
     const int key = (tix * AT_WAVES + wave) * 32 + (lane & 31);
     const bool live = key < nk;
 
-    const T *kp = a.k + b * a.ks[0] + (live ? key : 0) * a.ks[1] + hk * a.ks[2], *vp = a.v + b * a.vs[0] + (live ? key : 0) * a.vs[1] + hk * a.vs[2];
-    at_op<T> kf[NG], vf[VL ? 1 : NG];
+    auto walk = [&](auto cut) {                   // cut: ds goes in as two parts
+        const T *kp = a.k + b * a.ks[0] + (live ? key : 0) * a.ks[1] + hk * a.ks[2], *vp = a.v + b * a.vs[0] + (live ? key : 0) * a.vs[1] + hk * a.vs[2];
+        at_op<T> kf[NG], vf[VL ? 1 : NG];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        const int d = (2 * g + h) * 8;
-        at_op<T> x;
-        at_read(kp + d, live && d < a.d, kf[g]);
-        at_read(vp + d, live && d < a.d, x);
-        if (VL) *(at_op<T> *)(vt + (wave * NG + g) * 1024 + lane * 16) = x;
-        else vf[VL ? 0 : g] = x;
-    }
+        for (int g = 0; g < NG; ++g) {
+            const int d = (2 * g + h) * 8;
+            at_op<T> x;
+            at_read(kp + d, live && d < a.d, kf[g]);
+            at_read(vp + d, live && d < a.d, x);
+            if (VL) *(at_op<T> *)(vt + (wave * NG + g) * 1024 + lane * 16) = x;
+            else vf[VL ? 0 : g] = x;
+        }
 
-    const int w0 = min(W, sp * a.per), w1 = min(W, w0 + a.per);
-    int wg = ht ? w0 / ht : 0, wn = ht ? w0 - wg * ht : 0;       // the next tile to load
-    u32x4 qr[at_loader<T, DP, KT, LEAN>::NL], gr[at_loader<T, DP, KT, LEAN>::NL];
-    const at_loader<T, DP, KT, LEAN> ql(a.q + b * a.qs[0] + hk * G * a.qs[2], a.qs[1], a.d), gl(a.g + b * a.gs[0] + hk * G * a.gs[2], a.gs[1], a.d);
-    __shared__ __attribute__((aligned(16))) u32 mws[2][AT_WAVES][MASK ? KT : 4];
-    const u32 *mp = MASK ? a.bits + b * a.bs : nullptr;
-    u64 sr = 0;
-    u32 mr = 0;
-    auto load = [&]() {
-        const int n0 = wn * KT, rows = nq - n0;
-        at_loader<T, DP, KT, LEAN> q1 = ql, g1 = gl;
-        q1.base += wg * a.qs[2];
-        g1.base += wg * a.gs[2];
-        q1.load(qr, n0, rows);
-        g1.load(gr, n0, rows);
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(a.stat + ((int64_t)b * a.hq + hk * G + wg) * a.nq + n0), 0, AT_OUT, 0x00027000);
-        // the rows' statistics; zeros behind the end, where q and grad_out are zeros too
-        sr = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(rs, (int)threadIdx.x < min(KT, rows) ? (int)threadIdx.x * 8 : AT_OUT, 0, 0));
-        if (MASK && threadIdx.x < KT * AT_WAVES) {   // the words of the tile's rows for each wave's keys
-            const int n = threadIdx.x / AT_WAVES, kw = tix * AT_WAVES + threadIdx.x % AT_WAVES;
-            mr = n < rows && kw < a.words ? mp[(int64_t)(n0 + n) * a.words + kw] : 0;
-        }
-        if (++wn == ht) { wn = 0; ++wg; }
-    };
-    auto store = [&](int buf) {
-        if (MASK) {                               // the row's log-sum already says NaN (k_attn_delta)
-#pragma unroll
-            for (int i = 0; i < ql.NL; ++i) {
-                at_scrub<T>(qr[i]);
-                at_scrub<T>(gr[i]);
+        const int w0 = min(W, sp * a.per), w1 = min(W, w0 + a.per);
+        int wg = ht ? w0 / ht : 0, wn = ht ? w0 - wg * ht : 0;       // the next tile to load
+        u32x4 qr[at_loader<T, DP, KT, LEAN>::NL], gr[at_loader<T, DP, KT, LEAN>::NL];
+        const at_loader<T, DP, KT, LEAN> ql(a.q + b * a.qs[0] + hk * G * a.qs[2], a.qs[1], a.d), gl(a.g + b * a.gs[0] + hk * G * a.gs[2], a.gs[1], a.d);
+        const u32 *mp = MASK ? a.bits + b * a.bs : nullptr;
+        u64 sr = 0;
+        u32 mr = 0;
+        auto load = [&]() {
+            const int n0 = wn * KT, rows = nq - n0;
+            at_loader<T, DP, KT, LEAN> q1 = ql, g1 = gl;
+            q1.base += wg * a.qs[2];
+            g1.base += wg * a.gs[2];
+            q1.load(qr, n0, rows);
+            g1.load(gr, n0, rows);
+            const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(a.stat + ((int64_t)b * a.hq + hk * G + wg) * a.nq + n0), 0, AT_OUT, 0x00027000);
+            // the rows' statistics; zeros behind the end, where q and grad_out are zeros too
+            sr = __builtin_bit_cast(u64, __builtin_amdgcn_raw_buffer_load_b64(rs, (int)threadIdx.x < min(KT, rows) ? (int)threadIdx.x * 8 : AT_OUT, 0, 0));
+            if (MASK && threadIdx.x < KT * AT_WAVES) {   // the words of the tile's rows for each wave's keys
+                const int n = threadIdx.x / AT_WAVES, kw = tix * AT_WAVES + threadIdx.x % AT_WAVES;
+                mr = n < rows && kw < a.words ? mp[(int64_t)(n0 + n) * a.words + kw] : 0;
             }
-        }
-        ql.store(lds[buf][0], qr);
-        gl.store(lds[buf][1], gr);
-        if (MASK && threadIdx.x < KT * AT_WAVES) mws[buf][threadIdx.x % AT_WAVES][threadIdx.x / AT_WAVES] = mr;
-        if (threadIdx.x < KT) {
-            st[buf][0][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[0];
-            st[buf][1][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[1];
-        }
-    };
+            if (++wn == ht) { wn = 0; ++wg; }
+        };
+        auto store = [&](int buf) {
+            if (MASK) {                               // the row's log-sum already says NaN (k_attn_delta)
+#pragma unroll
+                for (int i = 0; i < ql.NL; ++i) {
+                    at_scrub<T>(qr[i]);
+                    at_scrub<T>(gr[i]);
+                }
+            }
+            ql.store(lds[buf][0], qr);
+            gl.store(lds[buf][1], gr);
+            if (MASK && threadIdx.x < KT * AT_WAVES) mws[buf][threadIdx.x % AT_WAVES][threadIdx.x / AT_WAVES] = mr;
+            if (threadIdx.x < KT) {
+                st[buf][0][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[0];
+                st[buf][1][threadIdx.x] = __builtin_bit_cast(f32x2, sr)[1];
+            }
+        };
 
-    f32x16 ok[NB], ov[NB];
+        f32x16 ok[NB], ov[NB];
 #pragma unroll
-    for (int i = 0; i < NB; ++i) ok[i] = ov[i] = (f32x16)(0.f);
-    if (w0 < w1) {
-        load();
-        store(0);
-    }
-    __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
-    __syncthreads();
-    int buf = 0;
-    for (int w = w0; w < w1; ++w, buf ^= 1) {
-        const bool more = w + 1 < w1;
-        if (more) load();
-        const char *Q = lds[buf][0], *GO = lds[buf][1];
-        // the LDS addresses of a tile are formed anew in every turn: kept across the loop they would cost a wave of the SIMD
-        int ln = lane;
-        asm volatile("" : "+v"(ln));
-        const int lr = ln & 31, lh = ln >> 5;
-        f32x16 s = (f32x16)(0.f), dp;
-        AT_PRIO(2);
-#pragma unroll
-        for (int g = 0; g < NG; ++g) s = at_mma(tile::row(Q, lr, 2 * g + lh), kf[g], s);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) dp[e] = (*(const f32x4 *)&st[buf][1][2 * (e & ~3) + 4 * lh])[e & 3];
-#pragma unroll
-        for (int g = 0; g < NG; ++g)
-            dp = at_mma(tile::row(GO, lr, 2 * g + lh), VL ? *(const at_op<T> *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
-        AT_PRIO(0);
-        AT_PART(DP >= 64);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -(*(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh])[e & 3]));
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float ds = s[e] * dp[e];
-            if (MASK) {
-                const bool see = live && ((*(const u32x4 *)&mws[buf][wave][2 * (e & ~3) + 4 * lh])[e & 3] >> lr) & 1;
-                s[e] = see ? s[e] : 0.f;
-                ds = see ? ds : 0.f;
-            }
-            dp[e] = ds;
+        for (int i = 0; i < NB; ++i) ok[i] = ov[i] = (f32x16)(0.f);
+        if (w0 < w1) {
+            load();
+            store(0);
         }
-        AT_PRIO(1);
-        tile::acc_t(ov, GO, 0, s, ln);
-        tile::template acc_t<FINE>(ok, Q, 0, dp, ln);
-        AT_PRIO(0);
-        if (more) store(buf ^ 1);
+        __builtin_amdgcn_s_waitcnt(AT_VM0);           // what the loop keeps in registers has arrived: no turn of it waits for a load but its own
         __syncthreads();
-    }
-    if (key >= a.nk) return;
-    const int64_t rows = (int64_t)(gridDim.x / a.tiles / a.splits) * a.nk, prow = ((int64_t)b * a.hk + hk) * a.nk + key;
-    float *pk = a.part + prow * a.splits * a.d + (int64_t)sp * a.d, *pv = pk + rows * a.splits * a.d;
-    const int64_t orow = (((int64_t)b * a.nk + key) * a.hk + hk) * a.d;
+        int buf = 0;
+        for (int w = w0; w < w1; ++w, buf ^= 1) {
+            const bool more = w + 1 < w1;
+            if (more) load();
+            const char *Q = lds[buf][0], *GO = lds[buf][1];
+            // the LDS addresses of a tile are formed anew in every turn: kept across the loop they would cost a wave of the SIMD
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+            const int lr = ln & 31, lh = ln >> 5;
+            f32x16 s = (f32x16)(0.f), dp;
+            AT_PRIO(2);
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
+            for (int g = 0; g < NG; ++g) s = at_mma(tile::row(Q, lr, 2 * g + lh), kf[g], s);
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int d = i * 32 + 2 * e + 4 * h;
-            if (d >= a.d) continue;
-            f32x4 x = (f32x4){ok[i][e], ok[i][e + 1], ok[i][e + 2], ok[i][e + 3]} * a.scale, y = (f32x4){ov[i][e], ov[i][e + 1], ov[i][e + 2], ov[i][e + 3]};
-            if (!live) x = y = (f32x4)(0.f);
-            if (a.splits > 1) {
-                *(f32x4 *)(pk + d) = x;
-                *(f32x4 *)(pv + d) = y;
-            } else {
-                *(quad *)(a.dk + orow + d) = __builtin_convertvector(x, quad);
-                *(quad *)(a.dv + orow + d) = __builtin_convertvector(y, quad);
+            for (int e = 0; e < 16; ++e) dp[e] = (*(const f32x4 *)&st[buf][1][2 * (e & ~3) + 4 * lh])[e & 3];
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                dp = at_mma(tile::row(GO, lr, 2 * g + lh), VL ? *(const at_op<T> *)(vt + (wave * NG + g) * 1024 + ln * 16) : vf[VL ? 0 : g], dp);
+            AT_PRIO(0);
+            AT_PART(DP >= 64);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.c, -(*(const f32x4 *)&st[buf][0][2 * (e & ~3) + 4 * lh])[e & 3]));
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                float ds = s[e] * dp[e];
+                if (MASK) {
+                    const bool see = live && ((*(const u32x4 *)&mws[buf][wave][2 * (e & ~3) + 4 * lh])[e & 3] >> lr) & 1;
+                    s[e] = see ? s[e] : 0.f;
+                    ds = see ? ds : 0.f;
+                }
+                dp[e] = ds;
             }
+            AT_PRIO(1);
+            tile::acc_t(ov, GO, 0, s, ln);
+            tile::template acc_t<decltype(cut)::value>(ok, Q, 0, dp, ln);
+            AT_PRIO(0);
+            if (more) store(buf ^ 1);
+            __syncthreads();
         }
+        if (key >= a.nk) return;
+        const int64_t rows = (int64_t)(gridDim.x / a.tiles / a.splits) * a.nk, prow = ((int64_t)b * a.hk + hk) * a.nk + key;
+        float *pk = a.part + prow * a.splits * a.d + (int64_t)sp * a.d, *pv = pk + rows * a.splits * a.d;
+        const int64_t orow = (((int64_t)b * a.nk + key) * a.hk + hk) * a.d;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = i * 32 + 2 * e + 4 * h;
+                if (d >= a.d) continue;
+                f32x4 x = (f32x4){ok[i][e], ok[i][e + 1], ok[i][e + 2], ok[i][e + 3]} * a.scale, y = (f32x4){ov[i][e], ov[i][e + 1], ov[i][e + 2], ov[i][e + 3]};
+                if (!live) x = y = (f32x4)(0.f);
+                if (a.splits > 1) {
+                    *(f32x4 *)(pk + d) = x;
+                    *(f32x4 *)(pv + d) = y;
+                } else {
+                    *(quad *)(a.dk + orow + d) = __builtin_convertvector(x, quad);
+                    *(quad *)(a.dv + orow + d) = __builtin_convertvector(y, quad);
+                }
+            }
+    };
+    if (AT_CUT(nk)) walk(std::true_type());
+    else walk(std::false_type());
 }
 
 // sums a gradient's splits in their order: rows (b, h, n) of the partial sums -> (b, n, h); rows behind a count are left alone; a second
@@ -1055,10 +1067,10 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
     const at_plan p = at_plan_of(s);
     at_args<T> a = at_fill<T>(s, q, k, v, qc, kc);
     ws = at_bits(s, p, mask, a, ws, st);
-    constexpr int FINE = sizeof(T) == 2 ? AT_FINE : AT_PLAIN;
+    constexpr int FINE = sizeof(T) == 2 ? AT_FINE : AT_PLAIN, COUNTED = sizeof(T) == 2 ? AT_COUNTED : AT_PLAIN;
     // 16 x 500 rows and keys x 64: dq 36 -> 39 us, dk, dv 47 -> 51, for errors of dq, dk of 1.0 instead of 1.45 roundings of the result (2.3 at 10
     // keys of which a fifth is seen); 16000 x 128: dq 1575 -> 1980, dk, dv 2235 -> 2545, for 1.0 instead of 1.42
-    const bool fine = s->nk <= 512;
+    const bool fine = s->nk <= AT_FEW;
     f32x2 *stat = (f32x2 *)ws;
     a.g = (const T *)g; a.rest = (T *)rest; a.stat = stat; a.part = (float *)((char *)ws + p.stats);
     if (s->nq > 0) {
@@ -1073,6 +1085,7 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
         const int64_t grid = s->batch * s->k_heads * p.qtiles * p.qsplits;
         if (a.bits) AT_LAUNCH(k_attn_dq, AT_MASKED, grid, a);
         else if (fine) AT_LAUNCH(k_attn_dq, FINE, grid, a);
+        else if (kc) AT_LAUNCH(k_attn_dq, COUNTED, grid, a);
         else AT_LAUNCH(k_attn_dq, AT_PLAIN, grid, a);
         if (p.qsplits > 1)
             hipLaunchKernelGGL((k_attn_sum<T>), dim3((unsigned)dg_cdiv(p.rows * s->d / 4, AT_THREADS)), dim3(AT_THREADS), 0, st, (const float *)a.part, (T *)dq, (T *)nullptr, qc, p.rows,
@@ -1084,6 +1097,7 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
         const int64_t grid = s->batch * s->k_heads * p.ktiles * p.ksplits;
         if (a.bits) AT_LAUNCH(k_attn_dkv, AT_MASKED, grid, a);
         else if (fine) AT_LAUNCH(k_attn_dkv, FINE, grid, a);
+        else if (kc) AT_LAUNCH(k_attn_dkv, COUNTED, grid, a);
         else AT_LAUNCH(k_attn_dkv, AT_PLAIN, grid, a);
         if (p.ksplits > 1) {
             const int64_t rows = s->batch * s->k_heads * s->nk;
