@@ -35,3 +35,67 @@ def test_roi_attention_one_row_of_a_far_apart_bank(Nq, Nk, dtype):
         o, s = ops.roi_attention(a, b, c)
         assert torch.equal(o, out) and torch.equal(s, lse), far
         assert all(torch.equal(x, y) for x, y in zip(ops.roi_attention_backward(g, a, b, c, out, lse), grads)), far
+
+
+# ------------------------------------------------------------------ few keys under long padding
+@pytest.mark.gpu
+@pytest.mark.parametrize("Nk", [700, 2000])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_roi_attention_gradient_of_few_counted_keys(D, Nk):
+    """Images padded to more keys than those for which ds is cut in two by size alone: the count decides.  1, 3 and 7 keys of equal score:
+    p is 1 / n, the sum of ds over them 0, and dq, the sum of ds k over equal k, 0 too.  delta comes from out and its rest, 2^-16 of
+    |do| |out| apart, ds goes into its products as two parts, 2^-16 of it, and 32-bit sums of D terms add D 2^-24 of their
+    magnitudes.  The fourth image has all its keys, at the usual bounds."""
+    from vision_amd import fast_rcnn
+    N, u2, E32, counts = 150, 2.0 ** -16, 2.0 ** -24, (1, 3, 7, Nk)
+    q, k, v, do = _attn_inputs(81, 4, N, Nk, 2, 1, D, torch.bfloat16)
+    k[:3] = k[:3, :1]
+    kc = torch.tensor(counts).int()
+    want = _attn64(q[3:], k[3:], v[3:], None, None, None, None, do[3:])
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    dq, dk, dv = torch.autograd.grad(fast_rcnn.roi_attention(*leaves, k_counts=kc.cuda()), leaves, do.cuda())
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    for b, n in enumerate(counts[:3]):
+        V = v[b, :n, 0]
+        o = V.mean(0)
+        dp = do[b] @ V.T                             # (N, 2, n)
+        at = (do[b].abs() @ o.abs())[..., None]
+        ds = (dp - (do[b] @ o)[..., None]) / n
+        mag = do[b].abs() @ V.abs().T + at
+        eds = ds.abs() * (u2 + 16 * E32) + (at * u2 + (D + 8) * E32 * mag) / n + 8 * E32 * dp.abs() / n
+        sc = D ** -0.5
+        edq = (eds + n * E32 * ds.abs()).sum(-1, keepdim=True) * k[b, 0, 0].abs() * sc
+        _close(dq[b], (torch.zeros_like(q[b]), edq), ("dq", n))
+        wdk = torch.einsum("ihj,ihd->jd", ds, q[b]) * sc
+        edk = torch.einsum("ihj,ihd->jd", eds + 2 * N * E32 * ds.abs(), q[b].abs()) * sc + 2.0 ** -8 * wdk.abs()
+        _close(dk[b, :n, 0], (wdk, edk), ("dk", n))
+        assert float(dk[b, n:].abs().max()) == 0.0 and float(dv[b, n:].abs().max()) == 0.0
+    for got, name in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
+        _close(got[3:], want[name], name)
+
+
+# ------------------------------------------------------------------ long sums
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("above", [0.3, 1.0, 1.7])
+def test_roi_attention_long_sum_of_equal_scores(above, dtype):
+    """16001 keys of equal score behind a first one `above` them, enough rows that the walk is not split: the roundings of a sum of equal
+    terms do not average out.  lse: the terms share one relative error, of the score's product (3 units of 2^-24 of it: the query's value is
+    exact, scale, maximum and the rounding of the exponent's argument), and of the exponential (2); a tile's sum adds 5 levels, the
+    compensated sum over the tiles 4 and the two lanes 1; the logarithm 2 units of its value.  out, of equal values, is 1: numerator and
+    denominator each hold those errors, and the numerator's sum, which the matrix cores add up by 16 keys, at most 12 roundings a tile of 32
+    keys; at the end a division and the rounding to the type."""
+    from vision_amd import ops
+    B, N, M, H, D, E32 = 1, 4096, 16001, 8, 8, 2.0 ** -24
+    q, k = torch.zeros((B, N, H, D), dtype=dtype), torch.zeros((B, M, H, D), dtype=dtype)
+    q[..., 0] = 1.0
+    k[:, 0, :, 0] = above
+    v = torch.ones((B, M, H, D), dtype=dtype)
+    out, lse = ops.roi_attention(q.cuda(), k.cuda(), v.cuda(), scale=1.0)
+    s = float(k[0, 0, 0, 0])
+    want = math.log(math.exp(s) + (M - 1))
+    el = (3 * s + 2 + 5 + 4 + 1) * E32
+    err = float((lse.cpu().double() - want).abs().max())
+    assert err <= el + 2 * E32 * want, err / E32
+    eo = 12 * (M // 32 + 1) * E32 + 2 * el + 2 * E32 + (2.0 ** -8 + 2.0 ** -8 if dtype == torch.bfloat16 else E32)
+    assert float((out.cpu().double() - 1.0).abs().max()) <= eo

@@ -390,6 +390,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
 #pragma unroll
     for (int i = 0; i < NB; ++i) o[i] = (f32x16)(0.f);
     float m = -INFINITY, l = 0.f;                 // maximum in use (of s / scale, at most slack below the true one), this lane's part of the sum
+    float lost = 0.f;                             // what rounding added to l: see the end of a turn
 
     u32 mw[U], mnext[U];                          // MASK: this tile's words and the next one's
     if (k0 < k1) {
@@ -434,24 +435,31 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
         if (__any(mn > m + a.slack)) {            // otherwise the old maximum still does: no p exceeds 2^8
             const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
             l *= al;
+            lost *= al;
 #pragma unroll
             for (int i = 0; i < NB; ++i) o[i] *= al;
             m = mn;
         }
         AT_PART(DP == 128);
         const float base = m == -INFINITY ? 0.f : m * a.c;
+        f32x4 sum;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[u][e], a.c, -base));
                 s[u][e] = p;
-                l += p;
+                sum[e & 3] = u == 0 && e < 4 ? p : sum[e & 3] + p;
             }
             AT_PRIO(1);
             tile::acc_t(o, V, u * 32, s[u], lane);
             AT_PRIO(0);
         }
+        // A long walk over keys of like scores adds thousands of like values, whose roundings all point one way: a tile's are summed first,
+        // and what rounding did to l is taken from the next tile's sum (one by one: 7e-5 of l after 16000 keys, by tiles alone 6e-6, so 4e-8)
+        const float x = ((sum[0] + sum[1]) + (sum[2] + sum[3])) - lost, y = l + x;
+        lost = (y - l) - x;
+        l = y;
         if (more) store(buf ^ 1);
 #pragma unroll
         for (int u = 0; u < U; ++u) mw[u] = mnext[u];
