@@ -99,3 +99,30 @@ def test_roi_attention_long_sum_of_equal_scores(above, dtype):
     assert err <= el + 2 * E32 * want, err / E32
     eo = 12 * (M // 32 + 1) * E32 + 2 * el + 2 * E32 + (2.0 ** -8 + 2.0 ** -8 if dtype == torch.bfloat16 else E32)
     assert float((out.cpu().double() - 1.0).abs().max()) <= eo
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,c", [(4096, 131072), (300, 1000003), (300, 131072), (1, 131072)])
+def test_class_logprobs_long_sum_of_equal_scores(n, c, dtype):
+    """1024 equal scores before many equal lower ones, so that every lane's sum starts from a maximum above the rest.  The terms share one
+    relative error, of the exponent's argument (its size) and of the exponential (2 units of 2^-24); a turn's sum of sixteen adds 16,
+    sixteen turns 16, the sums put away one each (a wave alone takes 16384 scores for one, four waves four times as many), lanes,
+    waves and splits at most 8 joins of 2; log probabilities add 2 units of the logarithm's and their own size, the entropy as much of its
+    two terms."""
+    from vision_amd import ops
+    E32 = 2.0 ** -24
+    for above in (0.3, 1.0, 1.7):
+        z = torch.zeros((n, c), dtype=dtype, device="cuda")
+        z[:, :1024] = above
+        s = float(z[0, 0])
+        y = torch.arange(n, device="cuda") % 2 * (c - 1)                      # the first class or the last
+        logp, entropy, _, _, _ = ops.class_logprobs(z, y)
+        del z
+        L = math.log(1024 * math.exp(s) + c - 1024)
+        H = -(1024 * math.exp(s - L) * (s - L) - (c - 1024) * math.exp(-L) * L)
+        es = (s + 2 + 16 + 16 + c / 16384 + 16) * E32
+        want = torch.where(y == 0, s - L, -L).double()
+        assert float(((logp.double() - want).abs() - (es + 2 * E32 * (L - s + want.abs()))).max()) <= 0.0, above
+        spread = (c - 1024) * math.exp(-L) * s                                # w / s of the kernel's formula
+        assert float((entropy.double() - H).abs().max()) <= es + 2 * E32 * (L - s) + spread * (2 * es + 4 * E32) + E32 * H, above

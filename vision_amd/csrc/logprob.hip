@@ -77,17 +77,33 @@ struct lp_list {
     }
 };
 
-// statistics of a set of scores: maximum, sum of e^(z-m), sum of e^(z-m) (z-m)
+// statistics of a set of scores: maximum, sum of e^(z-m), sum of e^(z-m) (z-m); far: the part of the sums that has been put away.  The
+// roundings of a sum of thousands of like terms all point one way (131072 classes in one sum a lane: 2e-5 of a log probability was
+// lost), so a walk adds a turn's terms up first and puts sixteen turns away together.
 struct lp_sum {
-    float m = -INFINITY, s = 0.f, w = 0.f;
+    float m = -INFINITY, s = 0.f, w = 0.f, far_s = 0.f, far_w = 0.f;
     __device__ __forceinline__ void raise(float mx)
     {
         if (mx > m) {
             const float d = m - mx, f = __builtin_amdgcn_exp2f(d * LP_LOG2E);
             w = f == 0.f ? 0.f : f * fmaf(s, d, w);
             s *= f;
+            far_w = f == 0.f ? 0.f : f * fmaf(far_s, d, far_w);
+            far_s *= f;
             m = mx;
         }
+    }
+    __device__ __forceinline__ void put_away()
+    {
+        far_s += s;
+        far_w += w;
+        s = w = 0.f;
+    }
+    __device__ __forceinline__ void take_back()
+    {
+        s += far_s;
+        w += far_w;
+        far_s = far_w = 0.f;
     }
     __device__ __forceinline__ float from() const { return m == -INFINITY ? 0.f : m; }
     __device__ __forceinline__ void add(float z, float from)  // z <= m, or NaN
@@ -268,10 +284,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 8 : 6)) void k_logprob_walk(
         fetch(p0 + 64 * WPR * UN);
         t.raise(mx);
         const float from = t.from();
+        lp_sum turn;
 #pragma unroll
         for (int u = 0; u < UN; ++u)
 #pragma unroll
-            for (int e = 0; e < V; ++e) t.add(v[u][e], from);
+            for (int e = 0; e < V; ++e) turn.add(v[u][e], from);
+        t.s += turn.s;
+        t.w += turn.w;
+        if ((p0 & (64 * WPR * UN * 15)) == 64 * WPR * UN * 15) t.put_away();
         if (!keep) continue;
         // A score enters the list only from `least` on: the keep-th best so far, or, before there is a list, the keep-th largest of
         // the lanes' maxima -- which leaves little more than the best themselves to be sorted in, not the first ones met.
@@ -292,6 +312,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 ? 8 : 6)) void k_logprob_walk(
         }
     }
     if (wave == 0 || WPR == 1) single(b1, c1);    // in the order of the classes: an equal score that comes later never ranks before
+    t.take_back();
     t.join_lanes<64>();
     if (WPR == 4) {
         if (lane == 0) { sums[wave][0] = t.m; sums[wave][1] = t.s; sums[wave][2] = t.w; }
