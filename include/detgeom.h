@@ -343,7 +343,7 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
  * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products, in DG_F32 products
  * are formed from three bf16 parts of each operand, which keeps their 24 bits; a DG_F32 value of 3.39e38 or more counts as infinite.
- * rest (like out, bf16; may be NULL; DG_BF16 only): what rounding took from out, for the backward pass, whose delta is a sum of products
+ * rest (like out, bf16; may be NULL; refused in DG_F32): what rounding took from out, for the backward pass, whose delta is a sum of products
  * with out that cancels where a row sees few keys: without it dq and dk are off by up to 2^-8 of the terms of that sum.
  * Results are the same in every run (no atomics). */
 typedef struct dg_attn_shape {   /* host */

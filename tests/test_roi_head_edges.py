@@ -126,3 +126,21 @@ def test_class_logprobs_long_sum_of_equal_scores(n, c, dtype):
         assert float(((logp.double() - want).abs() - (es + 2 * E32 * (L - s + want.abs()))).max()) <= 0.0, above
         spread = (c - 1024) * math.exp(-L) * s                                # w / s of the kernel's formula
         assert float((entropy.double() - H).abs().max()) <= es + 2 * E32 * (L - s) + spread * (2 * es + 4 * E32) + E32 * H, above
+
+
+# ------------------------------------------------------------------ refusals
+def test_rest_of_float32_is_refused():
+    """On the host, before any launch: rest is of bf16, and a DG_F32 call that took it would clear padded rows at twice its size."""
+    import ctypes as C
+    from vision_amd import _abi
+    lib = _abi.load()
+    s = _abi.AttnShape(1, 8, 8, 1, 1, 64)
+    for t in "qkvg":
+        for a, n in (("batch", 512), ("row", 64), ("head", 64)):
+            setattr(s, f"{t}_stride_{a}", n)
+    s.scale, s.dtype = 0.125, _abi.F32
+    p = C.c_void_p(4096)                         # never touched: the calls end before a launch
+    assert lib.dg_roi_attn_fwd(s, p, p, p, None, None, None, p, p, p, p, 1 << 30, None) == _abi.EINVAL
+    assert "rest" in _abi.last_error()
+    assert lib.dg_roi_attn_bwd(s, p, p, p, p, p, p, p, None, None, None, p, p, p, p, 1 << 30, None) == _abi.EINVAL
+    assert "rest" in _abi.last_error()

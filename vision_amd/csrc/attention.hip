@@ -350,7 +350,7 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd
             T *o = a.o + (((int64_t)b * a.nq + n) * a.hq + hq) * a.d;
             for (int d = threadIdx.x; d < a.d; d += AT_THREADS) {
                 o[d] = (T)0.f;
-                if (a.rest) a.rest[o - a.o + d] = (T)0.f;
+                if (sizeof(T) == 2 && a.rest) a.rest[o - a.o + d] = (T)0.f;
             }
             if (threadIdx.x == 0) a.lse[((int64_t)b * a.hq + hq) * a.nq + n] = -INFINITY;
         }
@@ -1059,6 +1059,7 @@ extern "C" int dg_roi_attn_fwd(const dg_attn_shape *s, const void *q, const void
     if (rc != DG_OK) return rc;
     if (s->batch == 0 || s->nq == 0) return DG_OK;
     DG_REQUIRE(q && out && lse && (s->nk == 0 || (k && v && !mask == !s->masks)), "roi_attn_fwd: null pointer");
+    DG_REQUIRE(!rest || s->dtype == DG_BF16, "roi_attn_fwd: rest is for DG_BF16 only");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && ((((uintptr_t)out) | ((uintptr_t)rest)) & 15) == 0, "roi_attn_fwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
     const size_t need = dg_roi_attn_workspace_bytes(s, 0);
@@ -1125,6 +1126,7 @@ extern "C" int dg_roi_attn_bwd(const dg_attn_shape *s, const void *grad_out, con
     if (rc != DG_OK) return rc;
     if (s->batch == 0 || (s->nq == 0 && s->nk == 0)) return DG_OK;
     DG_REQUIRE((s->nq == 0 || (grad_out && q && out && lse)) && (s->nk == 0 || (k && v)) && !dk == !dv && (s->nk == 0 || s->nq == 0 || !mask == !s->masks), "roi_attn_bwd: null pointer");
+    DG_REQUIRE(!rest || s->dtype == DG_BF16, "roi_attn_bwd: rest is for DG_BF16 only");
     DG_REQUIRE(at_aligned(q, s->q_stride, s, s->nq, s->q_heads) && at_aligned(k, s->k_stride, s, s->nk, s->k_heads) &&
                    at_aligned(v, s->v_stride, s, s->nk, s->k_heads) && at_aligned(grad_out, s->g_stride, s, s->nq, s->q_heads) &&
                    ((((uintptr_t)out) | ((uintptr_t)rest) | ((uintptr_t)dq) | ((uintptr_t)dk) | ((uintptr_t)dv)) & 15) == 0, "roi_attn_bwd: pointers and strides must be multiples of 16 bytes, rows at most 2^22 values apart");
