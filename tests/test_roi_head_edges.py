@@ -144,3 +144,37 @@ def test_rest_of_float32_is_refused():
     assert "rest" in _abi.last_error()
     assert lib.dg_roi_attn_bwd(s, p, p, p, p, p, p, p, None, None, None, p, p, p, p, 1 << 30, None) == _abi.EINVAL
     assert "rest" in _abi.last_error()
+
+
+# ------------------------------------------------------------------ walks that are not split, many images
+def _both(case, dtype, seed, qc, kc, mask=None):
+    from vision_amd import ops
+    q, k, v, do = _attn_inputs(seed, *case, dtype)
+    want = _attn64(q, k, v, qc, kc, mask, None, do)
+    Q, K, V, G, QC, KC, M = (None if t is None else t.cuda() for t in (q, k, v, do, qc, kc, mask))
+    out, lse, rest = ops.roi_attention(Q, K, V, QC, KC, M, rest=True)
+    _close(out, want["out"], "out")
+    _close(lse, want["lse"], "lse")
+    for name, got in zip(("dq", "dk", "dv"), ops.roi_attention_backward(G, Q, K, V, out, lse, QC, KC, M, rest=rest)):
+        _close(got, want[name], name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,dtype", [(32, torch.bfloat16), (64, torch.bfloat16), (128, torch.bfloat16), (64, torch.float32)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_roi_attention_walks_that_are_not_split(D, dtype, ragged):
+    """256 tiles of rows and of keys and more: every workgroup walks all of its image, the maximum is renewed on the way, images and
+    heads go round the compute dies; ragged: one image of few keys, one of few rows, one of all."""
+    q, k = (torch.tensor([1900, 130, 1333]).int(), torch.tensor([300, 1900, 1200]).int()) if ragged else (None, None)
+    _both((3, 1900, 1900, 6, 6, D), dtype, 71, q, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("masked", [False, True])
+def test_roi_attention_many_images(masked, dtype):
+    """More images than a wave has lanes, which are taken in their own order; some without rows or keys."""
+    g = _gen(73)
+    B, Nq, Nk = 70, 45, 150
+    q, k = torch.randint(0, Nq + 1, (B,), generator=g).int(), torch.randint(0, Nk + 1, (B,), generator=g).int()
+    _both((B, Nq, Nk, 4, 2, 40), dtype, 72, q, k, torch.rand((B, Nq, Nk), generator=g) < 0.4 if masked else None)
