@@ -178,3 +178,12 @@ def test_roi_attention_many_images(masked, dtype):
     B, Nq, Nk = 70, 45, 150
     q, k = torch.randint(0, Nq + 1, (B,), generator=g).int(), torch.randint(0, Nk + 1, (B,), generator=g).int()
     _both((B, Nq, Nk, 4, 2, 40), dtype, 72, q, k, torch.rand((B, Nq, Nk), generator=g) < 0.4 if masked else None)
+
+
+@pytest.mark.gpu
+def test_heads_of_no_size_are_refused():
+    from vision_amd import fast_rcnn, ops
+    q, k = torch.zeros((1, 3, 2, 0), device="cuda"), torch.zeros((1, 4, 2, 0), device="cuda")
+    for call in (lambda: ops.roi_attention(q, k, k), lambda: fast_rcnn.roi_attention(q, k, k)):
+        with pytest.raises(ValueError, match="head size"):
+            call()

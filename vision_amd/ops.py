@@ -420,7 +420,7 @@ def _attn_plan(q_shape, k_shape, q_stride, k_stride, v_stride, g_stride, masks, 
     dense = [(shape[1] * shape[2] * D, shape[2] * D, D) for shape in (q_shape, k_shape)]
     strides = [(d if st is None else st)[:3] for st, d in ((q_stride, dense[0]), (k_stride, dense[1]), (v_stride, dense[1]), (g_stride, dense[0]))]
     s = _abi.AttnShape(B, Nq, k_shape[1], Hq, k_shape[2], D, *strides[0], *strides[1], *strides[2], *strides[3], masks, *mask_stride[:2],
-                       D ** -0.5 if scale is None else scale, _abi.TYPES[dtype])
+                       max(D, 1) ** -0.5 if scale is None else scale, _abi.TYPES[dtype])
     return s, load().dg_roi_attn_workspace_bytes(s, backward)
 
 
