@@ -339,7 +339,8 @@ int dg_voc_ap_f32(const int32_t *det_img, const float *det_box, const int32_t *o
  * (device bytes, a row's keys dense, strides of image and row in bytes; shape->masks of them, NULL with 0 = all).  What lies behind a count is
  * never read.  A row that sees nothing gives out = 0, lse = -inf and has no gradient; so do the rows behind q_counts, and dk = dv = 0
  * behind k_counts: every element of every output is written.  A pair that a count or a mask excludes adds nothing, whatever its values
- * are.  A NaN or an infinity in what a row does see makes that row's results NaN or infinite, and with a mask NaN.
+ * are.  A NaN or an infinity in what a row does see makes that row's results NaN or infinite, and with a mask NaN; but in DG_BF16 an infinity in
+ * q or k that makes a score -inf gives that pair no weight in out and lse (a row of such scores alone: out 0, lse -inf).
  * out (batch, nq, q_heads, d), dq, dk, dv like q, k, v: dense; lse (batch, q_heads, nq) fp32.  Sums, maxima and log-sums are held in
  * 32 bits; in DG_BF16 the probabilities and their gradients are rounded to bf16 as operands of the matrix products, in DG_F32 products
  * are formed from three bf16 parts of each operand, which keeps their 24 bits; a DG_F32 value of 3.39e38 or more counts as infinite.
