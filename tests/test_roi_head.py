@@ -4,6 +4,7 @@ positions over several axes, log probabilities of labels.
 Tolerances.  One rounding to a type moves a value by at most half a step, u = 2^-8 of it in bf16, 2^-11 in fp16, 2^-24 in fp32.
 Attention in bf16: p (and ds) is rounded once as an operand, the result once at the end, so an output element is off by at most
 u sum |p_ij v_j| + u |o_i|, and the sum itself is held in 32 bits; delta is formed from the rounded out (u |do| |out| per row).
+(Without the forward's rest, that is; with it delta is off by 2^-16 of its terms.)
 Each bound below is such a sum of magnitudes, formed in 64 bits from the same inputs, plus the 32-bit terms: a product of d
 terms is off by at most d 2^-24 sum |q k| scale, which moves p by that factor."""
 import math

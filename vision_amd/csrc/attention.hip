@@ -327,10 +327,11 @@ template <typename T, int DP> struct at_shape {
 
 // A workgroup: 128 rows (a wave: 32, one per lane pair), all keys of its split in tiles of KT.  K and V tiles are double buffered
 // in LDS; the next tile's loads are on their way while this one is computed.  Per 32 x 32 scores a wave spends 8 d / 64 matrix
-// instructions of 32 cycles and about 110 vector instructions (scale, exponential, sum, maximum, rounding): the vector unit bounds
-// 64 values a head, both units together 128.  Measured, bf16: 16 x 2000 rows and keys, 8 heads of 64: 170 us, 771 TFLOP/s; 16000, 8
-// heads of 128: 1040 us, 1008 TFLOP/s (a large matrix product reaches 1195); fp32, 8 x 2000, 8 heads of 64: 355 us,
-// 185 TFLOP/s (a library's matrix product of 32 bits: 153; by 32-bit matrix instructions it took 590).
+// instructions of 32 cycles and about 90 vector instructions (scale, exponential, sum, maximum, rounding; the 16 exponentials at a
+// quarter of the others' rate).  With 64 values a head the vector unit is busy 67% of the time and the matrix unit 32%, with 128 48%
+// and 49%: they take turns, and neither alone is the bound.  Measured, bf16: 16 x 2000 rows and keys, 8 heads of 64: 172 us, 762
+// TFLOP/s; 16000, 8 heads of 128: 1050 us, 999 TFLOP/s (a large matrix product reaches 1195); fp32, 8 x 2000, 8 heads of 64: 339 us,
+// 193 TFLOP/s (a library's matrix product of 32 bits: 153; by 32-bit matrix instructions it took 590).
 template <typename T, int DP, bool MASK>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC)) void k_attn_fwd(const at_args<T> a)
 {
@@ -602,8 +603,9 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_delta(const at_args<T> a, c
 }
 
 // dq: a workgroup owns 128 rows and walks the keys as the forward does; K is read as rows (scores) and transposed (dq), V as rows (dp).
-// Three products a tile.  Measured, bf16: 16 x 2000, 8 heads of 64: 247 us, 796 TFLOP/s; 16000, 8 heads of 128: 1511 us, 1041 TFLOP/s;
-// fp32, 8 x 2000, 8 heads of 64: 480 us, 205 TFLOP/s (by 32-bit matrix instructions 810).
+// Three products a tile.  Measured, bf16: 16 x 2000, 8 heads of 64: 247 us, 796 TFLOP/s; 16000, 8 heads of 128: 1491 us, 1055 TFLOP/s;
+// fp32, 8 x 2000, 8 heads of 64: 464 us, 212 TFLOP/s (by 32-bit matrix instructions 810).  About 120 vector instructions a tile, of which
+// some 45 select by the keys' end, which only the last tile needs; busy 57% of the time at 64, the matrix unit 33%.
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_dq(const at_args<T> a)
 {
@@ -729,8 +731,8 @@ __global__ __launch_bounds__(AT_THREADS, (at_shape<T, DP>::OCC_Q)) void k_attn_d
 #define AT_RT 32
 // dk, dv: a workgroup owns 128 keys (a wave: 32, one per lane pair) and walks the rows; Q and dO tiles are read as rows (scores,
 // dp) and transposed (dk, dv).  Four products a tile, and 2 x 32 x d accumulators a wave, which bound how many waves share a SIMD.
-// Measured, bf16: 16 x 2000, 8 heads of 64: 408 us, 642 TFLOP/s; 16000, 8 heads of 128: 2140 us, 980 TFLOP/s; fp32, 8 x 2000, 8 heads of
-// 64: 630 us, 208 TFLOP/s (by 32-bit matrix instructions 1084).
+// Measured, bf16: 16 x 2000, 8 heads of 64: 359 us, 730 TFLOP/s; 16000, 8 heads of 128: 2135 us, 982 TFLOP/s; fp32, 8 x 2000, 8 heads of
+// 64: 614 us, 213 TFLOP/s (by 32-bit matrix instructions 1084).  About 150 vector instructions a tile at 64, half of them addresses.
 template <typename T, int DP, int MODE>
 __global__ __launch_bounds__(AT_THREADS, (MODE == AT_MASKED && at_shape<T, DP>::OCC_KV == 3 ? 2 : at_shape<T, DP>::OCC_KV)) void k_attn_dkv(const at_args<T> a)
 {
@@ -925,7 +927,7 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_bits(const uint8_t *__restr
 
 // ------------------------------------------------------------------ host
 // A call that has too few tiles to fill the chip is split along the axis it walks: enough splits for two workgroups on each of
-// the 256 CUs, none shorter than 128 steps of that axis.
+// the 256 CUs, of 128 steps of that axis or more (a multiple of 64); the last one takes what is left, a single step at the least.
 static void at_split(int64_t blocks, int64_t walk, int64_t *splits, int64_t *per)
 {
     int64_t s = 1;
@@ -1078,7 +1080,8 @@ static int at_backward(const dg_attn_shape *s, const void *g, const void *q, con
     ws = at_bits(s, p, mask, a, ws, st);
     constexpr int FINE = sizeof(T) == 2 ? AT_FINE : AT_PLAIN, COUNTED = sizeof(T) == 2 ? AT_COUNTED : AT_PLAIN;
     // 16 x 500 rows and keys x 64: dq 36 -> 39 us, dk, dv 47 -> 51, for errors of dq, dk of 1.0 instead of 1.45 roundings of the result (2.3 at 10
-    // keys of which a fifth is seen); 16000 x 128: dq 1575 -> 1980, dk, dv 2235 -> 2545, for 1.0 instead of 1.42
+    // keys of which a fifth is seen); 16000 x 128: dq 1575 -> 1980, dk, dv 2235 -> 2545, for 1.0 instead of 1.42.  Both walks in one kernel, by
+    // count: 8 x 2000 to 1900 x 64 dq 121 -> 118, dk, dv 150 -> 152 (with delta); 4 x 4000 x 128 289 -> 287, 486 -> 497
     const bool fine = s->nk <= AT_FEW;
     f32x2 *stat = (f32x2 *)ws;
     a.g = (const T *)g; a.rest = (T *)rest; a.stat = stat; a.part = (float *)((char *)ws + p.stats);

@@ -222,8 +222,8 @@ __device__ __forceinline__ void lp_best(const lp_args &a, int64_t row, const lp_
     }
 }
 
-// 8192 x 20011 bf16: 85 us, 3.9 TB/s (maximum, three sums and the comparisons, about ten operations a score, bound it); 4096 x 32000
-// fp32: 98 us, 5.3 TB/s, the rate of a copy.  Sixteen scores a lane and turn: with 32 of them fewer waves fit (100 us).
+// 8192 x 20011 bf16: 87 us, 3.8 TB/s (maximum, three sums and the comparisons, about ten operations a score, bound it); 4096 x 32000
+// fp32: 99 us, 5.3 TB/s, the rate of a copy.  Sixteen scores a lane and turn: with 32 of them fewer waves fit (100 us).
 // WPR waves walk one row's split (4: a workgroup, 1: each wave a row of its own).  Scores come 16 bytes at a time from the first
 // aligned one on; the few before and behind are single loads.
 template <typename T, int WPR>
@@ -427,7 +427,8 @@ static int lp_check(int64_t n, int64_t c, int64_t stride, int dtype, int64_t top
     return DG_OK;
 }
 
-// rows that are too few to fill the chip are split over their classes, 4096 of them at least, 256 workgroups' worth
+// rows that are too few to fill the chip are split over their classes, 512 workgroups' worth but one split for 4096 classes at most: 2112
+// classes or more each (a multiple of 64), the last one what is left, a single class at the least
 static void lp_split(int64_t n, int64_t c, int64_t *splits, int64_t *per)
 {
     int64_t s = n > 0 && n < 256 ? dg_cdiv(512, n) : 1;
